@@ -779,6 +779,86 @@ int b2f_router_logits(const void* x, int64_t T, int64_t H, const void* wr, const
 /* Greedy next token: out[m] = argmax_v x[m, v] (ties to the lower index). */
 int b2f_argmax_rows(const void* x, int64_t M, int64_t V, int32_t* out, void* stream);
 
+/* ---- packed prompts and shared prefixes over the paged KV cache --------- */
+
+/* Workspace bytes of b2f_page_plan for B requests (0 up to 2048). */
+int64_t b2f_page_plan_workspace_bytes(int64_t B);
+
+/* Block tables, slot map and positions of a batch from its lengths, without
+ * a host round trip.  Request b holds context_lens[b] tokens (NULL: none) in
+ * the first ceil(context/page_size) entries of block_table row b and gets
+ * new_lens[b] more; pages are taken from free_pages[0..n_free) in request
+ * order and written to the entries that follow.  Other entries stay.
+ * Token t of the packed batch (requests back to back) gets its request
+ * rows[t], its position in the request, and its slot page*page_size +
+ * position % page_size.  Tokens past the batch's sum: row -1, position 0,
+ * slot -1; tokens past T are not written.  Where the free list or the table
+ * row is too short the entry is -1 (or dropped) and the slots -1.
+ * cu_seqlens int32 [B+1], seq_lens int32 [B] (context + new), counts int32
+ * [2] = tokens in the batch, pages that the batch needs (more than n_free:
+ * the list was too short).  new_lens sums below 2^31; negative lengths count
+ * as 0.  positions, slots and rows 16-byte aligned. */
+int b2f_page_plan(const int32_t* new_lens, const int32_t* context_lens, int64_t B,
+                  const int32_t* free_pages, int64_t n_free, int64_t page_size, int32_t* block_table,
+                  int64_t max_pages, int64_t T, int32_t* cu_seqlens, int32_t* positions,
+                  int64_t* slots, int32_t* rows, int32_t* seq_lens, int32_t* counts,
+                  void* workspace, int64_t workspace_bytes, void* stream);
+
+/* Per-head RMSNorm + rotary position of packed rows qkv [T, >= (Hq+2Hkv)*D]
+ * (`dtype` bf16 or f16, ld elements between rows, rows [q | k | v]) into
+ * q_out [T, Hq, D] and k_out [T, Hkv, D]: float32 inside, one rounding.
+ * The first rotary_dim values of a head (a multiple of 16, 0: none) turn by
+ * positions[t] * inv_freq[i] in halves (i, i + rotary_dim/2); inv_freq is a
+ * device array of rotary_dim/2 doubles.  D in {64, 128, 256}.
+ * With slots (int64 [T], page*page_size + slot, -1: skip the row) the K rows
+ * and the V rows of qkv are also quantized (KV-SYM, group 64, `bits`) into
+ * head-major pages [page][Hkv][slot], the bytes b2f_kv_quantize_sym writes. */
+int b2f_qk_norm_rope_rows(const void* qkv, int64_t ld, int dtype, int64_t T, int64_t Hq, int64_t Hkv,
+                          int64_t D, const void* q_norm, const void* k_norm, float eps,
+                          const double* inv_freq, int64_t rotary_dim, const int32_t* positions,
+                          void* q_out, void* k_out, const int64_t* slots, uint8_t* k_codes,
+                          float* k_scales, uint8_t* v_codes, float* v_scales, int64_t page_size,
+                          int bits, void* stream);
+
+/* Attention of packed sequences over themselves: q [T, Hq, D], k and v
+ * [T, Hkv, D] of `dtype` (bf16 or f16) with the given row and head strides in
+ * elements (multiples of 8; the last axis is dense); sequence b is rows
+ * [cu_seqlens[b], cu_seqlens[b+1]) (int32 [B+1], from 0, at most T).  With
+ * causal, a row sees its sequence up to itself.  out [T, Hq, D] of `dtype`;
+ * rows past the last sequence are 0.  lse (float32 [T, Hq] or NULL): natural
+ * log of each row's sum of exp(score), -inf where a row sees nothing.
+ * D a multiple of 8 up to 128; Hq/Hkv up to 128. */
+int b2f_prompt_attn(const void* q, int64_t q_row, int64_t q_head, const void* k, int64_t k_row,
+                    int64_t k_head, const void* v, int64_t v_row, int64_t v_head, int dtype,
+                    const int32_t* cu_seqlens, int64_t B, int64_t T, int64_t Hq, int64_t Hkv,
+                    int64_t D, int causal, float softmax_scale, void* out, float* lse,
+                    void* stream);
+
+/* Workspace bytes of b2f_shared_prefix_attn. */
+int64_t b2f_shared_prefix_attn_workspace_bytes(int64_t B, int64_t Hq, int64_t Hkv, int64_t D,
+                                               int64_t n_groups, int64_t max_prefix,
+                                               int64_t max_own);
+
+/* Decode attention of B requests (q bf16 [B, Hq, D], one token each) over
+ * head-major KV-SYM pages, where rows [group_offsets[g], group_offsets[g+1])
+ * share the prefix of prefix_lens[g] tokens in the pages prefix_table[g, :]
+ * and request b continues with its own seq_lens[b] tokens in block_table
+ * [b, :].  Group offsets rise and stay within [0, B]; a row of no group has
+ * no prefix.  A prefix is read and decoded once for its group.  out bf16
+ * [B, Hq, D]; a row that sees nothing is 0.  max_prefix / max_own: upper
+ * bounds of the lengths (they size the splits; longer lengths are cut).
+ * D in {64, 128}; bits in {2, 4, 8}; group_size 64; Hq/Hkv <= 16; page_size
+ * a multiple of 16. */
+int b2f_shared_prefix_attn(const void* q, const uint8_t* k_pages, const float* k_scales,
+                           const uint8_t* v_pages, const float* v_scales,
+                           const int32_t* prefix_table, int64_t prefix_pages,
+                           const int32_t* prefix_lens, const int32_t* group_offsets,
+                           int64_t n_groups, const int32_t* block_table, int64_t max_pages,
+                           const int32_t* seq_lens, int64_t B, int64_t Hq, int64_t Hkv, int64_t D,
+                           int64_t page_size, int bits, int group_size, float softmax_scale,
+                           int64_t max_prefix, int64_t max_own, void* workspace,
+                           int64_t workspace_bytes, void* out, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

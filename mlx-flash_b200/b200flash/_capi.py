@@ -126,6 +126,15 @@ SIGNATURES = {
     "b2f_ep_a2a_plan": (_I, [_P, _I64, _I64, _I64, _I64, _I, _P, _P, _P, _P, _I64, _P, _P]),
     "b2f_ep_a2a_combine": (_I, [_P, _I64, _P, _I64, _I64, _I64, _P, _P, _I64, _P]),
     "b2f_argmax_rows": (_I, [_P, _I64, _I64, _P, _P]),
+    "b2f_page_plan_workspace_bytes": (_I64, [_I64]),
+    "b2f_page_plan": (_I, [_P, _P, _I64, _P, _I64, _I64, _P, _I64, _I64, _P, _P, _P, _P, _P, _P, _P, _I64, _P]),
+    "b2f_qk_norm_rope_rows": (_I, [_P, _I64, _I, _I64, _I64, _I64, _I64, _P, _P, _F, _P, _I64, _P, _P, _P, _P, _P, _P,
+                                   _P, _P, _I64, _I, _P]),
+    "b2f_prompt_attn": (_I, [_P, _I64, _I64, _P, _I64, _I64, _P, _I64, _I64, _I, _P, _I64, _I64, _I64, _I64, _I64, _I,
+                             _F, _P, _P, _P]),
+    "b2f_shared_prefix_attn_workspace_bytes": (_I64, [_I64, _I64, _I64, _I64, _I64, _I64, _I64]),
+    "b2f_shared_prefix_attn": (_I, [_P, _P, _P, _P, _P, _P, _I64, _P, _P, _I64, _P, _I64, _P, _I64, _I64, _I64, _I64,
+                                    _I64, _I, _I, _F, _I64, _I64, _P, _I64, _P, _P]),
 }
 
 _lib = None
