@@ -114,6 +114,12 @@ __device__ __forceinline__ float warp_sum(float v) {
   return v;
 }
 
+// 2^-floor(log2 x) * 2^shift for finite x > 0, else 1
+__device__ __forceinline__ float pow2_inverse(float x, int shift) {
+  const int e = int(__float_as_uint(x) >> 23) - 127;
+  return x > 0.f && x < INFINITY ? __uint_as_float(uint32_t(127 + max(-126, min(126, shift - e))) << 23) : 1.f;
+}
+
 // ---- bit helpers -------------------------------------------------------
 // lop3: (a & b) | c
 __device__ __forceinline__ uint32_t and_or(uint32_t a, uint32_t b, uint32_t c) {

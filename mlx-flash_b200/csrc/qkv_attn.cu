@@ -38,7 +38,27 @@ struct AttnParams {
   __nv_bfloat16* out;
   int ring_bytes;  // ring path: shared-memory bytes of the page ring (the merge area follows)
   int slot_bytes;  // ring path: bytes of one ring slot
+  // PART kernels only: where the partials of this call's splits go, the
+  // longest sequence read
+  int part_stride, part_base, max_len;
 };
+
+// The kernels' PART form writes partials for a combine with other splits of
+// the same rows (prefix_attn.cu), whatever n_splits is, and takes q and V of
+// any magnitude: query rows are scaled into fp16 by a power of two from their
+// absmax, V scales by one from the split's first token; both are undone in
+// float32.
+__device__ __forceinline__ float v_reference(const AttnParams& p, int b, int hkv, int token, int DG, int shift) {
+  const int page = p.block_table[int64_t(b) * p.max_pages + token / p.PS];
+  const int64_t row = int64_t(page) * p.Hkv * p.PS + hkv * p.head_stride + (token % p.PS) * p.slot_stride;
+  float top = 0.f;
+  for (int g = 0; g < DG; ++g) top = fmaxf(top, p.vs[row * DG + g]);
+  return pow2_inverse(top, shift);
+}
+__device__ __forceinline__ float scaled_up_to(float s, float f, float top) {
+  const float x = s * f;
+  return x > top ? top : x;  // NaN stays
+}
 
 // Named barrier `id` over the first `n` threads of the CTA.
 __device__ __forceinline__ void named_bar_sync(int id, int n) {
@@ -66,7 +86,7 @@ __device__ __forceinline__ uint32_t hmul2_u(uint32_t a, uint32_t b) {
 }
 __device__ __forceinline__ float round_f16(float v) { return __half2float(__float2half_rn(v)); }
 
-template <int BITS, int D, bool RING>
+template <int BITS, int D, bool RING, bool PART = false>
 __global__ void __launch_bounds__(RING ? 160 : 128) qkv_decode_attn_kernel(const AttnParams p,
                                                                          const __grid_constant__ CUtensorMap tmk,
                                                                          const __grid_constant__ CUtensorMap tmv) {
@@ -84,7 +104,7 @@ __global__ void __launch_bounds__(RING ? 160 : 128) qkv_decode_attn_kernel(const
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int r = lane >> 2, c = lane & 3;
   const int G = p.G;
-  const int len = p.seq_lens[b];
+  const int len = PART ? min(max(p.seq_lens[b], 0), p.max_len) : p.seq_lens[b];
   const int n_sub = (len + 15) / 16;
   const int per_split = (n_sub + p.n_splits - 1) / p.n_splits;
   const int sub_begin = split * per_split;
@@ -93,11 +113,23 @@ __global__ void __launch_bounds__(RING ? 160 : 128) qkv_decode_attn_kernel(const
   // ---- Q fragments (fp16, pre-scaled) and per-group sums of q -----------
   uint32_t qa[KSTEPS][4];
   float qg[2][DG];
+  float hs[2];  // PART: scores = S * hs
+  const float vn = PART && sub_begin < sub_end ? v_reference(p, b, hkv, sub_begin * 16, DG, -7) : 1.f;
 #pragma unroll
   for (int h2 = 0; h2 < 2; ++h2) {
     const int head = r + 8 * h2;
     const bool hv = head < G;
     const __nv_bfloat16* qrow = p.q + (int64_t(b) * p.Hq + int64_t(hkv) * G + head) * D;
+    float qn = p.qscale;
+    if constexpr (PART) {
+      float top = 0.f;
+      for (int d = 0; hv && d < 16 * DG; ++d)
+        top = fmaxf(top, fabsf(__bfloat162float(qrow[64 * (d >> 4) + 16 * c + (d & 15)])));
+      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+      qn = pow2_inverse(top, 0);
+      hs[h2] = p.qscale / qn;
+    }
 #pragma unroll
     for (int g = 0; g < DG; ++g) {
       float v[16];
@@ -108,8 +140,8 @@ __global__ void __launch_bounds__(RING ? 160 : 128) qkv_decode_attn_kernel(const
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
           const __nv_bfloat162 h = *reinterpret_cast<const __nv_bfloat162*>(&w[i]);
-          v[2 * i] = round_f16(__low2float(h) * p.qscale);
-          v[2 * i + 1] = round_f16(__high2float(h) * p.qscale);
+          v[2 * i] = round_f16(__low2float(h) * qn);
+          v[2 * i + 1] = round_f16(__high2float(h) * qn);
         }
       } else {
 #pragma unroll
@@ -272,6 +304,7 @@ __global__ void __launch_bounds__(RING ? 160 : 128) qkv_decode_attn_kernel(const
 #pragma unroll
         for (int g = 0; g < DG; ++g) v += ksc[nt][e][g] * (sacc[g][i] - KOFF * qg[row][g]);
         const int tok = nt * 8 + 2 * c + e;
+        if constexpr (PART) v *= hs[row];
         s[nt][i] = (t0 + tok < len) ? v : -INFINITY;
       }
     }
@@ -310,8 +343,13 @@ __global__ void __launch_bounds__(RING ? 160 : 128) qkv_decode_attn_kernel(const
     uint32_t vs01[DG], vs23[DG];
 #pragma unroll
     for (int g = 0; g < DG; ++g) {
-      vs01[g] = pack_f16x2(vsc[0][g], vsc[1][g]);
-      vs23[g] = pack_f16x2(vsc[2][g], vsc[3][g]);
+      if constexpr (PART) {  // 255 * 256 is the last fp16 value
+        vs01[g] = pack_f16x2(scaled_up_to(vsc[0][g], vn, 256.f), scaled_up_to(vsc[1][g], vn, 256.f));
+        vs23[g] = pack_f16x2(scaled_up_to(vsc[2][g], vn, 256.f), scaled_up_to(vsc[3][g], vn, 256.f));
+      } else {
+        vs01[g] = pack_f16x2(vsc[0][g], vsc[1][g]);
+        vs23[g] = pack_f16x2(vsc[2][g], vsc[3][g]);
+      }
     }
     const uint32_t off2 = pack_f16x2(KOFF, KOFF);
 #pragma unroll
@@ -516,7 +554,14 @@ __global__ void __launch_bounds__(RING ? 160 : 128) qkv_decode_attn_kernel(const
       }
     }
     const int64_t bh = int64_t(b) * p.Hq + hq0 + head;
-    if (p.n_splits == 1) {
+    if constexpr (PART) {
+      const int64_t part = bh * p.part_stride + p.part_base + split;
+      p.o_part[part * D + d] = o / vn;
+      if (d == 0) {
+        p.ml_part[part * 2 + 0] = mstar;
+        p.ml_part[part * 2 + 1] = l;
+      }
+    } else if (p.n_splits == 1) {
       p.out[bh * D + d] = __float2bfloat16_rn(l > 0.f ? o / l : 0.f);
     } else {
       p.o_part[(bh * p.n_splits + split) * D + d] = o;
@@ -566,7 +611,7 @@ __device__ __forceinline__ float fast_exp2(float x) {
 // NT = 16-token tiles a warp takes per step (2 when the pages hold an even
 // number of tiles): the tiles' MMA chains, loads and conversions interleave,
 // and the softmax max and the O rescale are paid once per NT tiles.
-template <int D, int NT>
+template <int D, int NT, bool PART = false>
 __global__ void __launch_bounds__(160, 2) qkv_decode_attn_t8_kernel(const AttnParams p,
                                                                     const __grid_constant__ CUtensorMap tmk,
                                                                     const __grid_constant__ CUtensorMap tmv) {
@@ -614,7 +659,7 @@ __global__ void __launch_bounds__(160, 2) qkv_decode_attn_t8_kernel(const AttnPa
   __syncthreads();
   // the CTA's pages: pair (blockIdx.z, blockIdx.y), context split blockIdx.x
   const int b = blockIdx.z, hkv = blockIdx.y;
-  const int len = p.seq_lens[b];
+  const int len = PART ? min(max(p.seq_lens[b], 0), p.max_len) : p.seq_lens[b];
   const int n_sub = (len + 15) / 16;
   const int per_split = (n_sub + p.n_splits - 1) / p.n_splits;
   const int sub_begin = int(blockIdx.x) * per_split;
@@ -657,10 +702,23 @@ __global__ void __launch_bounds__(160, 2) qkv_decode_attn_t8_kernel(const AttnPa
   {
     uint32_t qb[DG * 4][2];
     float kq[2][DG];  // heads 2c, 2c+1
+    float hs[2];      // PART: scores = S * hs
+    const float vn = PART && sub_begin < sub_end ? v_reference(p, b, hkv, sub_begin * 16, DG, 0) : 1.f;
     // ---- q^T fragments (head g, dims 64grp+16c+[0,16)) and (1024+127)*sum(q)
     {
       const bool hv = g < G;
       const __nv_bfloat16* qrow = p.q + (int64_t(b) * p.Hq + int64_t(hkv) * G + g) * D;
+      float qn = p.qscale;
+      if constexpr (PART) {
+        float top = 0.f;
+        for (int d = 0; hv && d < 16 * DG; ++d)
+          top = fmaxf(top, fabsf(__bfloat162float(qrow[64 * (d >> 4) + 16 * c + (d & 15)])));
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+        qn = pow2_inverse(top, 0);
+        hs[0] = __shfl_sync(0xffffffffu, p.qscale / qn, 8 * c);
+        hs[1] = __shfl_sync(0xffffffffu, p.qscale / qn, 8 * c + 4);
+      }
 #pragma unroll
       for (int grp = 0; grp < DG; ++grp) {
         float v[16];
@@ -671,8 +729,8 @@ __global__ void __launch_bounds__(160, 2) qkv_decode_attn_t8_kernel(const AttnPa
 #pragma unroll
           for (int i = 0; i < 8; ++i) {
             const __nv_bfloat162 h = *reinterpret_cast<const __nv_bfloat162*>(&w[i]);
-            v[2 * i] = round_f16(__low2float(h) * p.qscale);
-            v[2 * i + 1] = round_f16(__high2float(h) * p.qscale);
+            v[2 * i] = round_f16(__low2float(h) * qn);
+            v[2 * i + 1] = round_f16(__high2float(h) * qn);
           }
         } else {
 #pragma unroll
@@ -749,8 +807,13 @@ __global__ void __launch_bounds__(160, 2) qkv_decode_attn_t8_kernel(const AttnPa
                 const float2 vv = *reinterpret_cast<const float2*>(vsb + row * DG);
                 ksc[t][h][0] = kk.x;
                 ksc[t][h][1] = kk.y;
-                vsc[t][h][0] = valid[t][h] ? vv.x : 0.f;
-                vsc[t][h][1] = valid[t][h] ? vv.y : 0.f;
+                if constexpr (PART) {  // P <= 1, so P' stays below fp16's last value
+                  vsc[t][h][0] = valid[t][h] ? scaled_up_to(vv.x, vn, 32768.f) : 0.f;
+                  vsc[t][h][1] = valid[t][h] ? scaled_up_to(vv.y, vn, 32768.f) : 0.f;
+                } else {
+                  vsc[t][h][0] = valid[t][h] ? vv.x : 0.f;
+                  vsc[t][h][1] = valid[t][h] ? vv.y : 0.f;
+                }
               }
             }
 
@@ -778,6 +841,7 @@ __global__ void __launch_bounds__(160, 2) qkv_decode_attn_t8_kernel(const AttnPa
                 float v = 0.f;
     #pragma unroll
                 for (int grp = 0; grp < DG; ++grp) v += ksc[t][h][grp] * (sacc[grp][i] - kq[e][grp]);
+                if constexpr (PART) v *= hs[e];
                 s[t][i] = valid[t][h] ? v : -INFINITY;
               }
             }
@@ -889,7 +953,14 @@ __global__ void __launch_bounds__(160, 2) qkv_decode_attn_t8_kernel(const AttnPa
         }
       }
       const int64_t bh = int64_t(b) * p.Hq + hq0 + head;
-      if (p.n_splits == 1) {
+      if constexpr (PART) {
+        const int64_t part = bh * p.part_stride + p.part_base + int(blockIdx.x);
+        p.o_part[part * D + d] = o / vn;
+        if (d == 0) {
+          p.ml_part[part * 2 + 0] = mstar;
+          p.ml_part[part * 2 + 1] = l;
+        }
+      } else if (p.n_splits == 1) {
         p.out[bh * D + d] = __float2bfloat16_rn(l > 0.f ? o / l : 0.f);
       } else {
         const int split = blockIdx.x;
@@ -941,7 +1012,7 @@ static int make_kv_map(CUtensorMap* map, const uint8_t* base, int RB, int PS) {
   return r == CUDA_SUCCESS ? B2F_OK : B2F_ERR_INVALID;
 }
 
-template <int BITS, int D>
+template <int BITS, int D, bool PART = false>
 static int launch_attn(AttnParams p, cudaStream_t st) {
   constexpr int RB = D * BITS / 8;
   constexpr int DG = D / 64;
@@ -963,12 +1034,13 @@ static int launch_attn(AttnParams p, cudaStream_t st) {
     p.ring_bytes = ATTN_RING * p.slot_bytes + 128;
     smem = p.ring_bytes + merge;
   }
-  auto kern = qkv_decode_attn_kernel<BITS, D, false>;
+  auto kern = qkv_decode_attn_kernel<BITS, D, false, PART>;
   if constexpr (RING_OK) {
-    if (ring) kern = qkv_decode_attn_kernel<BITS, D, true>;
+    if (ring) kern = qkv_decode_attn_kernel<BITS, D, true, PART>;
   }
   if constexpr (BITS == 8 && D == 128) {
-    if (ring && p.G <= 8) kern = (p.PS / 16) % 2 == 0 ? qkv_decode_attn_t8_kernel<D, 2> : qkv_decode_attn_t8_kernel<D, 1>;
+    if (ring && p.G <= 8)
+      kern = (p.PS / 16) % 2 == 0 ? qkv_decode_attn_t8_kernel<D, 2, PART> : qkv_decode_attn_t8_kernel<D, 1, PART>;
   }
   if (smem > 48 * 1024) {
     cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
@@ -979,10 +1051,49 @@ static int launch_attn(AttnParams p, cudaStream_t st) {
   }
   const dim3 grid{unsigned(p.n_splits), unsigned(p.Hkv), unsigned(p.B)};
   int rc = launch_kernel(kern, grid, dim3{ring ? 160u : 128u}, size_t(smem), st, p, mk, mv);
-  if (rc != B2F_OK || p.n_splits == 1) return rc;
+  if (rc != B2F_OK || PART || p.n_splits == 1) return rc;
   return launch_kernel(attn_combine_kernel, dim3{unsigned(int64_t(p.B) * p.Hq)}, dim3{128}, 0, st,
                        static_cast<const float*>(p.o_part), static_cast<const float*>(p.ml_part), p.n_splits, D,
                        p.out);
+}
+
+template <int D>
+static int launch_part_bits(const AttnParams& p, int bits, cudaStream_t st) {
+  if (bits == 8) return launch_attn<8, D, true>(p, st);
+  if (bits == 4) return launch_attn<4, D, true>(p, st);
+  return launch_attn<2, D, true>(p, st);
+}
+
+// Decode attention over head-major pages as partials of splits part_base ..
+// part_base + n_splits - 1 of part_stride (prefix_attn.cu joins them).
+int launch_own_partials(const __nv_bfloat16* q, const uint8_t* kc, const float* ks, const uint8_t* vc, const float* vs,
+                        const int32_t* table, int64_t width, const int32_t* lens, int B, int Hq, int Hkv, int D, int P,
+                        int bits, float scale, int n_splits, int max_len, float* o_part, float* ml_part,
+                        int part_stride, int part_base, cudaStream_t st) {
+  AttnParams p{};
+  p.q = q;
+  p.kp = kc;
+  p.ks = ks;
+  p.vp = vc;
+  p.vs = vs;
+  p.block_table = table;
+  p.max_pages = width;
+  p.seq_lens = lens;
+  p.B = B;
+  p.Hq = Hq;
+  p.Hkv = Hkv;
+  p.G = Hq / Hkv;
+  p.PS = P;
+  p.head_stride = P;
+  p.slot_stride = 1;
+  p.n_splits = n_splits;
+  p.qscale = scale * 1.4426950408889634f;
+  p.o_part = o_part;
+  p.ml_part = ml_part;
+  p.part_stride = part_stride;
+  p.part_base = part_base;
+  p.max_len = max_len;
+  return D == 64 ? launch_part_bits<64>(p, bits, st) : launch_part_bits<128>(p, bits, st);
 }
 
 B2F_DEFINE_WAIT_CONTROLS(attn)
