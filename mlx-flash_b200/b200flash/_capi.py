@@ -186,19 +186,19 @@ def call(name: str, *args) -> int:
 
 def require_cuda(*tensors) -> torch.device:
     """All tensors must live on one CUDA device; returns it."""
-    dev = None
+    first = index = None
     for t in tensors:
         if t is None:
             continue
-        if not isinstance(t, torch.Tensor) or t.device.type != "cuda":
+        if not isinstance(t, torch.Tensor) or not t.is_cuda:
             raise ValueError("b200flash kernels take CUDA tensors (no CPU fallback)")
-        if dev is None:
-            dev = t.device
-        elif t.device != dev:
+        if first is None:
+            first, index = t, t.get_device()
+        elif t.get_device() != index:
             raise ValueError("all tensors must be on the same CUDA device")
-    if dev is None:
+    if first is None:
         raise ValueError("no tensor arguments")
-    return dev
+    return first.device
 
 
 def ptr(t) -> int:
@@ -229,7 +229,9 @@ def dependent_launches(on: bool = True):
 
 
 def stream_of(device) -> int:
-    return torch.cuda.current_stream(device).cuda_stream
+    # the current stream's handle without building a Stream object (2 us a call)
+    index = torch.device(device).index
+    return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device() if index is None else index)
 
 
 def aligned_contiguous(t: torch.Tensor, align: int = 16) -> torch.Tensor:

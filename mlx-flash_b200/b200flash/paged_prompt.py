@@ -36,10 +36,15 @@ class PagePlan(NamedTuple):
 
 
 def _int32(name, t, *shape):
-    if t.dtype != torch.int32 or t.dim() != len(shape) or any(s is not None and s != n for s, n in zip(shape, t.shape)):
+    """``t`` contiguous, after checking that it is int32 of ``shape`` (None: any extent)."""
+    ok = t.dtype is torch.int32 and t.dim() == len(shape)
+    if ok:
+        for want, got in zip(shape, t.shape):
+            ok = ok and (want is None or want == got)
+    if not ok:
         want = ", ".join("*" if s is None else str(s) for s in shape)
         raise ValueError(f"{name} must be int32 [{want}], got {t.dtype} {list(t.shape)}")
-    return t.contiguous()
+    return t if t.is_contiguous() else t.contiguous()
 
 
 def plan_pages(new_lens: torch.Tensor, free_pages: torch.Tensor, page_size: int, total_tokens: int,
@@ -66,9 +71,11 @@ def plan_pages(new_lens: torch.Tensor, free_pages: torch.Tensor, page_size: int,
     if not block_table.is_contiguous():
         raise ValueError("block_table is extended in place: it must be contiguous")
     _int32("block_table", block_table, B, None)
-    ints = {"dtype": torch.int32, "device": dev}
-    out = PagePlan(torch.empty(B + 1, **ints), torch.empty(T, **ints), torch.empty(T, dtype=torch.int64, device=dev),
-                   torch.empty(T, **ints), torch.empty(B, **ints), torch.empty(2, **ints))
+    # one allocation for the int32 outputs, positions and rows on 16-byte boundaries
+    pad = -T % 4
+    ints = torch.empty(2 * (T + pad) + 2 * B + 3, dtype=torch.int32, device=dev)
+    positions, _, rows, _, cu, lens, counts = ints.split((T, pad, T, pad, B + 1, B, 2))
+    out = PagePlan(cu, positions, torch.empty(T, dtype=torch.int64, device=dev), rows, lens, counts)
     ws_bytes = int(_capi.lib().b2f_page_plan_workspace_bytes(B))
     ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev) if ws_bytes else None
     call("b2f_page_plan", ptr(n), ptr(context_lens), B, ptr(free), free.shape[0], page_size, ptr(block_table),
@@ -150,10 +157,12 @@ def qk_norm_rope(qkv: torch.Tensor, n_heads: int, n_kv_heads: int, positions: to
 
 
 def _rows_of_heads(t):
-    """A [T, H, D] tensor whose strides the attention kernel takes (a copy only where they do not fit)."""
-    if t.stride(2) != 1 or t.stride(0) % 8 or t.stride(1) % 8 or t.data_ptr() % 16 or min(t.stride()) <= 0:
-        return aligned_contiguous(t)
-    return t
+    """A [T, H, D] tensor that the attention kernel takes (copied only where its strides do not fit), its strides."""
+    rows, heads, last = t.stride()
+    if last != 1 or rows % 8 or heads % 8 or rows <= 0 or heads <= 0 or t.data_ptr() % 16:
+        t = aligned_contiguous(t)
+        rows, heads, _ = t.stride()
+    return t, rows, heads
 
 
 def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqlens: torch.Tensor, causal: bool = True,
@@ -181,11 +190,10 @@ def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqle
         raise ValueError("cu_seqlens must hold at least one offset")
     if softmax_scale is None:
         softmax_scale = D ** -0.5
-    q, k, v = _rows_of_heads(q), _rows_of_heads(k), _rows_of_heads(v)
+    (q, q_row, q_head), (k, k_row, k_head), (v, v_row, v_head) = (_rows_of_heads(t) for t in (q, k, v))
     out = torch.empty(T, Hq, D, dtype=q.dtype, device=dev)
     lse = torch.empty(T, Hq, dtype=torch.float32, device=dev) if return_lse else None
-    call("b2f_prompt_attn", ptr(q), q.stride(0), q.stride(1), ptr(k), k.stride(0), k.stride(1), ptr(v), v.stride(0),
-         v.stride(1), DTYPE_CODES[q.dtype], ptr(cu), cu.shape[0] - 1, T, Hq, Hkv, D, int(bool(causal)),
+    call("b2f_prompt_attn", ptr(q), q_row, q_head, ptr(k), k_row, k_head, ptr(v), v_row, v_head, DTYPE_CODES[q.dtype], ptr(cu), cu.shape[0] - 1, T, Hq, Hkv, D, int(bool(causal)),
          float(softmax_scale), ptr(out), ptr(lse), stream_of(dev))
     return (out, lse) if return_lse else out
 

@@ -77,12 +77,14 @@ inline bool aligned(const void* p, uintptr_t a) {
 // IEEE round-to-nearest-even (the rounding MLX applies after an f32 op).
 struct TagBF16 {
   using T = __nv_bfloat16;
+  static constexpr int kBits = 8;  // of the significand
   static __device__ __forceinline__ float to_f(T v) { return __bfloat162float(v); }
   static __device__ __forceinline__ T from_f(float v) { return __float2bfloat16_rn(v); }
   static __device__ __forceinline__ float round(float v) { return to_f(from_f(v)); }
 };
 struct TagF16 {
   using T = __half;
+  static constexpr int kBits = 11;
   static __device__ __forceinline__ float to_f(T v) { return __half2float(v); }
   static __device__ __forceinline__ T from_f(float v) { return __float2half_rn(v); }
   static __device__ __forceinline__ float round(float v) { return to_f(from_f(v)); }

@@ -172,10 +172,14 @@ __global__ void __launch_bounds__(kPlanThreads) page_plan_fill_kernel(const Page
 //   y = x * rsqrt(mean(x^2) + eps) * w
 //   (y_i, y_{i+R/2}) -> (y_i cos a - y_{i+R/2} sin a, y_{i+R/2} cos a + y_i sin a),
 //   a = pos * inv_freq[i], i < R/2 (R = rotary width; dims past R unrotated)
-// D / 8 lanes hold one head, 8 consecutive values each (16-byte loads and
-// stores); a rotary pair sits R/16 lanes apart.  Everything is float32 with
-// one rounding at the end; the angle is formed and reduced in double, because
-// pos * inv_freq in float32 is off by 2^-25 * pos (0.004 rad at 131072).
+// HBM-bound: q and k are read and written once.  D / 8 lanes hold one head,
+// each two pieces of 4 values that rotate into one another (pieces i and
+// i + R/8 of the head; past R two neighbours), so the rotation needs no
+// shuffles, and a lane keeps one token: w cos and w sin stay in registers for
+// all of the token's heads.
+// Everything is float32 with one rounding at the end; the angle is formed and
+// reduced in double, because pos * inv_freq in float32 is off by 2^-25 * pos
+// (0.004 rad at 131072).
 // Appended K rows are the rounded k output through the cache's quantizer
 // (per 64 values: scale = absmax / max_int, each step rounded to the rows'
 // type), V rows are quantized as they are.
@@ -197,120 +201,334 @@ struct NormRopeParams {
   int T, Hq, Hkv, P, R, bits;
 };
 
-template <typename Tag, int D, bool APPEND>
-__global__ void __launch_bounds__(256) qk_norm_rope_rows_kernel(const NormRopeParams p) {
-  pdl_enter();
-  using E = typename Tag::T;
-  constexpr int LPH = D / 8;  // lanes per head
-  __shared__ float cs[D / 2], sn[D / 2];
-  const int t = blockIdx.x;
-  const int half = p.R / 2;
-  if (int(threadIdx.x) < half) {
-    constexpr double kTwoPi = 6.283185307179586476925;
-    const double a = double(p.positions[t]) * p.inv_freq[threadIdx.x];
-    sincosf(float(a - kTwoPi * rint(a / kTwoPi)), &sn[threadIdx.x], &cs[threadIdx.x]);
+template <typename Tag>
+__device__ __forceinline__ void unpack4(uint2 w, float (&v)[4]) {
+  const typename Tag::T* e = reinterpret_cast<const typename Tag::T*>(&w);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) v[i] = Tag::to_f(e[i]);
+}
+template <typename Tag>
+__device__ __forceinline__ uint2 pack4(const float (&v)[4]) {
+  typename Tag::T e[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) e[i] = Tag::from_f(v[i]);
+  return *reinterpret_cast<uint2*>(e);
+}
+
+// One 8-value piece (lane `sub` of a row) of a K or V row through the cache's
+// quantizer; 8 neighbouring lanes hold a group of 64.
+template <typename Tag, int D>
+__device__ __forceinline__ void append_piece(uint4 w, int sub, int64_t row, int bits, uint8_t* codes, float* scales) {
+  const float mi = bits == 8 ? 127.f : bits == 4 ? 7.f : 1.f;
+  const typename Tag::T* e = reinterpret_cast<const typename Tag::T*>(&w);
+  float v[8], m = 0.f;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    v[i] = Tag::to_f(e[i]);
+    m = fmaxf(m, fabsf(v[i]));
   }
-  __syncthreads();
-  const int sub = threadIdx.x % LPH;  // this lane's 8 values of the head
-  const E* row = static_cast<const E*>(p.qkv) + int64_t(t) * p.ld;
-  const int NH = p.Hq + p.Hkv * (APPEND ? 2 : 1);
-  const int pair = half / 8;  // lanes between the halves of a rotary pair
-  const int lane = threadIdx.x & 31;
-  const int partner = sub < pair ? lane + pair : sub < 2 * pair ? lane - pair : lane;
-  int64_t slot = -1;
-  if constexpr (APPEND) slot = p.slots[t];
-  // every lane takes the same number of turns: the shuffles below are warp-wide
-  const int per = blockDim.x / LPH;
-  for (int h0 = 0; h0 < NH; h0 += per) {
-    const int h = h0 + threadIdx.x / LPH;
-    const bool on = h < NH;
-    float v[8];
-    {
-      const uint4 w = on ? *reinterpret_cast<const uint4*>(row + int64_t(h) * D + sub * 8) : make_uint4(0, 0, 0, 0);
-      const E* e = reinterpret_cast<const E*>(&w);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) v[i] = Tag::to_f(e[i]);
-    }
-    const bool is_q = h < p.Hq, is_v = h >= p.Hq + p.Hkv;
-    float ss = 0.f;
+  for (int k = 1; k < 8; k <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, k));
+  if (row < 0) return;
+  float scale = Tag::round(__fdiv_rn(m, mi));
+  if (scale == 0.f) scale = 1.f;
+  // round(v / scale) to the rows' type: the product with the reciprocal is
+  // within 2 ulp of the quotient, so both round alike unless the product lies
+  // within 8 ulp of a midpoint of the type; there, divide.  Then to the nearest
+  // integer (ties to even) by adding 1.5 * 2^23.
+  const float rs = __frcp_rn(scale);
+  constexpr uint32_t kLow = (1u << (24 - Tag::kBits)) - 1;  // float bits below the type's last
+  uint32_t c[8];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) ss += v[i] * v[i];
-#pragma unroll
-    for (int o = LPH / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-    if (!is_v) {
-      const float r = rsqrtf(ss / float(D) + p.eps);
-      const uint4 w = *reinterpret_cast<const uint4*>(static_cast<const E*>(is_q ? p.qw : p.kw) + sub * 8);
-      const E* e = reinterpret_cast<const E*>(&w);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) v[i] *= r * Tag::to_f(e[i]);
-    }
-    float u[8];
-#pragma unroll
-    for (int i = 0; i < 8; ++i) u[i] = __shfl_sync(0xffffffffu, v[i], partner);
-    if (!is_v && sub < 2 * pair) {
-      const int f = (sub < pair ? sub : sub - pair) * 8;
-      const float sign = sub < pair ? -1.f : 1.f;
-#pragma unroll
-      for (int i = 0; i < 8; ++i) v[i] = v[i] * cs[f + i] + sign * u[i] * sn[f + i];
-    }
-    E o[8];
-#pragma unroll
-    for (int i = 0; i < 8; ++i) o[i] = Tag::from_f(v[i]);
-    if (on && !is_v) {
-      E* dst = is_q ? static_cast<E*>(p.q_out) + (int64_t(t) * p.Hq + h) * D
-                    : static_cast<E*>(p.k_out) + (int64_t(t) * p.Hkv + h - p.Hq) * D;
-      *reinterpret_cast<uint4*>(dst + sub * 8) = *reinterpret_cast<const uint4*>(o);
-    }
-    if constexpr (APPEND) {
-      const float mi = p.bits == 8 ? 127.f : p.bits == 4 ? 7.f : 1.f;
-      float m = 0.f;
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        v[i] = Tag::to_f(o[i]);
-        m = fmaxf(m, fabsf(v[i]));
-      }
-#pragma unroll
-      for (int k = 1; k < 8; k <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, k));
-      if (!on || is_q || slot < 0) continue;
-      float scale = Tag::round(__fdiv_rn(m, mi));
-      if (scale == 0.f) scale = 1.f;
-      uint32_t c[8];
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const float x = Tag::round(rintf(Tag::round(__fdiv_rn(v[i], scale))));
-        c[i] = uint32_t(int(Tag::round(fminf(fmaxf(x, -mi), mi) + mi)));
-      }
-      const int kvh = (h - p.Hq) % p.Hkv;
-      const int64_t page = slot / p.P;
-      const int64_t r = (page * p.Hkv + kvh) * p.P + (slot - page * p.P);
-      if (sub % 8 == 0) (is_v ? p.v_scales : p.k_scales)[r * (D / 64) + sub / 8] = scale;
-      uint8_t* dst = (is_v ? p.v_codes : p.k_codes) + r * (D * p.bits / 8) + sub * p.bits;
-      if (p.bits == 8) {
-        *reinterpret_cast<uint2*>(dst) = make_uint2(c[0] | c[1] << 8 | c[2] << 16 | c[3] << 24,
-                                                    c[4] | c[5] << 8 | c[6] << 16 | c[7] << 24);
-      } else if (p.bits == 4) {
-        *reinterpret_cast<uint32_t*>(dst) = (c[0] << 4 | c[1]) | (c[2] << 4 | c[3]) << 8 |
-                                            (c[4] << 4 | c[5]) << 16 | (c[6] << 4 | c[7]) << 24;
-      } else {
-        *reinterpret_cast<uint16_t*>(dst) = uint16_t((c[0] << 6 | c[1] << 4 | c[2] << 2 | c[3]) |
-                                                     (c[4] << 6 | c[5] << 4 | c[6] << 2 | c[7]) << 8);
-      }
-    }
+  for (int i = 0; i < 8; ++i) {
+    float x = __fmul_rn(v[i], rs);
+    if ((__float_as_uint(x) & kLow) - (kLow / 2 - 7u) <= 0x10u || !isfinite(rs)) x = __fdiv_rn(v[i], scale);
+    x = fminf(fmaxf(Tag::round(x), -mi), mi);
+    c[i] = __float_as_uint(__fadd_rn(x, 12582912.f)) - 0x4B400000u + uint32_t(int(mi));
+  }
+  if (sub % 8 == 0) scales[row * (D / 64) + sub / 8] = scale;
+  uint8_t* dst = codes + row * (D * bits / 8) + sub * bits;
+  if (bits == 8) {
+    *reinterpret_cast<uint2*>(dst) = make_uint2(c[0] | c[1] << 8 | c[2] << 16 | c[3] << 24,
+                                                c[4] | c[5] << 8 | c[6] << 16 | c[7] << 24);
+  } else if (bits == 4) {
+    *reinterpret_cast<uint32_t*>(dst) = (c[0] << 4 | c[1]) | (c[2] << 4 | c[3]) << 8 | (c[4] << 4 | c[5]) << 16 |
+                                        (c[6] << 4 | c[7]) << 24;
+  } else {
+    *reinterpret_cast<uint16_t*>(dst) = uint16_t((c[0] << 6 | c[1] << 4 | c[2] << 2 | c[3]) |
+                                                 (c[4] << 6 | c[5] << 4 | c[6] << 2 | c[7]) << 8);
   }
 }
 
+// One lane's share of the heads of a token.
 template <typename Tag, int D>
+struct NormRopeLane {
+  using E = typename Tag::T;
+  static constexpr int LPH = D / 8;  // lanes a head
+  const NormRopeParams& p;
+  int sub, ea, eb;  // lane of the head, first values of the lane's two pieces
+  bool turns;
+  float cs[4], sn[4];
+  float ac[4], bs[4], bc[4], as[4];  // (a, b) -> (a * ac - b * bs, b * bc + a * as)
+
+  __device__ __forceinline__ explicit NormRopeLane(const NormRopeParams& q) : p(q) {
+    sub = threadIdx.x % LPH;
+    turns = sub < p.R / 8;
+    ea = turns ? 4 * sub : p.R + 8 * (sub - p.R / 8);
+    eb = turns ? ea + p.R / 2 : ea + 4;
+  }
+  // The angle is within [-pi, pi], where __sincosf is off by at most 2^-20.9.
+  __device__ __forceinline__ void angles(int position) {
+    constexpr double kTwoPi = 6.283185307179586476925;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const double a = turns ? double(position) * p.inv_freq[4 * sub + i] : 0.0;
+      __sincosf(float(a - kTwoPi * rint(a * (1.0 / kTwoPi))), &sn[i], &cs[i]);
+    }
+  }
+  __device__ __forceinline__ void weights(const void* w) {
+    float wa[4], wb[4];
+    unpack4<Tag>(*reinterpret_cast<const uint2*>(static_cast<const E*>(w) + ea), wa);
+    unpack4<Tag>(*reinterpret_cast<const uint2*>(static_cast<const E*>(w) + eb), wb);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      ac[i] = wa[i] * cs[i];
+      as[i] = wa[i] * sn[i];
+      bc[i] = wb[i] * cs[i];
+      bs[i] = wb[i] * sn[i];
+    }
+  }
+  __device__ __forceinline__ int64_t page_row(int64_t slot) const {  // cache row of head 0, -1: none
+    if (slot < 0) return -1;
+    const int64_t page = slot >> 32 ? slot / p.P : int64_t(uint32_t(slot) / uint32_t(p.P));
+    return page * p.Hkv * p.P + (slot - page * p.P);
+  }
+  // One head from the lane's two pieces; every lane of the warp calls it
+  // (shuffles).  Norm and rotate (unless `raw`); dst: null where nothing is
+  // written; QUANT: append to cache row `row` (-1: none).
+  template <bool QUANT>
+  __device__ __forceinline__ void head(uint2 xa, uint2 xb, bool raw, E* dst, int64_t row, uint8_t* codes,
+                                       float* scales) const {
+    uint2 ya = xa, yb = xb;
+    float a[4], b[4], ss = 0.f;
+    unpack4<Tag>(xa, a);
+    unpack4<Tag>(xb, b);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) ss = fmaf(a[i], a[i], fmaf(b[i], b[i], ss));
+#pragma unroll
+    for (int o = LPH / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+    const float r = rsqrtf(fmaf(ss, 1.f / float(D), p.eps));
+    float c[4], d[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      c[i] = r * (a[i] * ac[i] - b[i] * bs[i]);
+      d[i] = r * (b[i] * bc[i] + a[i] * as[i]);
+    }
+    if (!raw) {
+      ya = pack4<Tag>(c);
+      yb = pack4<Tag>(d);
+    }
+    if (dst) {
+      *reinterpret_cast<uint2*>(dst + ea) = ya;
+      *reinterpret_cast<uint2*>(dst + eb) = yb;
+    }
+    if constexpr (QUANT) {
+      if (!__any_sync(0xffffffffu, row >= 0)) return;
+      // 8 consecutive values a lane: 4-value pieces 2 sub and 2 sub + 1 from the lanes that hold them
+      uint2 piece[2];
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        const int j = 2 * sub + k, q8 = p.R / 8;
+        const int from = j < q8 ? j : j < 2 * q8 ? j - q8 : q8 + (j - 2 * q8) / 2;
+        const bool second = j < q8 ? false : j < 2 * q8 ? true : (j - 2 * q8) & 1;
+        const int src = (threadIdx.x & 31 & ~(LPH - 1)) + from;
+        const uint2 va = make_uint2(__shfl_sync(0xffffffffu, ya.x, src), __shfl_sync(0xffffffffu, ya.y, src));
+        const uint2 vb = make_uint2(__shfl_sync(0xffffffffu, yb.x, src), __shfl_sync(0xffffffffu, yb.y, src));
+        piece[k] = second ? vb : va;
+      }
+      append_piece<Tag, D>(make_uint4(piece[0].x, piece[0].y, piece[1].x, piece[1].y), sub, row, p.bits, codes, scales);
+    }
+  }
+};
+
+// Few tokens: a CTA on each, the heads side by side (latency).
+template <typename Tag, int D, bool APPEND>
+__global__ void __launch_bounds__(256) qk_norm_rope_few_kernel(const NormRopeParams p) {
+  pdl_enter();
+  using E = typename Tag::T;
+  constexpr int STEP = 256 / (D / 8);  // heads at a time
+  NormRopeLane<Tag, D> lane(p);
+  const int t = blockIdx.x, NH = p.Hq + p.Hkv * (APPEND ? 2 : 1);
+  const E* row = static_cast<const E*>(p.qkv) + int64_t(t) * p.ld;
+  int h = threadIdx.x / (D / 8);
+  uint2 xa = make_uint2(0u, 0u), xb = xa;
+  auto load = [&](int head) {
+    if (head >= NH) return;
+    xa = *reinterpret_cast<const uint2*>(row + head * D + lane.ea);
+    xb = *reinterpret_cast<const uint2*>(row + head * D + lane.eb);
+  };
+  load(h);
+  lane.angles(p.positions[t]);
+  bool for_k = h >= p.Hq;
+  lane.weights(for_k ? p.kw : p.qw);
+  const int64_t row0 = APPEND ? lane.page_row(p.slots[t]) : -1;
+  // every lane takes the same number of turns: the shuffles are warp-wide
+  for (int h0 = 0; h0 < NH; h0 += STEP, h += STEP) {
+    const uint2 a = xa, b = xb;
+    load(h + STEP);
+    if (!for_k && h >= p.Hq) {
+      lane.weights(p.kw);
+      for_k = true;
+    }
+    const bool is_v = h >= p.Hq + p.Hkv;
+    E* dst = h < p.Hq ? static_cast<E*>(p.q_out) + (int64_t(t) * p.Hq + h) * D
+                      : static_cast<E*>(p.k_out) + (int64_t(t) * p.Hkv + h - p.Hq) * D;
+    const int64_t at = row0 < 0 || h < p.Hq || h >= NH ? -1 : row0 + int64_t(h - p.Hq - (is_v ? p.Hkv : 0)) * p.P;
+    lane.template head<APPEND>(a, b, is_v, is_v || h >= NH ? nullptr : dst, at, is_v ? p.v_codes : p.k_codes,
+                                     is_v ? p.v_scales : p.k_scales);
+  }
+}
+
+// Many tokens: a warp takes runs of up to 4 KB of a token's q, k or v heads
+// from a ring of its own that bulk copies keep filled, so memory has work
+// while the warp computes (loads to registers: 4.4 TB/s at 32768 tokens of 40
+// heads).  Each warp has the same number of consecutive runs, and forms the
+// angles once for those of one token.
+constexpr int NR_WARPS = 4, NR_STAGES = 3, NR_CHUNK = 4096;
+constexpr int NR_CTAS = 4;  // per SM: 48 KB of ring each
+
+template <typename Tag, int D, bool APPEND>
+__global__ void __launch_bounds__(32 * NR_WARPS, NR_CTAS) qk_norm_rope_stream_kernel(const NormRopeParams p) {
+  pdl_enter();
+  using E = typename Tag::T;
+  constexpr int CH = NR_CHUNK / (2 * D), PER = 32 / (D / 8);  // heads of a run, of a warp's turn
+  extern __shared__ __align__(128) uint8_t nr_smem[];
+  __shared__ uint64_t full[NR_WARPS][NR_STAGES];
+  const int warp = threadIdx.x >> 5, l = threadIdx.x & 31;
+  uint8_t* ring = nr_smem + warp * NR_STAGES * NR_CHUNK;
+  if (l == 0) {
+    for (int s = 0; s < NR_STAGES; ++s) mbar_init(&full[warp][s], 1);
+    fence_mbarrier_init();
+  }
+  __syncwarp();
+  // runs of a token: nq of q heads, nk of k heads, as many of v heads
+  const int nq = (p.Hq + CH - 1) / CH, nk = (p.Hkv + CH - 1) / CH, NC = nq + nk * (APPEND ? 2 : 1);
+  const int64_t runs = int64_t(p.T) * NC;
+  const int warps = gridDim.x * NR_WARPS, w = blockIdx.x * NR_WARPS + warp;
+  const int64_t begin = runs * w / warps;
+  const int count = int(runs * (w + 1) / warps - begin);
+  struct Run {
+    int t, c;  // token, run of the token
+  };
+  // first head of the run in the row, number of heads
+  auto heads = [&](int c, int& n) {
+    const int base = c < nq ? 0 : c < nq + nk ? p.Hq : p.Hq + p.Hkv;
+    const int k = (c < nq ? c : c < nq + nk ? c - nq : c - nq - nk) * CH;
+    n = min(CH, (c < nq ? p.Hq : p.Hkv) - k);
+    return base + k;
+  };
+  auto advance = [&](Run& r) {
+    if (++r.c == NC) r.c = 0, ++r.t;
+  };
+  const bool stall = producers_stalled();  // test control: nothing is issued
+  Run ahead{int(begin / NC), int(begin % NC)}, now = ahead;
+  int issued = 0;
+  auto issue = [&]() {
+    if (issued >= count) return;
+    if (l == 0 && !stall) {
+      int n;
+      const int s = issued % NR_STAGES, h = heads(ahead.c, n);
+      const uint32_t bytes = uint32_t(n) * D * 2;
+      mbar_arrive_expect_tx(&full[warp][s], bytes);
+      bulk_g2s(ring + s * NR_CHUNK, static_cast<const E*>(p.qkv) + ahead.t * p.ld + h * D, bytes, &full[warp][s]);
+    }
+    ++issued;
+    advance(ahead);
+  };
+  for (int s = 0; s < NR_STAGES; ++s) issue();
+  NormRopeLane<Tag, D> lane(p);
+  int pos = 0;
+  int64_t slot = -1, row0 = -1;
+  auto look = [&](int t) {
+    if (t >= p.T) return;
+    pos = p.positions[t];
+    if constexpr (APPEND) slot = p.slots[t];
+  };
+  look(now.t);
+  bool ok = true;
+  int n = 0;
+  for (; n < count; ++n) {
+    const int c = now.c, t = now.t;
+    if (n == 0 || c == 0) {
+      lane.angles(pos);
+      if constexpr (APPEND) row0 = lane.page_row(slot);
+      look(t + 1);  // a token ahead
+    }
+    if (n == 0 || c == 0 || c == nq) lane.weights(c < nq ? p.qw : p.kw);
+    const int s = n % NR_STAGES;
+    ok = __all_sync(0xffffffffu, mbar_wait_bounded(&full[warp][s], uint32_t((n / NR_STAGES) & 1)));
+    if (!ok) break;
+    int hn;
+    const int h0 = heads(c, hn), hl = l / (D / 8);
+    const uint8_t* src = ring + s * NR_CHUNK + hl * D * 2;
+    const bool is_q = c < nq, is_v = APPEND && c >= nq + nk;
+    const int kh = h0 - (is_q ? 0 : is_v ? p.Hq + p.Hkv : p.Hq) + hl;  // this lane's first head of its kind
+    E* dst = (is_q ? static_cast<E*>(p.q_out) + (int64_t(t) * p.Hq + kh) * D
+                   : static_cast<E*>(p.k_out) + (int64_t(t) * p.Hkv + kh) * D);
+    int64_t row = row0 + int64_t(kh) * p.P;
+    for (int i = hl; i - hl < hn; i += PER) {
+      const bool on = i < hn;  // a piece past the run is read from the ring, and dropped
+      const uint2 xa = *reinterpret_cast<const uint2*>(src + lane.ea * 2), xb = *reinterpret_cast<const uint2*>(src + lane.eb * 2);
+      const int64_t at = on && row0 >= 0 ? row : -1;
+      if (is_q) lane.template head<false>(xa, xb, false, on ? dst : nullptr, -1, nullptr, nullptr);
+      else if (!is_v) lane.template head<APPEND>(xa, xb, false, on ? dst : nullptr, at, p.k_codes, p.k_scales);
+      else if constexpr (APPEND)
+        append_piece<Tag, D>(*reinterpret_cast<const uint4*>(src + lane.sub * 16), lane.sub, at, p.bits, p.v_codes, p.v_scales);
+      src += PER * D * 2;
+      dst += PER * D;
+      row += int64_t(PER) * p.P;
+    }
+    advance(now);
+    __syncwarp();  // the run has been read
+    issue();
+  }
+  if (!ok) {
+    // copies already issued land before the CTA goes away
+    for (int k = n; k < issued && !stall; ++k)
+      mbar_wait_bounded(&full[warp][k % NR_STAGES], uint32_t((k / NR_STAGES) & 1), 100000000ull);
+    if (l == 0) report_timeout(nullptr);
+  }
+}
+
+template <typename Tag, int D, bool APPEND>
 static int launch_norm_rope(const NormRopeParams& p, cudaStream_t st) {
-  auto kern = p.slots ? qk_norm_rope_rows_kernel<Tag, D, true> : qk_norm_rope_rows_kernel<Tag, D, false>;
-  return launch_kernel(kern, dim3{unsigned(p.T)}, dim3{256}, 0, st, p);
+  // a CTA each up to 4 per SM: measured for 36 heads of 128 at 592 tokens, few F1, stream F2
+  if (p.T <= 4 * 148)
+    return launch_kernel(qk_norm_rope_few_kernel<Tag, D, APPEND>, dim3{unsigned(p.T)}, dim3{256}, 0, st, p);
+  auto kern = qk_norm_rope_stream_kernel<Tag, D, APPEND>;
+  constexpr int smem = NR_WARPS * NR_STAGES * NR_CHUNK;
+  const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  if (e != cudaSuccess) {
+    set_last_cuda_error(e);
+    return B2F_ERR_CUDA;
+  }
+  const int want = p.T, most = NR_CTAS * 148;
+  return launch_kernel(kern, dim3{unsigned(want < most ? want : most)}, dim3{32 * NR_WARPS}, smem, st, p);
+}
+
+template <typename Tag, int D>
+static int launch_norm_rope_a(const NormRopeParams& p, cudaStream_t st) {
+  return p.slots ? launch_norm_rope<Tag, D, true>(p, st) : launch_norm_rope<Tag, D, false>(p, st);
 }
 
 template <typename Tag>
 static int launch_norm_rope_d(const NormRopeParams& p, int64_t D, cudaStream_t st) {
-  if (D == 64) return launch_norm_rope<Tag, 64>(p, st);
-  if (D == 128) return launch_norm_rope<Tag, 128>(p, st);
-  return launch_norm_rope<Tag, 256>(p, st);
+  if (D == 64) return launch_norm_rope_a<Tag, 64>(p, st);
+  if (D == 128) return launch_norm_rope_a<Tag, 128>(p, st);
+  return launch_norm_rope_a<Tag, 256>(p, st);
 }
+
+B2F_DEFINE_WAIT_CONTROLS(prompt_ops)
 
 }  // namespace b2f
 

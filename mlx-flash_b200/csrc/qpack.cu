@@ -515,10 +515,12 @@ int b2f_wait_controls_attn(int op, long long* v);
 int b2f_wait_controls_p2p(int op, long long* v);
 int b2f_wait_controls_prompt_attn(int op, long long* v);
 int b2f_wait_controls_prefix_attn(int op, long long* v);
+int b2f_wait_controls_prompt_ops(int op, long long* v);
 static int (*const k_wait_units[])(int, long long*) = {b2f_wait_controls_mma, b2f_wait_controls_tc,
                                                         b2f_wait_controls_tc2, b2f_wait_controls_gemv,
                                                         b2f_wait_controls_attn, b2f_wait_controls_p2p,
-                                                        b2f_wait_controls_prompt_attn, b2f_wait_controls_prefix_attn};
+                                                        b2f_wait_controls_prompt_attn, b2f_wait_controls_prefix_attn,
+                                                        b2f_wait_controls_prompt_ops};
 }  // namespace b2f
 
 extern "C" {

@@ -117,6 +117,8 @@ def norm_rope_reference(x, w, pos, inv, eps):
 @pytest.mark.parametrize("T,Hq,Hkv,D,dt,rot", [
     (1, 32, 4, 128, "bf16", None), (3, 5, 1, 64, "f16", None), (37, 8, 8, 128, "f16", None), (130, 6, 2, 256, "bf16", None),
     (64, 32, 4, 128, "bf16", 32), (9, 3, 3, 64, "bf16", 8), (5, 4, 2, 128, "f16", 0),
+    (601, 32, 4, 128, "bf16", None), (700, 41, 3, 64, "f16", None), (2049, 9, 1, 256, "bf16", None),
+    (1203, 17, 2, 128, "f16", 40),
 ])
 def test_qk_norm_rope(dev, T, Hq, Hkv, D, dt, rot):
     from b200flash.paged_prompt import qk_norm_rope
@@ -139,20 +141,21 @@ def test_qk_norm_rope(dev, T, Hq, Hkv, D, dt, rot):
     assert torch.equal(v, x[:, Hq + Hkv:])
 
 
+@pytest.mark.parametrize("T", [70, 1300])
 @pytest.mark.parametrize("D,dt,bits,page", [(128, "bf16", 8, 64), (64, "bf16", 4, 16), (128, "f16", 2, 48),
                                             (256, "bf16", 8, 16), (128, "f16", 4, 64)])
-def test_qk_norm_rope_append(dev, D, dt, bits, page):
+def test_qk_norm_rope_append(dev, D, dt, bits, page, T):
     """The appended bytes are the quantizer's on the returned k and on v; skipped slots stay untouched."""
     from b200flash.paged_prompt import qk_norm_rope
     from b200flash.quantized_kv_cache import quantize_tensor
 
-    T, Hq, Hkv = 70, 6, 3
+    Hq, Hkv = 6, 3
     g = torch.Generator(device=dev).manual_seed(bits)
     qkv = torch.randn(T, (Hq + 2 * Hkv) * D, device=dev, generator=g).to(DT[dt])
     qkv[4] = 0  # a row of zeros: scale 1
     w = torch.ones(D, device=dev, dtype=DT[dt])
     pos = torch.arange(T, dtype=torch.int32, device=dev)
-    pages = 9
+    pages = -(-T // page) + 2
     slots = torch.randperm(pages * page, device=dev, generator=g)[:T]
     slots[7] = slots[33] = -1
     lead = (pages, Hkv, page)
