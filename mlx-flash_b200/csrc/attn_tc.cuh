@@ -32,13 +32,38 @@ __device__ __forceinline__ void tma_load_4d(void* dst, const CUtensorMap* map, i
       : "memory");
 }
 
-// D[tmem] (+)= A[tmem] . B[smem]
-__device__ __forceinline__ void tc_mma_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc, uint32_t idesc,
-                                          uint32_t accumulate) {
+// The warp that issues MMAs runs converged and one elected lane issues: the
+// descriptors are then formed in uniform registers, which the instruction
+// takes.  From a branch that one lane enters alone an MMA took 82 to 140
+// cycles to issue, against 64 to execute.
+__device__ __forceinline__ uint32_t elect_lane() {
+  uint32_t is;
+  asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}\n" : "=r"(is));
+  return is;
+}
+// D[tmem] (+)= A[smem] . B[smem], by the elected lane
+__device__ __forceinline__ void tc_mma_ss(uint32_t elected, uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc,
+                                          uint32_t idesc, uint32_t accumulate) {
   asm volatile(
-      "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
-      " tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, {%5, %5, %5, %5}, p;\n}\n" ::"r"(d_tmem),
-      "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(accumulate), "r"(0u)
+      "{\n .reg .pred p, q;\n setp.ne.b32 p, %4, 0;\n setp.ne.b32 q, %5, 0;\n"
+      " @q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(d_tmem),
+      "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate), "r"(elected)
+      : "memory");
+}
+// D[tmem] (+)= A[tmem] . B[smem], by the elected lane
+__device__ __forceinline__ void tc_mma_ts(uint32_t elected, uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc,
+                                          uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n .reg .pred p, q;\n setp.ne.b32 p, %4, 0;\n setp.ne.b32 q, %5, 0;\n"
+      " @q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n" ::"r"(d_tmem),
+      "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(accumulate), "r"(elected)
+      : "memory");
+}
+__device__ __forceinline__ void tc_commit_by(uint32_t elected, uint64_t* bar) {
+  asm volatile(
+      "{\n .reg .pred q;\n setp.ne.b32 q, %1, 0;\n"
+      " @q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n}\n" ::"r"(smem_u32(bar)),
+      "r"(elected)
       : "memory");
 }
 
@@ -109,6 +134,14 @@ __device__ __forceinline__ void tmem_ld128(uint32_t taddr, uint32_t (&v)[128]) {
       : "r"(taddr)
       : "memory");
 }
+__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&v)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15};"
+      :
+      : "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]),
+        "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15]), "r"(taddr)
+      : "memory");
+}
 __device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t (&v)[32]) {
   asm volatile(
       "tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31};"
@@ -118,6 +151,101 @@ __device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t (&v)[32
         "r"(v[16]), "r"(v[17]), "r"(v[18]), "r"(v[19]), "r"(v[20]), "r"(v[21]), "r"(v[22]), "r"(v[23]),
         "r"(v[24]), "r"(v[25]), "r"(v[26]), "r"(v[27]), "r"(v[28]), "r"(v[29]), "r"(v[30]), "r"(v[31]), "r"(taddr)
       : "memory");
+}
+
+// ---- softmax of one score row per thread ------------------------------------
+// Two floats in a 64-bit register: the packed FMA, add and multiply issue once
+// for both.
+__device__ __forceinline__ uint64_t f32x2(float lo, float hi) {
+  uint64_t d;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "f"(lo), "f"(hi));
+  return d;
+}
+__device__ __forceinline__ uint64_t f32x2_bits(uint32_t lo, uint32_t hi) {
+  uint64_t d;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "r"(lo), "r"(hi));
+  return d;
+}
+__device__ __forceinline__ float2 f32x2_parts(uint64_t v) {
+  float2 d;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(d.x), "=f"(d.y) : "l"(v));
+  return d;
+}
+__device__ __forceinline__ uint64_t fma_x2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+  return d;
+}
+__device__ __forceinline__ uint64_t add_x2(uint64_t a, uint64_t b) {
+  uint64_t d;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float d;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+
+template <int N>
+__device__ __forceinline__ float row_max(const uint32_t (&s)[N]) {
+  float m[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+  for (int c = 0; c < N; c += 2)
+    m[(c >> 1) & 3] = max3(m[(c >> 1) & 3], __uint_as_float(s[c]), __uint_as_float(s[c + 1]));
+  return fmaxf(max3(m[0], m[1], m[2]), m[3]);
+}
+
+// 2^x for a pair on the FMA pipe, for -126 <= x < 128 (below: 2^-126): with n
+// the nearest integer, 2^x = 2^n p(x - n), p a polynomial fitted to the least
+// relative error on [-1/2, 1/2] (degree 3: 2^-13.7, for bf16 results; degree
+// 4: 2^-18.5, for fp16), n added to the exponent bits.
+template <bool BF16>
+__device__ __forceinline__ uint64_t exp2_poly_x2(uint64_t x2) {
+  const float2 x = f32x2_parts(x2);
+  constexpr float kRound = 12582912.f;  // 1.5 * 2^23: the sum's low bits are the nearest integer
+  const uint64_t v = f32x2(fmaxf(x.x, -126.f), fmaxf(x.y, -126.f));
+  const uint64_t t = add_x2(v, f32x2(kRound, kRound));
+  const uint64_t n = add_x2(t, f32x2(-kRound, -kRound));
+  const uint64_t r = fma_x2(n, f32x2(-1.f, -1.f), v);
+  uint64_t p;
+  if constexpr (BF16) {
+    p = fma_x2(r, f32x2(0.055171669f, 0.055171669f), f32x2(0.242611122f, 0.242611122f));
+    p = fma_x2(p, r, f32x2(0.693260985f, 0.693260985f));
+    p = fma_x2(p, r, f32x2(0.999928074f, 0.999928074f));
+  } else {
+    p = fma_x2(r, f32x2(0.00957010191f, 0.00957010191f), f32x2(0.0559178603f, 0.0559178603f));
+    p = fma_x2(p, r, f32x2(0.240247448f, 0.240247448f));
+    p = fma_x2(p, r, f32x2(0.693121815f, 0.693121815f));
+    p = fma_x2(p, r, f32x2(0.999999261f, 0.999999261f));
+  }
+  const float2 pf = f32x2_parts(p), tf = f32x2_parts(t);
+  return f32x2_bits(__float_as_uint(pf.x) + (__float_as_uint(tf.x) << 23),
+                    __float_as_uint(pf.y) + (__float_as_uint(tf.y) << 23));
+}
+
+// P = 2^(s * scale - ref) of N scores as packed 16-bit pairs, their sum added
+// to sum[0..1] (pairs).  With POLY, one pair of four goes to the FMA pipe: the
+// 16 exponentials a cycle of the SM are what bounds a head of 128 otherwise
+// (2 * 128 * 128 of them per 2048 cycles of tensor work).
+template <bool BF16, bool POLY, int N>
+__device__ __forceinline__ void exp_row(const uint32_t (&s)[N], float scale, float ref, uint64_t (&sum)[2],
+                                        uint32_t (&out)[N / 2]) {
+  const uint64_t k = f32x2(scale, scale), b = f32x2(-ref, -ref);
+#pragma unroll
+  for (int c = 0; c < N / 2; ++c) {
+    const uint64_t x = fma_x2(f32x2_bits(s[2 * c], s[2 * c + 1]), k, b);
+    uint64_t p;
+    if (POLY && (c & 3) == 3) {
+      p = exp2_poly_x2<BF16>(x);
+    } else {
+      const float2 v = f32x2_parts(x);
+      p = f32x2(ex2(v.x), ex2(v.y));
+    }
+    sum[c & 1] = add_x2(sum[c & 1], p);
+    const float2 e = f32x2_parts(p);
+    out[c] = BF16 ? pack_bf16x2(e.x, e.y) : pack_f16x2(e.x, e.y);
+  }
 }
 
 }  // namespace b2f

@@ -184,46 +184,50 @@ __global__ void __launch_bounds__(PX_THREADS, 1) prefix_attn_kernel(const Prefix
 
   if (warp == 12) {
     // ============================ MMA issuer ====================================
-    if (lane == 0) {
+    {
+      const uint32_t one = elect_lane();
+      auto wait_all = [&](uint64_t* bar, uint32_t parity) {
+        return bool(__all_sync(0xffffffffu, px_wait(bar, parity, abort_flag)));
+      };
       constexpr uint32_t id_s = mma_idesc(PX_BN, false, false, false), id_o = mma_idesc(DP, false, true, false);
       auto score = [&](int t, int j) {  // S_t = Q_t K_j^T
         const uint8_t *a = sq + t * TILE, *b = ring + ((2 * j) % NST) * TILE;
 #pragma unroll
         for (int ks = 0; ks < DP / 16; ++ks)
-          tc_mma(tmem + 128 * t, sw128_desc(a + (ks >> 2) * HALF) + 2 * (ks & 3),
+          tc_mma_ss(one, tmem + 128 * t, sw128_desc(a + (ks >> 2) * HALF) + 2 * (ks & 3),
                  sw128_desc(b + (ks >> 2) * HALF) + 2 * (ks & 3), id_s, ks > 0);
-        tc_commit(&s_full[t]);
+        tc_commit_by(one, &s_full[t]);
       };
-      auto full_of = [&](int it) { return px_wait(&full[it % NST], uint32_t((it / NST) & 1), abort_flag); };
-      bool ok = px_wait(q_full, 0u, abort_flag) && full_of(0);
+      auto full_of = [&](int it) { return wait_all(&full[it % NST], uint32_t((it / NST) & 1)); };
+      bool ok = wait_all(q_full, 0u) && full_of(0);
       if (ok) {
         tc_fence_after();
         for (int t = 0; t < n_tiles; ++t) score(t, 0);
-        tc_commit(&empty[0]);
+        tc_commit_by(one, &empty[0]);
       }
       for (int j = 0; ok && j < n; ++j) {
         ok = full_of(2 * j + 1);
         for (int t = 0; ok && t < n_tiles; ++t) {
-          ok = px_wait(&p_full[t], uint32_t(j & 1), abort_flag);
+          ok = wait_all(&p_full[t], uint32_t(j & 1));
           if (!ok) break;
           tc_fence_after();
           const uint8_t* v = ring + ((2 * j + 1) % NST) * TILE;
 #pragma unroll
           for (int ks = 0; ks < PX_BN / 16; ++ks)  // O_t += P_t V_j
-            tc_mma_ts(tmem + 256 + DP * t, tmem + 128 * t + 8 * ks, sw128_mn_desc(v + ks * 2048, HALF), id_o,
+            tc_mma_ts(one, tmem + 256 + DP * t, tmem + 128 * t + 8 * ks, sw128_mn_desc(v + ks * 2048, HALF), id_o,
                       j > 0 || ks > 0);
-          tc_commit(&pv_done[t]);
+          tc_commit_by(one, &pv_done[t]);
           if (j + 1 < n) {
             if (t == 0) ok = full_of(2 * j + 2);
             if (ok) score(t, j + 1);
           }
         }
         if (!ok) break;
-        tc_commit(&empty[(2 * j + 1) % NST]);
-        if (j + 1 < n) tc_commit(&empty[(2 * j + 2) % NST]);
+        tc_commit_by(one, &empty[(2 * j + 1) % NST]);
+        if (j + 1 < n) tc_commit_by(one, &empty[(2 * j + 2) % NST]);
       }
       // all MMAs issued by this thread complete before TMEM is released
-      tc_commit(drain);
+      tc_commit_by(one, drain);
       mbar_wait_bounded(drain, 0u, 100000000ull);
     }
     __syncwarp();

@@ -41,7 +41,7 @@ struct PromptParams {
   float* lse;
   float scale2;   // |softmax_scale| * log2(e)
   int negate;     // softmax_scale < 0: the MMA negates Q
-  int B, T, Hq, Hkv, G, D, causal, bf16;
+  int B, T, Hq, Hkv, G, D, causal;
   int tpt;        // tokens per tile
 };
 
@@ -49,7 +49,7 @@ template <int DP>
 struct PromptSmem {
   static constexpr int TILE = 128 * DP * 2;  // bytes of a Q tile, of a K or V block
   static constexpr int STAGES = DP == 128 ? 5 : 8;
-  static constexpr int BARS = 320;
+  static constexpr int BARS = 320;  // barriers, TMEM address, work item
   static constexpr int BYTES = 1024 + 2 * TILE + STAGES * TILE + BARS + 3 * DP * 4;
 };
 
@@ -61,7 +61,7 @@ __device__ __forceinline__ bool wait_or_abort(uint64_t* bar, uint32_t parity, vo
   return false;
 }
 
-template <int DP>
+template <int DP, bool BF16>
 __global__ void __launch_bounds__(PA_THREADS, 1) prompt_attn_kernel(const PromptParams p,
                                                                     const __grid_constant__ CUtensorMap tmq,
                                                                     const __grid_constant__ CUtensorMap tmk,
@@ -75,10 +75,10 @@ __global__ void __launch_bounds__(PA_THREADS, 1) prompt_attn_kernel(const Prompt
   uint8_t* ring = smem + 2 * TILE;  // [NST][TILE], K_0 V_0 K_1 V_1 ...
   uint64_t* bars = reinterpret_cast<uint64_t*>(ring + NST * TILE);
   uint64_t *full = bars, *empty = full + NST, *q_full = empty + NST, *s_full = q_full + 1, *p_full = s_full + 2,
-           *pv_done = p_full + 2, *v_raw = pv_done + 2, *v_fix = v_raw + 3, *drain = v_fix + 3;
+           *pv_done = p_full + 4, *v_raw = pv_done + 2, *v_fix = v_raw + 3, *drain = v_fix + 3;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
-  int* item = reinterpret_cast<int*>(tmem_slot + 2);                                // first row, rows, first token of the item
+  int* item = reinterpret_cast<int*>(tmem_slot + 2);                                // first row, rows, first token of the item; anything in `bad`
   int* bad = reinterpret_cast<int*>(reinterpret_cast<uint8_t*>(bars) + SM::BARS);  // [3][DP] first key: NaN, +inf, -inf
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
 
@@ -128,7 +128,8 @@ __global__ void __launch_bounds__(PA_THREADS, 1) prompt_attn_kernel(const Prompt
     mbar_init(q_full, 1);
     for (int i = 0; i < 2; ++i) {
       mbar_init(&s_full[i], 1);
-      mbar_init(&p_full[i], 4);
+      mbar_init(&p_full[2 * i], 4);
+      mbar_init(&p_full[2 * i + 1], 4);
       mbar_init(&pv_done[i], 1);
     }
     for (int i = 0; i < 3; ++i) {
@@ -137,6 +138,7 @@ __global__ void __launch_bounds__(PA_THREADS, 1) prompt_attn_kernel(const Prompt
     }
     mbar_init(drain, 1);
     *abort_flag = 0;
+    item[3] = 0;
     fence_mbarrier_init();
   }
   for (int i = tid; i < 3 * DP; i += PA_THREADS) bad[i] = 0x7fffffff;
@@ -217,7 +219,7 @@ __global__ void __launch_bounds__(PA_THREADS, 1) prompt_attn_kernel(const Prompt
           *at = make_uint4(0u, 0u, 0u, 0u);
         } else if (p.causal) {
           uint4 w = *at;
-          const uint32_t expo = p.bf16 ? 0x7F80u : 0x7C00u;
+          constexpr uint32_t expo = BF16 ? 0x7F80u : 0x7C00u;
           uint32_t* u = reinterpret_cast<uint32_t*>(&w);
           bool any = false;
 #pragma unroll
@@ -230,6 +232,7 @@ __global__ void __launch_bounds__(PA_THREADS, 1) prompt_attn_kernel(const Prompt
               if ((x & expo) != expo) continue;
               const int cls = (x & ~expo & 0x7FFFu) ? 0 : (x & 0x8000u) ? 2 : 1;
               atomicMin(&bad[cls * DP + 64 * h + 8 * c + k], j * PA_BN + key);
+              item[3] = 1;
               u[k >> 1] &= ~(0xFFFFu << (16 * (k & 1)));
             }
             *at = w;
@@ -243,49 +246,57 @@ __global__ void __launch_bounds__(PA_THREADS, 1) prompt_attn_kernel(const Prompt
     __syncwarp();
   } else if (warp == 8) {
     // ============================ MMA issuer ====================================
-    if (lane == 0) {
-      const uint32_t id_s = mma_idesc(PA_BN, p.bf16, false, p.negate), id_o = mma_idesc(DP, p.bf16, true, false);
+    {
+      const uint32_t one = elect_lane();
+      auto wait_all = [&](uint64_t* bar, uint32_t parity) {
+        return bool(__all_sync(0xffffffffu, wait_or_abort(bar, parity, abort_flag)));
+      };
+      const uint32_t id_s = mma_idesc(PA_BN, BF16, false, p.negate), id_o = mma_idesc(DP, BF16, true, false);
       auto score = [&](int i, int j) {  // S_i = Q_i K_j^T
         const uint8_t *a = sq + i * TILE, *b = ring + ((2 * j) % NST) * TILE;
 #pragma unroll
         for (int ks = 0; ks < DP / 16; ++ks)
-          tc_mma(tmem + 128 * i, sw128_desc(a + (ks >> 2) * HALF) + 2 * (ks & 3),
-                 sw128_desc(b + (ks >> 2) * HALF) + 2 * (ks & 3), id_s, ks > 0);
-        tc_commit(&s_full[i]);
+          tc_mma_ss(one, tmem + 128 * i, sw128_desc(a + (ks >> 2) * HALF) + 2 * (ks & 3),
+                    sw128_desc(b + (ks >> 2) * HALF) + 2 * (ks & 3), id_s, ks > 0);
+        tc_commit_by(one, &s_full[i]);
       };
-      auto full_of = [&](int it) { return wait_or_abort(&full[it % NST], uint32_t((it / NST) & 1), abort_flag); };
-      bool ok = wait_or_abort(q_full, 0u, abort_flag) && full_of(0);
+      auto full_of = [&](int it) { return wait_all(&full[it % NST], uint32_t((it / NST) & 1)); };
+      bool ok = wait_all(q_full, 0u) && full_of(0);
       if (ok) {
         tc_fence_after();
         for (int i = 0; i < 2; ++i)
           if (n_blk[i]) score(i, 0);
-        tc_commit(&empty[0]);
+        tc_commit_by(one, &empty[0]);
       }
       for (int j = 0; ok && j < n_all; ++j) {
-        ok = j < j_mask ? full_of(2 * j + 1) : wait_or_abort(&v_fix[j - j_mask], 0u, abort_flag);
+        ok = j < j_mask ? full_of(2 * j + 1) : wait_all(&v_fix[j - j_mask], 0u);
         bool next = false;  // K_{j+1} has landed
         for (int i = 0; ok && i < 2; ++i) {
           if (j >= n_blk[i]) continue;
-          ok = wait_or_abort(&p_full[i], uint32_t(j & 1), abort_flag);
-          if (!ok) break;
-          tc_fence_after();
           const uint8_t* v = ring + ((2 * j + 1) % NST) * TILE;
+          // O_i += P_i V_j, the first 64 keys while the others' P is formed
+          for (int h = 0; ok && h < 2; ++h) {
+            ok = wait_all(&p_full[2 * i + h], uint32_t(j & 1));
+            if (!ok) break;
+            tc_fence_after();
 #pragma unroll
-          for (int ks = 0; ks < PA_BN / 16; ++ks)  // O_i += P_i V_j
-            tc_mma_ts(tmem + 256 + DP * i, tmem + 128 * i + 8 * ks, sw128_mn_desc(v + ks * 2048, HALF), id_o,
-                      j > 0 || ks > 0);
-          tc_commit(&pv_done[i]);
+            for (int ks = 4 * h; ks < 4 * h + 4; ++ks)
+              tc_mma_ts(one, tmem + 256 + DP * i, tmem + 128 * i + 8 * ks, sw128_mn_desc(v + ks * 2048, HALF), id_o,
+                        j > 0 || ks > 0);
+          }
+          if (!ok) break;
+          tc_commit_by(one, &pv_done[i]);
           if (j + 1 < n_blk[i]) {
             if (!next) ok = next = full_of(2 * j + 2);
             if (ok) score(i, j + 1);
           }
         }
         if (!ok) break;
-        tc_commit(&empty[(2 * j + 1) % NST]);
-        if (j + 1 < n_all) tc_commit(&empty[(2 * j + 2) % NST]);
+        tc_commit_by(one, &empty[(2 * j + 1) % NST]);
+        if (j + 1 < n_all) tc_commit_by(one, &empty[(2 * j + 2) % NST]);
       }
       // all MMAs issued by this thread complete before TMEM is released
-      tc_commit(drain);
+      tc_commit_by(one, drain);
       mbar_wait_bounded(drain, 0u, 100000000ull);
     }
     __syncwarp();
@@ -305,16 +316,14 @@ __global__ void __launch_bounds__(PA_THREADS, 1) prompt_attn_kernel(const Prompt
       tc_fence_after();
       uint32_t s[128];
       tmem_ld128(s_at, s);
-      if (j >= j_mask) {
+      const bool masked = j >= j_mask;
+      if (masked) {
         const int rel = last - j * PA_BN;
 #pragma unroll
         for (int c = 0; c < 128; ++c)
           if (c > rel) s[c] = 0xFF800000u;
       }
-      float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-      for (int c = 0; c < 128; ++c) mx[c & 3] = fmaxf(mx[c & 3], __uint_as_float(s[c]));
-      const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * p.scale2;
+      const float top = row_max(s) * p.scale2;
       if (j == 0) {
         m = top;
       } else {
@@ -328,41 +337,38 @@ __global__ void __launch_bounds__(PA_THREADS, 1) prompt_attn_kernel(const Prompt
           if (move) m = top;
           l *= f;
 #pragma unroll
-          for (int c = 0; c < DP; c += 32) {
-            uint32_t o[32];
-            tmem_ld32(o_at + c, o);
+          for (int c = 0; c < DP; c += 16) {
+            uint32_t o[16];
+            tmem_ld16(o_at + c, o);
 #pragma unroll
-            for (int k = 0; k < 32; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * f);
-            tmem_st32(o_at + c, o);
+            for (int k = 0; k < 16; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * f);
+            tmem_st16(o_at + c, o);
           }
         }
       }
       const float ref = m == -INFINITY ? 0.f : m;
-      float sum[4] = {0.f, 0.f, 0.f, 0.f};
+      uint64_t sum[2] = {0ull, 0ull};
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
+        const uint32_t(&sh)[64] = *reinterpret_cast<const uint32_t(*)[64]>(&s[64 * h]);
         uint32_t pk[32];
-#pragma unroll
-        for (int k = 0; k < 32; ++k) {
-          const float a = ex2(fmaf(__uint_as_float(s[64 * h + 2 * k]), p.scale2, -ref));
-          const float b = ex2(fmaf(__uint_as_float(s[64 * h + 2 * k + 1]), p.scale2, -ref));
-          sum[(2 * k) & 3] += a;
-          sum[(2 * k + 1) & 3] += b;
-          pk[k] = p.bf16 ? pack_bf16x2(a, b) : pack_f16x2(a, b);
-        }
+        if (masked) exp_row<BF16, false>(sh, p.scale2, ref, sum, pk);  // exact zeros
+        else exp_row<BF16, true>(sh, p.scale2, ref, sum, pk);
         tmem_st32(s_at + 32 * h, pk);
+        tmem_wait_st();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&p_full[2 * i + h]);
       }
-      l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
-      tmem_wait_st();
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&p_full[i]);
+      const float2 l2 = f32x2_parts(add_x2(sum[0], sum[1]));
+      l += l2.x + l2.y;
     }
     if (ok && n_blk[i]) {
       ok = __all_sync(0xffffffffu, wait_or_abort(&pv_done[i], uint32_t((n_blk[i] - 1) & 1), abort_flag));
       tc_fence_after();
       const int64_t row = int64_t(row0 + t) * p.Hq + hk * p.G + r % p.G;
       const float inv = l > 0.f ? 1.f / l : l;  // l is NaN where a score is
+      const bool any_bad = *const_cast<volatile int*>(&item[3]) != 0;
       if (ok) {
 #pragma unroll
         for (int c = 0; c < DP; c += 32) {
@@ -375,7 +381,7 @@ __global__ void __launch_bounds__(PA_THREADS, 1) prompt_attn_kernel(const Prompt
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
               x[e] = __uint_as_float(o[k + e]) * inv;
-              if (p.causal) {
+              if (any_bad) {
                 const int d = c + k + e;
                 if (bad[d] <= t) x[e] = __int_as_float(0x7fffffff);
                 if (bad[DP + d] <= t) x[e] += INFINITY;
@@ -385,7 +391,7 @@ __global__ void __launch_bounds__(PA_THREADS, 1) prompt_attn_kernel(const Prompt
             uint32_t w[4];
 #pragma unroll
             for (int e = 0; e < 4; ++e)
-              w[e] = p.bf16 ? pack_bf16x2(x[2 * e], x[2 * e + 1]) : pack_f16x2(x[2 * e], x[2 * e + 1]);
+              w[e] = BF16 ? pack_bf16x2(x[2 * e], x[2 * e + 1]) : pack_f16x2(x[2 * e], x[2 * e + 1]);
             *reinterpret_cast<uint4*>(static_cast<uint16_t*>(p.out) + row * p.D + c + k) =
                 make_uint4(w[0], w[1], w[2], w[3]);
           }
@@ -427,10 +433,10 @@ static int make_rows_map(CUtensorMap* map, const void* base, bool bf16, int64_t 
   return r == CUDA_SUCCESS ? B2F_OK : B2F_ERR_INVALID;
 }
 
-template <int DP>
+template <int DP, bool BF16>
 static int launch_prompt(const PromptParams& p, const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv,
                          unsigned grid, cudaStream_t st) {
-  auto kern = prompt_attn_kernel<DP>;
+  auto kern = prompt_attn_kernel<DP, BF16>;
   const int smem = PromptSmem<DP>::BYTES;
   const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
   if (e != cudaSuccess) {
@@ -474,8 +480,9 @@ extern "C" int b2f_prompt_attn(const void* q, int64_t q_row, int64_t q_head, con
     return rc;
   const float s2 = fabsf(softmax_scale) * kLog2e;
   PromptParams p{cu_seqlens, out, lse, s2 > 1e-30f ? s2 : 1e-30f, softmax_scale < 0.f, int(B), int(T), int(Hq),
-                 int(Hkv), int(G), int(D), causal != 0, bf16, int(tpt)};
+                 int(Hkv), int(G), int(D), causal != 0, int(tpt)};
   cudaStream_t st = as_stream(stream);
-  return D <= 64 ? launch_prompt<64>(p, mq, mk, mv, unsigned(items), st)
-                 : launch_prompt<128>(p, mq, mk, mv, unsigned(items), st);
+  const unsigned n = unsigned(items);
+  if (bf16) return D <= 64 ? launch_prompt<64, true>(p, mq, mk, mv, n, st) : launch_prompt<128, true>(p, mq, mk, mv, n, st);
+  return D <= 64 ? launch_prompt<64, false>(p, mq, mk, mv, n, st) : launch_prompt<128, false>(p, mq, mk, mv, n, st);
 }
