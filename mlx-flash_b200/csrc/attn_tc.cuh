@@ -153,6 +153,40 @@ __device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t (&v)[32
       : "memory");
 }
 
+// OR of a predicate over the `n` threads of named barrier `id`
+__device__ __forceinline__ bool bar_or(int id, int n, bool v) {
+  uint32_t r;
+  asm volatile(
+      "{\n .reg .pred p, q;\n setp.ne.b32 p, %1, 0;\n bar.red.or.pred q, %2, %3, p;\n selp.u32 %0, 1, 0, q;\n}\n"
+      : "=r"(r)
+      : "r"(uint32_t(v)), "r"(id), "r"(n)
+      : "memory");
+  return r != 0;
+}
+__device__ __forceinline__ void bar_all(int id, int n) { asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(n) : "memory"); }
+
+// ---- a running CTA takes over one that has not been launched -----------------
+// The answer (16 bytes in shared memory) lands on `bar`.
+__device__ __forceinline__ void next_cta_ask(void* answer, uint64_t* bar) {
+  asm volatile(
+      "clusterlaunchcontrol.try_cancel.async.shared::cta.mbarrier::complete_tx::bytes.b128 [%0], [%1];" ::"r"(
+          smem_u32(answer)),
+      "r"(smem_u32(bar))
+      : "memory");
+}
+// its blockIdx.x, or -1 when none is left
+__device__ __forceinline__ int next_cta_answer(const void* answer) {
+  uint32_t ok, x;
+  asm volatile(
+      "{\n .reg .b128 a;\n .reg .pred p;\n ld.shared.b128 a, [%2];\n"
+      " clusterlaunchcontrol.query_cancel.is_canceled.pred.b128 p, a;\n selp.u32 %0, 1, 0, p;\n mov.u32 %1, 0;\n"
+      " @p clusterlaunchcontrol.query_cancel.get_first_ctaid.v4.b32.b128 {%1, _, _, _}, a;\n}\n"
+      : "=r"(ok), "=r"(x)
+      : "r"(smem_u32(answer))
+      : "memory");
+  return ok ? int(x) : -1;
+}
+
 // ---- softmax of one score row per thread ------------------------------------
 // Two floats in a 64-bit register: the packed FMA, add and multiply issue once
 // for both.

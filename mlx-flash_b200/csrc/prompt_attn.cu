@@ -7,24 +7,31 @@
 // are staged once for all heads that share them, and only the tile's own
 // tokens, not 128 of them, see a diagonal block.  Per block of 128 keys:
 //   S = Q K^T        tcgen05.mma, Q and K in shared memory (TMA, 128B swizzle)
-//   P = 2^(S c - m)  one thread per row: the row comes out of TMEM into
-//                    registers, the running maximum m and sum l are the
-//                    thread's own (no shuffles), P goes back over S as 16 bits
+//   P = 2^(S c - m)  two threads per row, 64 keys each: the scores come out of
+//                    TMEM into registers, P goes back over S as 16 bits
 //   O += P V         tcgen05.mma with P read from TMEM, V as it lies (MN-major)
 // Softmax in base 2, m and l and O in float32; P is rounded to the inputs'
 // type because the tensor core takes both operands alike (its relative error
 // is that of the output's own rounding).  m is a reference, not the exact
 // maximum: it moves, and O is rescaled, only where a row's new maximum passes
-// it by more than 8 (P stays below 2^8), which after the first blocks is rare,
-// so the rescale lives in the softmax warps and needs no warps of its own.
+// it by more than 8 (P stays below 2^8), which after the first blocks is rare.
+// So a row's two threads have to agree on one bit per block (a reduction in
+// the barrier that keeps P off the scores still being read), and the rescale
+// needs no warps of its own.
 //
-// Warps: 0-3 softmax of tile 0, 4-7 of tile 1 (also the epilogue), 8 issues
-// the MMAs, 9 the TMA loads, 10-11 mend value tiles (below).  The two tiles
-// alternate on the tensor core: while it works on one, the other's softmax
-// runs.
+// Warps: 0-7 softmax of tile 0, 8-15 of tile 1 (also the epilogue), 16 issues
+// the MMAs, 17 plans the items and issues the TMA loads, 18-19 mend value
+// tiles (below).  The two tiles alternate on the tensor core: while it works
+// on one, the other's softmax runs.  One thread per row left a warp of each
+// tile on a scheduler, 2400 cycles a block of softmax and 1250 of MMA in a
+// chain (1.17 PFLOP/s at 16384 tokens); two threads shorten the former.
+//
+// A CTA (one per SM) takes item after item from the grid by cancelling CTAs
+// that have not been launched; the items' roles overlap: loads and the first
+// scores of the next one run under the epilogue of this one.
 //
 // Rows of V that a tile's rows must not see meet P = 0, and 0 * NaN is NaN.
-// So in the blocks in which anything is masked, warps 10-11 zero the rows past
+// So in the blocks in which anything is masked, warps 18-19 zero the rows past
 // the item's last key (they belong to other tokens or sequences) and replace
 // what is not finite by 0, keeping for each column the first key with a NaN,
 // +inf or -inf; the epilogue adds those back to the rows that see them.
@@ -32,8 +39,11 @@
 
 namespace b2f {
 
-constexpr int PA_THREADS = 384;
-constexpr int PA_BN = 128;  // keys per block
+constexpr int PA_THREADS = 640;
+constexpr int PA_BN = 128;         // keys per block
+constexpr int PA_MEND = 4;         // value tiles being mended (3 fit the ring)
+constexpr int PA_STOP = -0x7fffffff - 1;
+constexpr uint32_t PA_NO_BAD = 0x3fffffffu;  // 3 x 10 bits: no key
 
 struct PromptParams {
   const int32_t* cu;
@@ -45,12 +55,25 @@ struct PromptParams {
   int tpt;        // tokens per tile
 };
 
+struct PromptItem {
+  int row0, len, tok0, hk;  // first row and tokens of the sequence, first token of the item, KV head
+};
+
 template <int DP>
 struct PromptSmem {
   static constexpr int TILE = 128 * DP * 2;  // bytes of a Q tile, of a K or V block
   static constexpr int STAGES = DP == 128 ? 5 : 8;
-  static constexpr int BARS = 320;  // barriers, TMEM address, work item
-  static constexpr int BYTES = 1024 + 2 * TILE + STAGES * TILE + BARS + 3 * DP * 4;
+  uint8_t q[2][TILE];
+  uint8_t ring[STAGES][TILE];  // K_0 V_0 K_1 V_1 ...
+  float exchange[2][128];      // between the two threads of a row
+  uint32_t bad[2][DP];         // per column: first key that is NaN | +inf | -inf, from the first masked block on
+  int any_bad[2];
+  PromptItem item[2];
+  uint4 next;  // the answer of next_cta_ask
+  uint64_t full[STAGES], empty[STAGES], q_full, q_empty, s_full[2], p_full[4], pv_done[2], v_raw[PA_MEND],
+      v_fix[PA_MEND], item_full[2], item_empty[2], asked, drain;
+  uint32_t tmem;
+  int abort_flag;
 };
 
 // Waits with the CTA's abort flag; false once any wait gave up.
@@ -61,6 +84,23 @@ __device__ __forceinline__ bool wait_or_abort(uint64_t* bar, uint32_t parity, vo
   return false;
 }
 
+// Blocks of the item's tiles and the first block in which anything is masked.
+struct PromptBlocks {
+  int n[2], all, kend, mask;
+  __device__ __forceinline__ PromptBlocks(const PromptParams& p, const PromptItem& x) {
+    kend = 0;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int t = x.tok0 + i * p.tpt;
+      const int e = t >= x.len ? 0 : p.causal ? min(x.len, t + p.tpt) : x.len;
+      n[i] = (e + PA_BN - 1) / PA_BN;
+      kend = max(kend, e);
+    }
+    all = max(n[0], n[1]);
+    mask = p.causal ? x.tok0 / PA_BN : x.len / PA_BN;  // at most 3 blocks from there: two tiles span <= 256 tokens
+  }
+};
+
 template <int DP, bool BF16>
 __global__ void __launch_bounds__(PA_THREADS, 1) prompt_attn_kernel(const PromptParams p,
                                                                     const __grid_constant__ CUtensorMap tmq,
@@ -70,340 +110,453 @@ __global__ void __launch_bounds__(PA_THREADS, 1) prompt_attn_kernel(const Prompt
   using SM = PromptSmem<DP>;
   constexpr int NST = SM::STAGES, TILE = SM::TILE, HALF = 128 * 128;  // HALF: 64 columns of a tile
   extern __shared__ __align__(1024) uint8_t smem_raw[];
-  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  uint8_t* sq = smem;               // [2][TILE]
-  uint8_t* ring = smem + 2 * TILE;  // [NST][TILE], K_0 V_0 K_1 V_1 ...
-  uint64_t* bars = reinterpret_cast<uint64_t*>(ring + NST * TILE);
-  uint64_t *full = bars, *empty = full + NST, *q_full = empty + NST, *s_full = q_full + 1, *p_full = s_full + 2,
-           *pv_done = p_full + 4, *v_raw = pv_done + 2, *v_fix = v_raw + 3, *drain = v_fix + 3;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
-  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
-  int* item = reinterpret_cast<int*>(tmem_slot + 2);                                // first row, rows, first token of the item; anything in `bad`
-  int* bad = reinterpret_cast<int*>(reinterpret_cast<uint8_t*>(bars) + SM::BARS);  // [3][DP] first key: NaN, +inf, -inf
+  SM& sm = *reinterpret_cast<SM*>(smem_raw);
+  volatile int* abort_flag = &sm.abort_flag;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-
-  // ---- the work item -------------------------------------------------------
-  const int hk = blockIdx.x % p.Hkv;
-  if (warp == 0) {
-    int left = blockIdx.x / p.Hkv, row0 = 0, rows = 0, pair = 0, found = 0;
-    const int span = 2 * p.tpt;
-    // sequence B: the rows past the last sequence
-    for (int b0 = 0; b0 <= p.B && !found; b0 += 32) {
-      const int b = b0 + lane;
-      int lo = 0, hi = 0;
-      if (b <= p.B) {
-        lo = min(max(p.cu[b], 0), p.T);
-        hi = b < p.B ? min(max(p.cu[b + 1], lo), p.T) : p.T;
-      }
-      const int n = (hi - lo + span - 1) / span;
-      int s = n;
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const int a = __shfl_up_sync(0xffffffffu, s, o);
-        if (lane >= o) s += a;
-      }
-      const unsigned hit = __ballot_sync(0xffffffffu, s > left);
-      if (hit) {
-        const int w = __ffs(hit) - 1;
-        row0 = __shfl_sync(0xffffffffu, lo, w);
-        rows = __shfl_sync(0xffffffffu, b0 + w < p.B ? hi - lo : lo - hi, w);  // negative: rows of no sequence
-        // the longest rows of a sequence first: they set the tail of the grid
-        pair = __shfl_sync(0xffffffffu, s, w) - 1 - left;
-        found = 1;
-      } else {
-        left -= __shfl_sync(0xffffffffu, s, 31);
-      }
-    }
-    if (lane == 0) {
-      item[0] = row0;
-      item[1] = rows;
-      item[2] = pair * span;
-    }
-  }
-  if (tid == 32) {
-    for (int s = 0; s < NST; ++s) {
-      mbar_init(&full[s], 1);
-      mbar_init(&empty[s], 1);
-    }
-    mbar_init(q_full, 1);
-    for (int i = 0; i < 2; ++i) {
-      mbar_init(&s_full[i], 1);
-      mbar_init(&p_full[2 * i], 4);
-      mbar_init(&p_full[2 * i + 1], 4);
-      mbar_init(&pv_done[i], 1);
-    }
-    for (int i = 0; i < 3; ++i) {
-      mbar_init(&v_raw[i], 1);
-      mbar_init(&v_fix[i], 2);
-    }
-    mbar_init(drain, 1);
-    *abort_flag = 0;
-    item[3] = 0;
-    fence_mbarrier_init();
-  }
-  for (int i = tid; i < 3 * DP; i += PA_THREADS) bad[i] = 0x7fffffff;
-  __syncthreads();
-  const int row0 = item[0], len = item[1], tok0 = item[2];
-  if (len <= 0) {
-    // rows of no sequence: zeros (the grid's spare items have none)
-    const int n = min(2 * p.tpt, -len - tok0);
-    for (int i = tid; i < n * p.G; i += PA_THREADS) {
-      const int64_t r = int64_t(row0 + tok0 + i / p.G) * p.Hq + hk * p.G + i % p.G;
-      for (int d = 0; d < p.D; d += 8)
-        *reinterpret_cast<uint4*>(static_cast<uint16_t*>(p.out) + r * p.D + d) = make_uint4(0u, 0u, 0u, 0u);
-      if (p.lse) p.lse[r] = -INFINITY;
-    }
+  if (smem_u32(smem_raw) & 1023) {  // the swizzled tiles need it; the runtime gives it
+    if (tid == 0) report_timeout(nullptr);
     return;
   }
-  if (warp == 8) {
-    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(512u)
+
+  if (tid == 0) {
+    for (int s = 0; s < NST; ++s) {
+      mbar_init(&sm.full[s], 1);
+      mbar_init(&sm.empty[s], 1);
+    }
+    mbar_init(&sm.q_full, 1);
+    mbar_init(&sm.q_empty, 1);
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&sm.s_full[i], 1);
+      mbar_init(&sm.p_full[2 * i], 4);
+      mbar_init(&sm.p_full[2 * i + 1], 4);
+      mbar_init(&sm.pv_done[i], 1);
+      mbar_init(&sm.item_full[i], 1);
+      mbar_init(&sm.item_empty[i], 19);  // the warps but the planner's
+      sm.any_bad[i] = 0;
+    }
+    for (int i = 0; i < PA_MEND; ++i) {
+      mbar_init(&sm.v_raw[i], 1);
+      mbar_init(&sm.v_fix[i], 2);
+    }
+    mbar_init(&sm.asked, 1);
+    mbar_init(&sm.drain, 1);
+    sm.abort_flag = 0;
+    fence_mbarrier_init();
+  }
+  if (warp == 16) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&sm.tmem)), "r"(512u)
                  : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
+  for (int i = tid; i < 2 * DP; i += PA_THREADS) sm.bad[i / DP][i % DP] = PA_NO_BAD;
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tmem = *tmem_slot;
+  const uint32_t tmem = sm.tmem;
 
-  // keys and blocks of each tile; the first block in which anything is masked
-  int n_blk[2], kend = 0;
-#pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    const int t = tok0 + i * p.tpt;
-    const int e = t >= len ? 0 : p.causal ? min(len, t + p.tpt) : len;
-    n_blk[i] = (e + PA_BN - 1) / PA_BN;
-    kend = max(kend, e);
-  }
-  const int n_all = max(n_blk[0], n_blk[1]);
-  // (at most 3 of them: a pair of tiles spans 256 tokens or fewer)
-  const int j_mask = p.causal ? tok0 / PA_BN : len / PA_BN;
-
-  if (warp == 9) {
-    // ============================ TMA producer ==================================
-    if (lane == 0 && !producers_stalled()) {  // test control: stalled producers issue nothing
-      const int qrows = p.tpt * p.G;
-      mbar_arrive_expect_tx(q_full, uint32_t((n_blk[1] ? 2 : 1) * (DP / 64) * qrows * 128));
-      for (int i = 0; i < (n_blk[1] ? 2 : 1); ++i)
-        for (int h = 0; h < DP / 64; ++h)
-          tma_load_4d(sq + i * TILE + h * HALF, &tmq, 64 * h, 0, hk, row0 + tok0 + i * p.tpt, q_full);
-      int it = 0;
-      for (; it < 2 * n_all; ++it) {
-        const int s = it % NST;
-        if (it >= NST && !wait_or_abort(&empty[s], uint32_t((it / NST - 1) & 1), abort_flag)) break;
-        // a value block with masked rows lands on a barrier of its own, for warps 10-11
-        const bool mend = (it & 1) && (it >> 1) >= j_mask;
-        uint64_t* bar = mend ? &v_raw[(it >> 1) - j_mask] : &full[s];
-        if (mend) mbar_arrive(&full[s]);
-        mbar_arrive_expect_tx(bar, uint32_t(TILE));
-        for (int h = 0; h < DP / 64; ++h)
-          tma_load_3d(ring + s * TILE + h * HALF, it & 1 ? &tmv : &tmk, 64 * h, hk, row0 + (it >> 1) * PA_BN, bar);
+  if (warp == 17) {
+    // ============================ items and TMA loads ===========================
+    const int span = 2 * p.tpt;
+    int cta = blockIdx.x, asks = 0, items = 0, it = 0, mends = 0, loads = 0;
+    bool ok = true;
+    // hands `x` to the other warps
+    auto publish = [&](const PromptItem& x) {
+      const int slot = items & 1;
+      ok = items < 2 || __all_sync(0xffffffffu, wait_or_abort(&sm.item_empty[slot], uint32_t((items / 2 - 1) & 1), abort_flag));
+      if (!ok) return;
+      if (sm.any_bad[slot]) {  // left by the item before last
+        for (int i = lane; i < DP; i += 32) sm.bad[slot][i] = PA_NO_BAD;
+        __syncwarp();
+        if (lane == 0) sm.any_bad[slot] = 0;
       }
-      // copies already issued land before the CTA goes away
-      mbar_wait_bounded(q_full, 0u, 100000000ull);
-      for (int k = 1; k <= NST && it - k >= 0; ++k)
-        mbar_wait_bounded(&full[(it - k) % NST], uint32_t(((it - k) / NST) & 1), 100000000ull);
-      for (int j = j_mask; 2 * j + 1 < it; ++j) mbar_wait_bounded(&v_raw[j - j_mask], 0u, 100000000ull);
-    }
-    __syncwarp();
-  } else if (warp >= 10) {
-    // ============================ value tiles with masked rows ==================
-    for (int j = j_mask; j < n_all; ++j) {
-      if (!__all_sync(0xffffffffu, wait_or_abort(&v_raw[j - j_mask], 0u, abort_flag))) break;
-      uint8_t* v = ring + ((2 * j + 1) % NST) * TILE;
-      const int valid = min(PA_BN, kend - j * PA_BN);
-      // a line = 64 columns of one key; warp 10 takes the even lines, 11 the odd
-      for (int line = (warp - 10) * 4 + (lane >> 3); line < 128 * (DP / 64); line += 8) {
-        const int key = line & 127, h = line >> 7, c = lane & 7;
-        uint4* at = reinterpret_cast<uint4*>(v + h * HALF + key * 128 + ((c ^ (key & 7)) << 4));
-        if (key >= valid) {
-          *at = make_uint4(0u, 0u, 0u, 0u);
-        } else if (p.causal) {
-          uint4 w = *at;
-          constexpr uint32_t expo = BF16 ? 0x7F80u : 0x7C00u;
-          uint32_t* u = reinterpret_cast<uint32_t*>(&w);
-          bool any = false;
+      __syncwarp();
+      if (lane == 0) {
+        sm.item[slot] = x;
+        mbar_arrive(&sm.item_full[slot]);
+      }
+      ++items;
+    };
+    while (ok) {
+      if (lane == 0) {
+        fence_proxy_async_smem();  // the last answer has been read
+        mbar_arrive_expect_tx(&sm.asked, 16);
+        next_cta_ask(&sm.next, &sm.asked);
+      }
+      // ---- the item of `cta`; sequence B: the rows past the last sequence ----
+      PromptItem x{0, 0, 0, cta % p.Hkv};
+      int left = cta / p.Hkv;
+      for (int b0 = 0; b0 <= p.B; b0 += 32) {
+        const int b = b0 + lane;
+        int lo = 0, hi = 0;
+        if (b <= p.B) {
+          lo = min(max(p.cu[b], 0), p.T);
+          hi = b < p.B ? min(max(p.cu[b + 1], lo), p.T) : p.T;
+        }
+        const int n = (hi - lo + span - 1) / span;
+        int s = n;
 #pragma unroll
-          for (int k = 0; k < 4; ++k)
-            any |= (u[k] & expo) == expo || ((u[k] >> 16) & expo) == expo;
-          if (any) {
-#pragma unroll
-            for (int k = 0; k < 8; ++k) {
-              const uint32_t x = (u[k >> 1] >> (16 * (k & 1))) & 0xFFFFu;
-              if ((x & expo) != expo) continue;
-              const int cls = (x & ~expo & 0x7FFFu) ? 0 : (x & 0x8000u) ? 2 : 1;
-              atomicMin(&bad[cls * DP + 64 * h + 8 * c + k], j * PA_BN + key);
-              item[3] = 1;
-              u[k >> 1] &= ~(0xFFFFu << (16 * (k & 1)));
+        for (int o = 1; o < 32; o <<= 1) {
+          const int a = __shfl_up_sync(0xffffffffu, s, o);
+          if (lane >= o) s += a;
+        }
+        const unsigned hit = __ballot_sync(0xffffffffu, s > left);
+        if (hit) {
+          const int w = __ffs(hit) - 1;
+          x.row0 = __shfl_sync(0xffffffffu, lo, w);
+          x.len = __shfl_sync(0xffffffffu, b0 + w < p.B ? hi - lo : lo - hi, w);  // negative: rows of no sequence
+          // the longest rows of a sequence first: they set the tail of the grid
+          x.tok0 = (__shfl_sync(0xffffffffu, s, w) - 1 - left) * span;
+          break;
+        }
+        left -= __shfl_sync(0xffffffffu, s, 31);
+      }
+      if (x.len != 0) publish(x);  // 0: a spare CTA of the grid
+      if (ok && x.len > 0) {
+        const PromptBlocks blk(p, x);
+        if (lane == 0 && !producers_stalled()) {  // test control: stalled producers issue nothing
+          auto load = [&](int i) {  // K (even i) or V of block i / 2
+            const int n = it + i, s = n % NST;
+            if (n >= NST && !wait_or_abort(&sm.empty[s], uint32_t((n / NST - 1) & 1), abort_flag)) return false;
+            // a value block with masked rows lands on a barrier of its own, for warps 18-19
+            const int j = i >> 1;
+            const bool mend = (i & 1) && j >= blk.mask;
+            uint64_t* bar = mend ? &sm.v_raw[(mends + j - blk.mask) % PA_MEND] : &sm.full[s];
+            if (mend) mbar_arrive(&sm.full[s]);
+            mbar_arrive_expect_tx(bar, uint32_t(TILE));
+            for (int h = 0; h < DP / 64; ++h)
+              tma_load_3d(sm.ring[s] + h * HALF, i & 1 ? &tmv : &tmk, 64 * h, x.hk, x.row0 + j * PA_BN, bar);
+            return true;
+          };
+          int i = 0;
+          ok = load(i++) && load(i++);
+          ok = ok && (loads == 0 || wait_or_abort(&sm.q_empty, uint32_t((loads - 1) & 1), abort_flag));
+          if (ok) {
+            const int tiles = blk.n[1] ? 2 : 1;
+            mbar_arrive_expect_tx(&sm.q_full, uint32_t(tiles * (DP / 64) * p.tpt * p.G * 128));
+            for (int t = 0; t < tiles; ++t)
+              for (int h = 0; h < DP / 64; ++h)
+                tma_load_4d(sm.q[t] + h * HALF, &tmq, 64 * h, 0, x.hk, x.row0 + x.tok0 + t * p.tpt, &sm.q_full);
+          }
+          while (ok && i < 2 * blk.all) ok = load(i++);
+          if (!ok) {
+            // copies already issued land before the CTA goes away
+            mbar_wait_bounded(&sm.q_full, uint32_t(loads & 1), 100000000ull);
+            for (int k = 1; k <= NST && it + i - k >= 0; ++k) {
+              const int n = it + i - k;
+              mbar_wait_bounded(&sm.full[n % NST], uint32_t((n / NST) & 1), 100000000ull);
             }
-            *at = w;
+            for (int j = blk.mask; 2 * j + 1 < i; ++j) {
+              const int m = mends + j - blk.mask;
+              mbar_wait_bounded(&sm.v_raw[m % PA_MEND], uint32_t((m / PA_MEND) & 1), 100000000ull);
+            }
           }
         }
+        ok = __shfl_sync(0xffffffffu, int(ok), 0) != 0;
+        it += 2 * blk.all;
+        mends += max(0, blk.all - blk.mask);
+        ++loads;
       }
-      fence_proxy_async_smem();
+      // the answer lands whatever happened (a bounded wait)
+      const bool landed = mbar_wait_bounded(&sm.asked, uint32_t(asks++ & 1));
+      if (!__all_sync(0xffffffffu, landed)) {
+        if (lane == 0) *abort_flag = 1;
+        ok = false;
+      }
+      if (!ok) break;
+      cta = next_cta_answer(&sm.next);
       __syncwarp();
-      if (lane == 0) mbar_arrive(&v_fix[j - j_mask]);
+      if (cta < 0) break;
+    }
+    if (ok) publish(PromptItem{0, PA_STOP, 0, 0});
+  } else if (warp >= 18) {
+    // ============================ value tiles with masked rows ==================
+    int it = 0, mends = 0;
+    for (int k = 0;; ++k) {
+      const int slot = k & 1;
+      if (!__all_sync(0xffffffffu, wait_or_abort(&sm.item_full[slot], uint32_t((k / 2) & 1), abort_flag))) break;
+      const PromptItem x = sm.item[slot];
+      if (x.len == PA_STOP) break;
+      bool ok = true;
+      if (x.len > 0) {
+        const PromptBlocks blk(p, x);
+        for (int j = blk.mask; j < blk.all; ++j, ++mends) {
+          const int b = mends % PA_MEND;
+          ok = __all_sync(0xffffffffu, wait_or_abort(&sm.v_raw[b], uint32_t((mends / PA_MEND) & 1), abort_flag));
+          if (!ok) break;
+          uint8_t* v = sm.ring[(it + 2 * j + 1) % NST];
+          const int valid = min(PA_BN, blk.kend - j * PA_BN);
+          // a line = 64 columns of one key; the two warps take four lines each in turn
+          for (int line = (warp - 18) * 4 + (lane >> 3); line < 128 * (DP / 64); line += 8) {
+            const int key = line & 127, h = line >> 7, c = lane & 7;
+            uint4* at = reinterpret_cast<uint4*>(v + h * HALF + key * 128 + ((c ^ (key & 7)) << 4));
+            if (key >= valid) {
+              *at = make_uint4(0u, 0u, 0u, 0u);
+            } else if (p.causal) {
+              uint4 w = *at;
+              constexpr uint32_t expo = BF16 ? 0x7F80u : 0x7C00u;
+              uint32_t* u = reinterpret_cast<uint32_t*>(&w);
+              bool any = false;
+#pragma unroll
+              for (int e = 0; e < 4; ++e) any |= (u[e] & expo) == expo || ((u[e] >> 16) & expo) == expo;
+              if (any) {
+                for (int e = 0; e < 8; ++e) {
+                  const uint32_t y = (u[e >> 1] >> (16 * (e & 1))) & 0xFFFFu;
+                  if ((y & expo) != expo) continue;
+                  const int at10 = (y & ~expo & 0x7FFFu) ? 0 : (y & 0x8000u) ? 20 : 10;  // NaN, +inf, -inf
+                  const uint32_t off = uint32_t((j - blk.mask) * PA_BN + key);
+                  uint32_t* word = &sm.bad[slot][64 * h + 8 * c + e];
+                  uint32_t old = *word, seen;
+                  do {
+                    seen = old;
+                    if (((seen >> at10) & 1023u) <= off) break;
+                    old = atomicCAS(word, seen, (seen & ~(1023u << at10)) | (off << at10));
+                  } while (old != seen);
+                  sm.any_bad[slot] = 1;
+                  u[e >> 1] &= ~(0xFFFFu << (16 * (e & 1)));
+                }
+                *at = w;
+              }
+            }
+          }
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&sm.v_fix[b]);
+        }
+        it += 2 * blk.all;
+      }
+      if (!ok) break;
+      if (lane == 0) mbar_arrive(&sm.item_empty[slot]);
     }
     __syncwarp();
-  } else if (warp == 8) {
+  } else if (warp == 16) {
     // ============================ MMA issuer ====================================
-    {
-      const uint32_t one = elect_lane();
-      auto wait_all = [&](uint64_t* bar, uint32_t parity) {
-        return bool(__all_sync(0xffffffffu, wait_or_abort(bar, parity, abort_flag)));
-      };
-      const uint32_t id_s = mma_idesc(PA_BN, BF16, false, p.negate), id_o = mma_idesc(DP, BF16, true, false);
-      auto score = [&](int i, int j) {  // S_i = Q_i K_j^T
-        const uint8_t *a = sq + i * TILE, *b = ring + ((2 * j) % NST) * TILE;
+    const uint32_t one = elect_lane();
+    const uint32_t id_s = mma_idesc(PA_BN, BF16, false, p.negate), id_o = mma_idesc(DP, BF16, true, false);
+    auto wait_all = [&](uint64_t* bar, uint32_t parity) {
+      return bool(__all_sync(0xffffffffu, wait_or_abort(bar, parity, abort_flag)));
+    };
+    auto full_of = [&](int n) { return wait_all(&sm.full[n % NST], uint32_t((n / NST) & 1)); };
+    auto score = [&](int i, int n) {  // S_i = Q_i K^T, K in the ring at n
+      const uint8_t *a = sm.q[i], *b = sm.ring[n % NST];
 #pragma unroll
-        for (int ks = 0; ks < DP / 16; ++ks)
-          tc_mma_ss(one, tmem + 128 * i, sw128_desc(a + (ks >> 2) * HALF) + 2 * (ks & 3),
-                    sw128_desc(b + (ks >> 2) * HALF) + 2 * (ks & 3), id_s, ks > 0);
-        tc_commit_by(one, &s_full[i]);
-      };
-      auto full_of = [&](int it) { return wait_all(&full[it % NST], uint32_t((it / NST) & 1)); };
-      bool ok = wait_all(q_full, 0u) && full_of(0);
-      if (ok) {
+      for (int ks = 0; ks < DP / 16; ++ks)
+        tc_mma_ss(one, tmem + 128 * i, sw128_desc(a + (ks >> 2) * HALF) + 2 * (ks & 3),
+                  sw128_desc(b + (ks >> 2) * HALF) + 2 * (ks & 3), id_s, ks > 0);
+      tc_commit_by(one, &sm.s_full[i]);
+    };
+    int it = 0, mends = 0, loads = 0;
+    int done[2] = {0, 0};  // blocks of each tile so far
+    bool ok = true;
+    for (int k = 0; ok; ++k) {
+      const int slot = k & 1;
+      ok = wait_all(&sm.item_full[slot], uint32_t((k / 2) & 1));
+      if (!ok) break;
+      const PromptItem x = sm.item[slot];
+      if (x.len == PA_STOP) break;
+      if (x.len > 0) {
+        const PromptBlocks blk(p, x);
+        ok = wait_all(&sm.q_full, uint32_t(loads++ & 1)) && full_of(it);
+        if (!ok) break;
         tc_fence_after();
         for (int i = 0; i < 2; ++i)
-          if (n_blk[i]) score(i, 0);
-        tc_commit_by(one, &empty[0]);
-      }
-      for (int j = 0; ok && j < n_all; ++j) {
-        ok = j < j_mask ? full_of(2 * j + 1) : wait_all(&v_fix[j - j_mask], 0u);
-        bool next = false;  // K_{j+1} has landed
-        for (int i = 0; ok && i < 2; ++i) {
-          if (j >= n_blk[i]) continue;
-          const uint8_t* v = ring + ((2 * j + 1) % NST) * TILE;
-          // O_i += P_i V_j, the first 64 keys while the others' P is formed
-          for (int h = 0; ok && h < 2; ++h) {
-            ok = wait_all(&p_full[2 * i + h], uint32_t(j & 1));
-            if (!ok) break;
-            tc_fence_after();
+          if (blk.n[i]) score(i, it);
+        tc_commit_by(one, &sm.empty[it % NST]);
+        if (blk.all == 1) tc_commit_by(one, &sm.q_empty);
+        for (int j = 0; ok && j < blk.all; ++j) {
+          const int nv = it + 2 * j + 1, nk = nv + 1;
+          if (j < blk.mask) {
+            ok = full_of(nv);
+          } else {
+            ok = wait_all(&sm.v_fix[mends % PA_MEND], uint32_t((mends / PA_MEND) & 1));
+            ++mends;
+          }
+          bool next = false;  // K_{j+1} has landed
+          for (int i = 0; ok && i < 2; ++i) {
+            if (j >= blk.n[i]) continue;
+            const uint8_t* v = sm.ring[nv % NST];
+            for (int h = 0; ok && h < 2; ++h) {  // O_i += P_i V_j
+              ok = wait_all(&sm.p_full[2 * i + h], uint32_t(done[i] & 1));
+              if (!ok) break;
+              tc_fence_after();
 #pragma unroll
-            for (int ks = 4 * h; ks < 4 * h + 4; ++ks)
-              tc_mma_ts(one, tmem + 256 + DP * i, tmem + 128 * i + 8 * ks, sw128_mn_desc(v + ks * 2048, HALF), id_o,
-                        j > 0 || ks > 0);
+              for (int ks = 0; ks < 4; ++ks)
+                tc_mma_ts(one, tmem + 256 + DP * i, tmem + 128 * i + 32 * h + 8 * ks,
+                          sw128_mn_desc(v + (4 * h + ks) * 2048, HALF), id_o, j > 0 || h > 0 || ks > 0);
+            }
+            if (!ok) break;
+            ++done[i];
+            tc_commit_by(one, &sm.pv_done[i]);
+            if (j + 1 < blk.n[i]) {
+              if (!next) ok = next = full_of(nk);
+              if (ok) score(i, nk);
+            }
           }
           if (!ok) break;
-          tc_commit_by(one, &pv_done[i]);
-          if (j + 1 < n_blk[i]) {
-            if (!next) ok = next = full_of(2 * j + 2);
-            if (ok) score(i, j + 1);
-          }
+          tc_commit_by(one, &sm.empty[nv % NST]);
+          if (j + 1 < blk.all) tc_commit_by(one, &sm.empty[nk % NST]);
+          if (j + 2 == blk.all) tc_commit_by(one, &sm.q_empty);  // the last scores are issued
         }
-        if (!ok) break;
-        tc_commit_by(one, &empty[(2 * j + 1) % NST]);
-        if (j + 1 < n_all) tc_commit_by(one, &empty[(2 * j + 2) % NST]);
+        it += 2 * blk.all;
       }
-      // all MMAs issued by this thread complete before TMEM is released
-      tc_commit_by(one, drain);
-      mbar_wait_bounded(drain, 0u, 100000000ull);
+      if (ok && lane == 0) mbar_arrive(&sm.item_empty[slot]);
     }
+    // all MMAs issued complete before TMEM is released
+    tc_commit_by(one, &sm.drain);
+    mbar_wait_bounded(&sm.drain, 0u, 100000000ull);
     __syncwarp();
   } else {
     // ============================ softmax and epilogue ==========================
-    const int i = warp >> 2, r = tid & 127;  // tile, MMA row
-    const int t = tok0 + i * p.tpt + r / p.G;
-    const bool live = r < p.tpt * p.G && t < len;
-    const int last = !live ? -1 : p.causal ? t : len - 1;  // last key the row sees
+    // Threads of a tile leave its loops together: what a wait that gave up
+    // says goes through the tile's barrier first.
+    const int i = warp >> 3, h = (warp >> 2) & 1, r = tid & 127;  // tile, half of the keys, MMA row
+    const int bar = 1 + i;
     const uint32_t lane_at = uint32_t(32 * (warp & 3)) << 16;
-    const uint32_t s_at = tmem + lane_at + 128 * i, o_at = tmem + lane_at + 256 + DP * i;
-    float m = -INFINITY, l = 0.f;  // m: reference of the exponents (scaled scores)
-    bool ok = true;
-    for (int j = 0; j < n_blk[i]; ++j) {
-      ok = __all_sync(0xffffffffu, wait_or_abort(&s_full[i], uint32_t(j & 1), abort_flag));
-      if (!ok) break;
-      tc_fence_after();
-      uint32_t s[128];
-      tmem_ld128(s_at, s);
-      const bool masked = j >= j_mask;
-      if (masked) {
-        const int rel = last - j * PA_BN;
-#pragma unroll
-        for (int c = 0; c < 128; ++c)
-          if (c > rel) s[c] = 0xFF800000u;
+    const uint32_t s_at = tmem + lane_at + 128 * i, o_at = tmem + lane_at + 256 + DP * i + DP / 2 * h;
+    auto wait_all = [&](uint64_t* b, uint32_t parity) {
+      return bool(__all_sync(0xffffffffu, wait_or_abort(b, parity, abort_flag)));
+    };
+    // max (or sum) with the row's other thread
+    auto join = [&](float v, bool add) {
+      if (h) sm.exchange[i][r] = v;
+      bar_all(bar, 256);
+      if (!h) {
+        const float o = sm.exchange[i][r];
+        v = add ? v + o : fmaxf(v, o);
+        sm.exchange[i][r] = v;
       }
-      const float top = row_max(s) * p.scale2;
-      if (j == 0) {
-        m = top;
-      } else {
-        const bool move = top > m + 8.f;
-        if (__any_sync(0xffffffffu, move)) {
-          // O holds blocks up to j - 1 once their product is done
-          ok = __all_sync(0xffffffffu, wait_or_abort(&pv_done[i], uint32_t((j - 1) & 1), abort_flag));
-          if (!ok) break;
-          tc_fence_after();
-          const float f = move ? ex2(m - top) : 1.f;
-          if (move) m = top;
-          l *= f;
-#pragma unroll
-          for (int c = 0; c < DP; c += 16) {
-            uint32_t o[16];
-            tmem_ld16(o_at + c, o);
-#pragma unroll
-            for (int k = 0; k < 16; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * f);
-            tmem_st16(o_at + c, o);
-          }
+      bar_all(bar, 256);
+      return h ? sm.exchange[i][r] : v;
+    };
+    int done = 0;  // blocks of this tile so far
+    for (int k = 0;; ++k) {
+      const int slot = k & 1;
+      bool ok = wait_all(&sm.item_full[slot], uint32_t((k / 2) & 1));
+      if (bar_or(bar, 256, !ok)) break;
+      const PromptItem x = sm.item[slot];
+      if (x.len == PA_STOP) break;
+      if (x.len < 0) {
+        // rows of no sequence: zeros
+        const int n = min(2 * p.tpt, -x.len - x.tok0);
+        for (int e = tid; e < n * p.G; e += 512) {
+          const int64_t row = int64_t(x.row0 + x.tok0 + e / p.G) * p.Hq + x.hk * p.G + e % p.G;
+          for (int d = 0; d < p.D; d += 8)
+            *reinterpret_cast<uint4*>(static_cast<uint16_t*>(p.out) + row * p.D + d) = make_uint4(0u, 0u, 0u, 0u);
+          if (p.lse) p.lse[row] = -INFINITY;
         }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&sm.item_empty[slot]);
+        continue;
       }
-      const float ref = m == -INFINITY ? 0.f : m;
-      uint64_t sum[2] = {0ull, 0ull};
+      const PromptBlocks blk(p, x);
+      const int nb = blk.n[i];
+      const int t = x.tok0 + i * p.tpt + r / p.G;
+      const bool live = r < p.tpt * p.G && t < x.len;
+      const int last = !live ? -1 : p.causal ? t : x.len - 1;  // last key the row sees
+      float m = -INFINITY, l = 0.f;  // m: reference of the exponents (scaled scores)
+      bool quit = false;
+      for (int j = 0; j < nb; ++j, ++done) {
+        ok = ok && wait_all(&sm.s_full[i], uint32_t(done & 1));
+        tc_fence_after();
+        uint32_t s[64];
+        tmem_ld64(s_at + 64 * h, s);
+        const bool masked = j >= blk.mask;
+        if (masked) {
+          const int rel = last - j * PA_BN - 64 * h;
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const uint32_t(&sh)[64] = *reinterpret_cast<const uint32_t(*)[64]>(&s[64 * h]);
+          for (int c = 0; c < 64; ++c)
+            if (c > rel) s[c] = 0xFF800000u;
+        }
+        const float top = row_max(s) * p.scale2;
+        // every score of the tile has been read past this barrier
+        if (bar_or(bar, 256, !ok || j == 0 || top > m + 8.f)) {
+          if (bar_or(bar, 256, !ok)) {
+            quit = true;
+            break;
+          }
+          const float both = join(top, false);
+          const bool move = j == 0 || both > m + 8.f;
+          if (j > 0) {
+            // O holds blocks up to j - 1 once their product is done
+            ok = wait_all(&sm.pv_done[i], uint32_t((done - 1) & 1));
+            tc_fence_after();
+            const float f = move ? ex2(m - both) : 1.f;
+            l *= f;
+            if (__any_sync(0xffffffffu, move)) {
+#pragma unroll
+              for (int c = 0; c < DP / 2; c += 16) {
+                uint32_t o[16];
+                tmem_ld16(o_at + c, o);
+#pragma unroll
+                for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
+                tmem_st16(o_at + c, o);
+              }
+            }
+          }
+          if (move) m = both;
+        }
+        const float ref = m == -INFINITY ? 0.f : m;
+        uint64_t sum[2] = {0ull, 0ull};
         uint32_t pk[32];
-        if (masked) exp_row<BF16, false>(sh, p.scale2, ref, sum, pk);  // exact zeros
-        else exp_row<BF16, true>(sh, p.scale2, ref, sum, pk);
+        if (masked) exp_row<BF16, false>(s, p.scale2, ref, sum, pk);  // exact zeros
+        else exp_row<BF16, true>(s, p.scale2, ref, sum, pk);
         tmem_st32(s_at + 32 * h, pk);
+        const float2 l2 = f32x2_parts(add_x2(sum[0], sum[1]));
+        l += l2.x + l2.y;
         tmem_wait_st();
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(&p_full[2 * i + h]);
+        if (lane == 0) mbar_arrive(&sm.p_full[2 * i + h]);
       }
-      const float2 l2 = f32x2_parts(add_x2(sum[0], sum[1]));
-      l += l2.x + l2.y;
-    }
-    if (ok && n_blk[i]) {
-      ok = __all_sync(0xffffffffu, wait_or_abort(&pv_done[i], uint32_t((n_blk[i] - 1) & 1), abort_flag));
-      tc_fence_after();
-      const int64_t row = int64_t(row0 + t) * p.Hq + hk * p.G + r % p.G;
-      const float inv = l > 0.f ? 1.f / l : l;  // l is NaN where a score is
-      const bool any_bad = *const_cast<volatile int*>(&item[3]) != 0;
-      if (ok) {
+      if (quit) break;
+      if (nb) {
+        l = join(l, true);
+        ok = ok && wait_all(&sm.pv_done[i], uint32_t((done - 1) & 1));
+        tc_fence_after();
+        const int64_t row = int64_t(x.row0 + t) * p.Hq + x.hk * p.G + r % p.G;
+        const float inv = l > 0.f ? 1.f / l : l;  // l is NaN where a score is
+        const bool any_bad = *const_cast<volatile int*>(&sm.any_bad[slot]) != 0;
+        const int seen = t - blk.mask * PA_BN;  // keys up to here, from the first masked block
+        if (ok) {
 #pragma unroll
-        for (int c = 0; c < DP; c += 32) {
-          uint32_t o[32];
-          tmem_ld32(o_at + c, o);
+          for (int c = 0; c < DP / 2; c += 32) {
+            uint32_t o[32];
+            tmem_ld32(o_at + c, o);
 #pragma unroll
-          for (int k = 0; k < 32; k += 8) {
-            if (!live || c + k >= p.D) continue;
-            float x[8];
+            for (int e = 0; e < 32; e += 8) {
+              const int d = DP / 2 * h + c + e;
+              if (!live || d >= p.D) continue;
+              float y[8];
 #pragma unroll
-            for (int e = 0; e < 8; ++e) {
-              x[e] = __uint_as_float(o[k + e]) * inv;
-              if (any_bad) {
-                const int d = c + k + e;
-                if (bad[d] <= t) x[e] = __int_as_float(0x7fffffff);
-                if (bad[DP + d] <= t) x[e] += INFINITY;
-                if (bad[2 * DP + d] <= t) x[e] -= INFINITY;
+              for (int f = 0; f < 8; ++f) {
+                y[f] = __uint_as_float(o[e + f]) * inv;
+                if (any_bad) {
+                  const uint32_t w = sm.bad[slot][d + f];
+                  if (int(w & 1023u) <= seen) y[f] = __int_as_float(0x7fffffff);
+                  if (int((w >> 10) & 1023u) <= seen) y[f] += INFINITY;
+                  if (int((w >> 20) & 1023u) <= seen) y[f] -= INFINITY;
+                }
               }
-            }
-            uint32_t w[4];
+              uint32_t w[4];
 #pragma unroll
-            for (int e = 0; e < 4; ++e)
-              w[e] = BF16 ? pack_bf16x2(x[2 * e], x[2 * e + 1]) : pack_f16x2(x[2 * e], x[2 * e + 1]);
-            *reinterpret_cast<uint4*>(static_cast<uint16_t*>(p.out) + row * p.D + c + k) =
-                make_uint4(w[0], w[1], w[2], w[3]);
+              for (int f = 0; f < 4; ++f)
+                w[f] = BF16 ? pack_bf16x2(y[2 * f], y[2 * f + 1]) : pack_f16x2(y[2 * f], y[2 * f + 1]);
+              *reinterpret_cast<uint4*>(static_cast<uint16_t*>(p.out) + row * p.D + d) =
+                  make_uint4(w[0], w[1], w[2], w[3]);
+            }
+            __syncwarp();
           }
-          __syncwarp();
+          if (live && p.lse && h == 0)
+            p.lse[row] = l > 0.f ? (m + log2f(l)) * 0.6931471805599453f : l == 0.f ? -INFINITY : l;
         }
-        if (live && p.lse) p.lse[row] = l > 0.f ? (m + log2f(l)) * 0.6931471805599453f : l == 0.f ? -INFINITY : l;
+        tc_fence_before();
       }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&sm.item_empty[slot]);
+      // a wait that gave up is told at the next item's barrier (the flag makes that wait fail too)
     }
-    tc_fence_before();
   }
   __syncthreads();
-  if (warp == 8) {
+  if (warp == 16) {
     tc_fence_after();
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
   }
@@ -437,7 +590,8 @@ template <int DP, bool BF16>
 static int launch_prompt(const PromptParams& p, const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv,
                          unsigned grid, cudaStream_t st) {
   auto kern = prompt_attn_kernel<DP, BF16>;
-  const int smem = PromptSmem<DP>::BYTES;
+  const int smem = int(sizeof(PromptSmem<DP>));
+  static_assert(sizeof(PromptSmem<DP>) <= 227 * 1024, "one CTA's shared memory");
   const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
   if (e != cudaSuccess) {
     set_last_cuda_error(e);
