@@ -112,7 +112,8 @@ __global__ void __launch_bounds__(PA_THREADS, 1) prompt_attn_kernel(const Prompt
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   SM& sm = *reinterpret_cast<SM*>(smem_raw);
   volatile int* abort_flag = &sm.abort_flag;
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  // (the shuffles tell the compiler that roles and items are uniform in a warp)
+  const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
   if (smem_u32(smem_raw) & 1023) {  // the swizzled tiles need it; the runtime gives it
     if (tid == 0) report_timeout(nullptr);
     return;
@@ -152,7 +153,7 @@ __global__ void __launch_bounds__(PA_THREADS, 1) prompt_attn_kernel(const Prompt
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tmem = sm.tmem;
+  const uint32_t tmem = __shfl_sync(0xffffffffu, sm.tmem, 0);
 
   if (warp == 17) {
     // ============================ items and TMA loads ===========================
@@ -335,45 +336,61 @@ __global__ void __launch_bounds__(PA_THREADS, 1) prompt_attn_kernel(const Prompt
     auto wait_all = [&](uint64_t* bar, uint32_t parity) {
       return bool(__all_sync(0xffffffffu, wait_or_abort(bar, parity, abort_flag)));
     };
-    auto full_of = [&](int n) { return wait_all(&sm.full[n % NST], uint32_t((n / NST) & 1)); };
-    auto score = [&](int i, int n) {  // S_i = Q_i K^T, K in the ring at n
-      const uint8_t *a = sm.q[i], *b = sm.ring[n % NST];
+    // position in the ring
+    struct Ring {
+      int s = 0;
+      uint32_t phase = 0;
+      __device__ __forceinline__ void next() {
+        if (++s == NST) s = 0, phase ^= 1;
+      }
+    };
+    auto full_of = [&](const Ring& r) { return wait_all(&sm.full[r.s], r.phase); };
+    const uint64_t q_desc = sw128_desc(sm.q[0]), k_desc = sw128_desc(sm.ring[0]), v_desc = sw128_mn_desc(sm.ring[0], HALF);
+    auto score = [&](int i, int stage) {  // S_i = Q_i K^T
+      const uint64_t a = q_desc + uint64_t(i * (TILE >> 4)), b = k_desc + uint64_t(stage * (TILE >> 4));
 #pragma unroll
-      for (int ks = 0; ks < DP / 16; ++ks)
-        tc_mma_ss(one, tmem + 128 * i, sw128_desc(a + (ks >> 2) * HALF) + 2 * (ks & 3),
-                  sw128_desc(b + (ks >> 2) * HALF) + 2 * (ks & 3), id_s, ks > 0);
+      for (int ks = 0; ks < DP / 16; ++ks) {
+        const uint64_t at = (ks >> 2) * (HALF >> 4) + 2 * (ks & 3);
+        tc_mma_ss(one, tmem + 128 * i, a + at, b + at, id_s, ks > 0);
+      }
       tc_commit_by(one, &sm.s_full[i]);
     };
-    int it = 0, mends = 0, loads = 0;
+    Ring ring;
+    int mends = 0, loads = 0;
     int done[2] = {0, 0};  // blocks of each tile so far
     bool ok = true;
     for (int k = 0; ok; ++k) {
       const int slot = k & 1;
       ok = wait_all(&sm.item_full[slot], uint32_t((k / 2) & 1));
       if (!ok) break;
-      const PromptItem x = sm.item[slot];
+      PromptItem x = sm.item[slot];
+      x.row0 = __shfl_sync(0xffffffffu, x.row0, 0);
+      x.len = __shfl_sync(0xffffffffu, x.len, 0);
+      x.tok0 = __shfl_sync(0xffffffffu, x.tok0, 0);
       if (x.len == PA_STOP) break;
       if (x.len > 0) {
         const PromptBlocks blk(p, x);
-        ok = wait_all(&sm.q_full, uint32_t(loads++ & 1)) && full_of(it);
+        ok = wait_all(&sm.q_full, uint32_t(loads++ & 1)) && full_of(ring);
         if (!ok) break;
         tc_fence_after();
         for (int i = 0; i < 2; ++i)
-          if (blk.n[i]) score(i, it);
-        tc_commit_by(one, &sm.empty[it % NST]);
+          if (blk.n[i]) score(i, ring.s);
+        tc_commit_by(one, &sm.empty[ring.s]);
         if (blk.all == 1) tc_commit_by(one, &sm.q_empty);
         for (int j = 0; ok && j < blk.all; ++j) {
-          const int nv = it + 2 * j + 1, nk = nv + 1;
+          ring.next();
+          const Ring rv = ring;  // V_j
           if (j < blk.mask) {
-            ok = full_of(nv);
+            ok = full_of(rv);
           } else {
             ok = wait_all(&sm.v_fix[mends % PA_MEND], uint32_t((mends / PA_MEND) & 1));
             ++mends;
           }
-          bool next = false;  // K_{j+1} has landed
+          if (j + 1 < blk.all) ring.next();  // K_{j+1}
+          bool next = false;                 // it has landed
           for (int i = 0; ok && i < 2; ++i) {
             if (j >= blk.n[i]) continue;
-            const uint8_t* v = sm.ring[nv % NST];
+            const uint64_t v = v_desc + uint64_t(rv.s * (TILE >> 4));
             for (int h = 0; ok && h < 2; ++h) {  // O_i += P_i V_j
               ok = wait_all(&sm.p_full[2 * i + h], uint32_t(done[i] & 1));
               if (!ok) break;
@@ -381,22 +398,22 @@ __global__ void __launch_bounds__(PA_THREADS, 1) prompt_attn_kernel(const Prompt
 #pragma unroll
               for (int ks = 0; ks < 4; ++ks)
                 tc_mma_ts(one, tmem + 256 + DP * i, tmem + 128 * i + 32 * h + 8 * ks,
-                          sw128_mn_desc(v + (4 * h + ks) * 2048, HALF), id_o, j > 0 || h > 0 || ks > 0);
+                          v + (4 * h + ks) * (2048 >> 4), id_o, j > 0 || h > 0 || ks > 0);
             }
             if (!ok) break;
             ++done[i];
             tc_commit_by(one, &sm.pv_done[i]);
             if (j + 1 < blk.n[i]) {
-              if (!next) ok = next = full_of(nk);
-              if (ok) score(i, nk);
+              if (!next) ok = next = full_of(ring);
+              if (ok) score(i, ring.s);
             }
           }
           if (!ok) break;
-          tc_commit_by(one, &sm.empty[nv % NST]);
-          if (j + 1 < blk.all) tc_commit_by(one, &sm.empty[nk % NST]);
+          tc_commit_by(one, &sm.empty[rv.s]);
+          if (j + 1 < blk.all) tc_commit_by(one, &sm.empty[ring.s]);
           if (j + 2 == blk.all) tc_commit_by(one, &sm.q_empty);  // the last scores are issued
         }
-        it += 2 * blk.all;
+        ring.next();
       }
       if (ok && lane == 0) mbar_arrive(&sm.item_empty[slot]);
     }
