@@ -153,6 +153,13 @@ __device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t (&v)[32
       : "memory");
 }
 
+// 32 bytes to a 32-byte aligned address in one store
+__device__ __forceinline__ void store_32b(void* dst, const uint32_t* v) {
+  asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(dst), "r"(v[0]), "r"(v[1]), "r"(v[2]),
+               "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7])
+               : "memory");
+}
+
 // OR of a predicate over the `n` threads of named barrier `id`
 __device__ __forceinline__ bool bar_or(int id, int n, bool v) {
   uint32_t r;

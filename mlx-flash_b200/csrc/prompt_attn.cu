@@ -53,6 +53,7 @@ struct PromptParams {
   int negate;     // softmax_scale < 0: the MMA negates Q
   int B, T, Hq, Hkv, G, D, causal;
   int tpt;        // tokens per tile
+  int wide;       // out takes 32-byte stores
 };
 
 struct PromptItem {
@@ -538,27 +539,33 @@ __global__ void __launch_bounds__(PA_THREADS, 1) prompt_attn_kernel(const Prompt
           for (int c = 0; c < DP / 2; c += 32) {
             uint32_t o[32];
             tmem_ld32(o_at + c, o);
+            if (any_bad) {
 #pragma unroll
-            for (int e = 0; e < 32; e += 8) {
-              const int d = DP / 2 * h + c + e;
-              if (!live || d >= p.D) continue;
-              float y[8];
-#pragma unroll
-              for (int f = 0; f < 8; ++f) {
-                y[f] = __uint_as_float(o[e + f]) * inv;
-                if (any_bad) {
-                  const uint32_t w = sm.bad[slot][d + f];
-                  if (int(w & 1023u) <= seen) y[f] = __int_as_float(0x7fffffff);
-                  if (int((w >> 10) & 1023u) <= seen) y[f] += INFINITY;
-                  if (int((w >> 20) & 1023u) <= seen) y[f] -= INFINITY;
-                }
+              for (int e = 0; e < 32; ++e) {
+                const uint32_t w = sm.bad[slot][DP / 2 * h + c + e];
+                float y = __uint_as_float(o[e]);
+                if (int(w & 1023u) <= seen) y = __int_as_float(0x7fffffff);
+                if (int((w >> 10) & 1023u) <= seen) y += INFINITY;
+                if (int((w >> 20) & 1023u) <= seen) y -= INFINITY;
+                o[e] = __float_as_uint(y);
               }
-              uint32_t w[4];
+            }
+            uint32_t w[16];
 #pragma unroll
-              for (int f = 0; f < 4; ++f)
-                w[f] = BF16 ? pack_bf16x2(y[2 * f], y[2 * f + 1]) : pack_f16x2(y[2 * f], y[2 * f + 1]);
-              *reinterpret_cast<uint4*>(static_cast<uint16_t*>(p.out) + row * p.D + d) =
-                  make_uint4(w[0], w[1], w[2], w[3]);
+            for (int e = 0; e < 16; ++e) {
+              const float y0 = __uint_as_float(o[2 * e]) * inv, y1 = __uint_as_float(o[2 * e + 1]) * inv;
+              w[e] = BF16 ? pack_bf16x2(y0, y1) : pack_f16x2(y0, y1);
+            }
+            const int d = DP / 2 * h + c;
+            uint16_t* dst = static_cast<uint16_t*>(p.out) + row * p.D + d;
+            if (live && p.wide && d + 32 <= p.D) {  // whole 32-byte sectors
+              store_32b(dst, &w[0]);
+              store_32b(dst + 16, &w[8]);
+            } else if (live) {
+#pragma unroll
+              for (int e = 0; e < 4; ++e)
+                if (d + 8 * e < p.D)
+                  *reinterpret_cast<uint4*>(dst + 8 * e) = make_uint4(w[4 * e], w[4 * e + 1], w[4 * e + 2], w[4 * e + 3]);
             }
             __syncwarp();
           }
@@ -651,7 +658,7 @@ extern "C" int b2f_prompt_attn(const void* q, int64_t q_row, int64_t q_head, con
     return rc;
   const float s2 = fabsf(softmax_scale) * kLog2e;
   PromptParams p{cu_seqlens, out, lse, s2 > 1e-30f ? s2 : 1e-30f, softmax_scale < 0.f, int(B), int(T), int(Hq),
-                 int(Hkv), int(G), int(D), causal != 0, int(tpt)};
+                 int(Hkv), int(G), int(D), causal != 0, int(tpt), aligned(out, 32) && D % 16 == 0};
   cudaStream_t st = as_stream(stream);
   const unsigned n = unsigned(items);
   if (bf16) return D <= 64 ? launch_prompt<64, true>(p, mq, mk, mv, n, st) : launch_prompt<128, true>(p, mq, mk, mv, n, st);
