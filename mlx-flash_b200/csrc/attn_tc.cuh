@@ -160,6 +160,16 @@ __device__ __forceinline__ void store_32b(void* dst, const uint32_t* v) {
                : "memory");
 }
 
+// 1-D bulk copy from shared to global memory, and the wait for this thread's
+// copies to have read their source.  16-byte aligned, size % 16 == 0.
+__device__ __forceinline__ void bulk_s2g(void* dst, const void* src, uint32_t bytes) {
+  asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(dst), "r"(smem_u32(src)), "r"(bytes)
+               : "memory");
+}
+__device__ __forceinline__ void bulk_s2g_wait() {
+  asm volatile("cp.async.bulk.commit_group;\n cp.async.bulk.wait_group 0;" ::: "memory");
+}
+
 // OR of a predicate over the `n` threads of named barrier `id`
 __device__ __forceinline__ bool bar_or(int id, int n, bool v) {
   uint32_t r;

@@ -5,10 +5,11 @@
 // prefix of p tokens that is B * p rows of K and V.  Here the query rows of a
 // group -- requests x the G query heads of a KV head -- are the M side of one
 // product with the prefix, which is then read and decoded once for all:
-//   1. prefix: CTA = (2 tiles of 128 rows, KV head, split of the prefix).
-//      S = Q K^T and O = P V on tcgen05 as in prompt_attn.cu; four warps turn
-//      the codes of a block of 128 keys into fp16 tiles in shared memory.
-//   2. own tokens: the paged decode kernels of qkv_attn.cu, writing partials.
+//   1. own tokens: the paged decode kernels of qkv_attn.cu, writing partials.
+//   2. prefix: CTA = (2 tiles of 128 rows, KV head, split of the prefix).
+//      S = Q K^T and O = P V on tcgen05 as in prompt_attn.cu; bulk copies bring
+//      the codes of a block of 128 keys, four warps turn them into fp16 tiles
+//      in shared memory.
 //   3. combine: out = sum 2^(m_s - m) O_s / sum 2^(m_s - m) l_s over splits.
 //
 // fp16 operands: a code is exact in 11 bits, and scale * code costs one
@@ -28,10 +29,10 @@ int launch_own_partials(const __nv_bfloat16* q, const uint8_t* kc, const float* 
                         int bits, float scale, int n_splits, int max_len, float* o_part, float* ml_part,
                         int part_stride, int part_base, cudaStream_t st);
 
-constexpr int PX_THREADS = 416;  // warps 0-7 softmax, 8-11 decode the codes, 12 issues the MMAs
+constexpr int PX_THREADS = 768;  // warps 0-15 softmax, 16-19 decode the codes, 20 issues the MMAs, 21 the copies
 constexpr int PX_BN = 128;       // keys per block
-constexpr int PX_STAGES = 5;     // K and V tiles in flight
-
+constexpr int PX_RAW = 3;        // blocks of codes in flight (K and V count apart)
+constexpr int PX_RING = 3;       // decoded tiles
 struct PrefixParams {
   const __nv_bfloat16* q;
   const uint8_t *kc, *vc;
@@ -39,8 +40,27 @@ struct PrefixParams {
   const int32_t *table, *lens, *off;
   int64_t width;
   float *o_part, *ml_part;
-  float scale2;  // softmax_scale * log2(e)
+  float scale2;   // |softmax_scale| * log2(e)
+  int negate;     // softmax_scale < 0: the MMA negates Q
   int B, Ng, Hq, Hkv, G, P, tpt, n_splits, part_stride, max_prefix;
+  int beside;     // launched to run beside the previous kernel (see launch_prefix)
+};
+
+template <int DP, int BITS>
+struct PrefixSmem {
+  static constexpr int TILE = 128 * DP * 2, RB = DP * BITS / 8, DG = DP / 64;
+  static constexpr int CODES = PX_BN * RB, RAW = CODES + PX_BN * DG * 4;  // codes, then scales
+  static constexpr int PITCH = DP * 4 + 16;                               // bytes between output rows on their way out
+  uint8_t q[2][TILE];           // at the end, with the ring, the output rows
+  uint8_t ring[PX_RING][TILE];  // K_0 V_0 K_1 V_1 ..., fp16
+  uint8_t raw[PX_RAW][RAW];     // the same blocks as codes
+  float exchange[2][128];       // between the two threads of a row
+  float largest[2][4];          // scales of the first block, per decoding warp
+  uint64_t raw_full[PX_RAW], raw_empty[PX_RAW], full[PX_RING], empty[PX_RING], q_full, s_full[2], p_full[4], pv_done[2],
+      drain;
+  int item[4];  // group, first request, requests from there, prefix length
+  uint32_t tmem;
+  int abort_flag;
 };
 
 // 4 codes (the bytes of w) as fp16 (code - top) * scale
@@ -83,37 +103,36 @@ __device__ __forceinline__ bool px_wait(uint64_t* bar, uint32_t parity, volatile
   *abort_flag = 1;
   return false;
 }
-
 template <int DP, int BITS>
 __global__ void __launch_bounds__(PX_THREADS, 1) prefix_attn_kernel(const PrefixParams p) {
-  pdl_enter();
-  constexpr int TILE = 128 * DP * 2, HALF = 128 * 128, NST = PX_STAGES;
-  constexpr int RB = DP * BITS / 8, DG = DP / 64, CPR = RB / 16;  // bytes, scales, 16-byte chunks of a code row
-  constexpr int LPR = CPR < 4 ? CPR : 4;                          // lanes on a row (and rows a lane has)
-  constexpr int CPT = CPR / LPR;                                  // chunks of a row that a lane has
+  if (p.beside) pdl_trigger();
+  else pdl_enter();
+  using SM = PrefixSmem<DP, BITS>;
+  constexpr int TILE = SM::TILE, HALF = 128 * 128, NST = PX_RING;
+  constexpr int RB = SM::RB, DG = SM::DG, CPR = RB / 16;  // bytes, scales, 16-byte chunks of a code row
+  constexpr int LPR = CPR < 4 ? CPR : 4;                  // lanes on a row (and rows a lane has)
+  constexpr int CPT = CPR / LPR;                          // chunks of a row that a lane has
   constexpr float TOP = float((1 << (BITS - 1)) - 1);
   extern __shared__ __align__(1024) uint8_t smem_raw[];
-  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  uint8_t* sq = smem;               // [2][TILE]
-  uint8_t* ring = smem + 2 * TILE;  // [NST][TILE], K_0 V_0 K_1 V_1 ...
-  uint64_t* bars = reinterpret_cast<uint64_t*>(ring + NST * TILE);
-  uint64_t *full = bars, *empty = full + NST, *q_full = empty + NST, *s_full = q_full + 1, *p_full = s_full + 2,
-           *pv_done = p_full + 2, *drain = pv_done + 2;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
-  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
-  int* item = reinterpret_cast<int*>(tmem_slot + 2);        // group, first row, rows of the group
-  float* red = reinterpret_cast<float*>(tmem_slot + 6);     // [2][4] largest scales of the first block
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  SM& sm = *reinterpret_cast<SM*>(smem_raw);
+  volatile int* abort_flag = &sm.abort_flag;
+  // (the shuffles tell the compiler that roles are uniform in a warp)
+  const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
+  if (smem_u32(smem_raw) & 1023) {  // the swizzled tiles need it; the runtime gives it
+    if (tid == 0) report_timeout(nullptr);
+    return;
+  }
 
   const int split = blockIdx.x % p.n_splits, hk = blockIdx.x / p.n_splits % p.Hkv;
   if (warp == 0) {
-    int left = blockIdx.x / p.n_splits / p.Hkv, g = -1, row0 = 0, rows = 0;
+    int left = blockIdx.x / p.n_splits / p.Hkv, g = -1, row0 = 0, rows = 0, len = 0;
     const int span = 2 * p.tpt;
     for (int g0 = 0; g0 < p.Ng && g < 0; g0 += 32) {
-      int lo = 0, hi = 0;
+      int lo = 0, hi = 0, n = 0;
       if (g0 + lane < p.Ng) {
         lo = min(max(p.off[g0 + lane], 0), p.B);
         hi = min(max(p.off[g0 + lane + 1], lo), p.B);
+        n = min(max(p.lens[g0 + lane], 0), p.max_prefix);
       }
       int s = (hi - lo + span - 1) / span;
 #pragma unroll
@@ -126,6 +145,7 @@ __global__ void __launch_bounds__(PX_THREADS, 1) prefix_attn_kernel(const Prefix
         const int w = __ffs(hit) - 1;
         const int before = w ? __shfl_sync(0xffffffffu, s, max(w - 1, 0)) : 0;
         const int a = __shfl_sync(0xffffffffu, lo, w), b = __shfl_sync(0xffffffffu, hi, w);
+        len = __shfl_sync(0xffffffffu, n, w);
         g = g0 + w;
         row0 = a + (left - before) * span;
         rows = b - row0;
@@ -134,375 +154,480 @@ __global__ void __launch_bounds__(PX_THREADS, 1) prefix_attn_kernel(const Prefix
       }
     }
     if (lane == 0) {
-      item[0] = g;
-      item[1] = row0;
-      item[2] = rows;
+      sm.item[0] = g;
+      sm.item[1] = row0;
+      sm.item[2] = rows;
+      sm.item[3] = len;
     }
-  }
-  if (tid == 32) {
+  } else if (tid == 32) {
+    for (int s = 0; s < PX_RAW; ++s) {
+      mbar_init(&sm.raw_full[s], 1);
+      mbar_init(&sm.raw_empty[s], 4);
+    }
     for (int s = 0; s < NST; ++s) {
-      mbar_init(&full[s], 4);
-      mbar_init(&empty[s], 1);
+      mbar_init(&sm.full[s], 4);
+      mbar_init(&sm.empty[s], 1);
     }
-    mbar_init(q_full, 8);
+    mbar_init(&sm.q_full, 16);
     for (int i = 0; i < 2; ++i) {
-      mbar_init(&s_full[i], 1);
-      mbar_init(&p_full[i], 4);
-      mbar_init(&pv_done[i], 1);
+      mbar_init(&sm.s_full[i], 1);
+      mbar_init(&sm.p_full[2 * i], 4);
+      mbar_init(&sm.p_full[2 * i + 1], 4);
+      mbar_init(&sm.pv_done[i], 1);
     }
-    mbar_init(drain, 1);
-    *abort_flag = 0;
+    mbar_init(&sm.drain, 1);
+    sm.abort_flag = 0;
     fence_mbarrier_init();
-  }
-  __syncthreads();
-  const int g = item[0], row0 = item[1], rows = item[2];
-  if (g < 0) return;  // a spare item of the grid
-  const int len = min(max(p.lens[g], 0), p.max_prefix);
-  const int blocks = (len + PX_BN - 1) / PX_BN, per = (blocks + p.n_splits - 1) / p.n_splits;
-  const int j0 = split * per, n = min(blocks, j0 + per) - j0;  // this split's blocks
-  const int n_tiles = rows > p.tpt ? 2 : 1;
-
-  // MMA row r of tile i: request row0 + i * tpt + r / G, query head hk * G + r % G
-  const int i = (warp >> 2) & 1, r = tid & 127;
-  const int req = i * p.tpt + r / p.G;
-  const bool live = warp < 8 && r < p.tpt * p.G && req < rows;
-  const int64_t bh = int64_t(row0 + req) * p.Hq + hk * p.G + r % p.G;
-  const int64_t part = bh * p.part_stride + split;
-  if (n <= 0) {  // fewer blocks than splits
-    if (live) *reinterpret_cast<float2*>(p.ml_part + part * 2) = make_float2(-INFINITY, 0.f);
-    return;
-  }
-  if (warp == 12) {
-    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(512u)
+  } else if (warp == 20) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&sm.tmem)), "r"(512u)
                  : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tmem = *tmem_slot;
+  const uint32_t tmem = __shfl_sync(0xffffffffu, sm.tmem, 0);
+  const int g = __shfl_sync(0xffffffffu, sm.item[0], 0), row0 = __shfl_sync(0xffffffffu, sm.item[1], 0);
+  const int rows = __shfl_sync(0xffffffffu, sm.item[2], 0), len = __shfl_sync(0xffffffffu, sm.item[3], 0);
+  const int blocks = (len + PX_BN - 1) / PX_BN, per = (blocks + p.n_splits - 1) / p.n_splits;
+  const int j0 = split * per;
+  const int n = g < 0 ? 0 : min(blocks, j0 + per) - j0;  // this split's blocks (g < 0: a spare CTA of the grid)
+  const int n_tiles = rows > p.tpt ? 2 : 1;
 
-  if (warp == 12) {
-    // ============================ MMA issuer ====================================
-    {
+  if (warp >= 20) {
+    if (warp == 20 && n > 0) {
+      // ============================ MMA issuer ==================================
       const uint32_t one = elect_lane();
+      const uint32_t id_s = mma_idesc(PX_BN, false, false, p.negate), id_o = mma_idesc(DP, false, true, false);
       auto wait_all = [&](uint64_t* bar, uint32_t parity) {
         return bool(__all_sync(0xffffffffu, px_wait(bar, parity, abort_flag)));
       };
-      constexpr uint32_t id_s = mma_idesc(PX_BN, false, false, false), id_o = mma_idesc(DP, false, true, false);
-      auto score = [&](int t, int j) {  // S_t = Q_t K_j^T
-        const uint8_t *a = sq + t * TILE, *b = ring + ((2 * j) % NST) * TILE;
-#pragma unroll
-        for (int ks = 0; ks < DP / 16; ++ks)
-          tc_mma_ss(one, tmem + 128 * t, sw128_desc(a + (ks >> 2) * HALF) + 2 * (ks & 3),
-                 sw128_desc(b + (ks >> 2) * HALF) + 2 * (ks & 3), id_s, ks > 0);
-        tc_commit_by(one, &s_full[t]);
+      // position in the ring
+      struct Ring {
+        int s = 0;
+        uint32_t phase = 0;
+        __device__ __forceinline__ void next() {
+          if (++s == NST) s = 0, phase ^= 1;
+        }
       };
-      auto full_of = [&](int it) { return wait_all(&full[it % NST], uint32_t((it / NST) & 1)); };
-      bool ok = wait_all(q_full, 0u) && full_of(0);
+      auto full_of = [&](const Ring& r) { return wait_all(&sm.full[r.s], r.phase); };
+      const uint64_t q_desc = sw128_desc(sm.q[0]), k_desc = sw128_desc(sm.ring[0]),
+                     v_desc = sw128_mn_desc(sm.ring[0], HALF);
+      auto score = [&](int t, int stage) {  // S_t = Q_t K^T
+        const uint64_t a = q_desc + uint64_t(t * (TILE >> 4)), b = k_desc + uint64_t(stage * (TILE >> 4));
+#pragma unroll
+        for (int ks = 0; ks < DP / 16; ++ks) {
+          const uint64_t at = (ks >> 2) * (HALF >> 4) + 2 * (ks & 3);
+          tc_mma_ss(one, tmem + 128 * t, a + at, b + at, id_s, ks > 0);
+        }
+        tc_commit_by(one, &sm.s_full[t]);
+      };
+      Ring ring;
+      bool ok = wait_all(&sm.q_full, 0u) && full_of(ring);
       if (ok) {
         tc_fence_after();
-        for (int t = 0; t < n_tiles; ++t) score(t, 0);
-        tc_commit_by(one, &empty[0]);
+        for (int t = 0; t < n_tiles; ++t) score(t, ring.s);
+        tc_commit_by(one, &sm.empty[ring.s]);
       }
       for (int j = 0; ok && j < n; ++j) {
-        ok = full_of(2 * j + 1);
+        ring.next();
+        const Ring rv = ring;  // V_j
+        ok = full_of(rv);
+        if (j + 1 < n) ring.next();  // K_{j+1}
         for (int t = 0; ok && t < n_tiles; ++t) {
-          ok = wait_all(&p_full[t], uint32_t(j & 1));
-          if (!ok) break;
-          tc_fence_after();
-          const uint8_t* v = ring + ((2 * j + 1) % NST) * TILE;
+          const uint64_t v = v_desc + uint64_t(rv.s * (TILE >> 4));
+          for (int h = 0; ok && h < 2; ++h) {  // O_t += P_t V_j
+            ok = wait_all(&sm.p_full[2 * t + h], uint32_t(j & 1));
+            if (!ok) break;
+            tc_fence_after();
 #pragma unroll
-          for (int ks = 0; ks < PX_BN / 16; ++ks)  // O_t += P_t V_j
-            tc_mma_ts(one, tmem + 256 + DP * t, tmem + 128 * t + 8 * ks, sw128_mn_desc(v + ks * 2048, HALF), id_o,
-                      j > 0 || ks > 0);
-          tc_commit_by(one, &pv_done[t]);
+            for (int ks = 0; ks < 4; ++ks)
+              tc_mma_ts(one, tmem + 256 + DP * t, tmem + 128 * t + 64 * h + 8 * ks, v + (4 * h + ks) * (2048 >> 4), id_o,
+                        j > 0 || h > 0 || ks > 0);
+          }
+          if (!ok) break;
+          tc_commit_by(one, &sm.pv_done[t]);
           if (j + 1 < n) {
-            if (t == 0) ok = full_of(2 * j + 2);
-            if (ok) score(t, j + 1);
+            if (t == 0) ok = full_of(ring);
+            if (ok) score(t, ring.s);
           }
         }
         if (!ok) break;
-        tc_commit_by(one, &empty[(2 * j + 1) % NST]);
-        if (j + 1 < n) tc_commit_by(one, &empty[(2 * j + 2) % NST]);
+        tc_commit_by(one, &sm.empty[rv.s]);
+        if (j + 1 < n) tc_commit_by(one, &sm.empty[ring.s]);
       }
-      // all MMAs issued by this thread complete before TMEM is released
-      tc_commit_by(one, drain);
-      mbar_wait_bounded(drain, 0u, 100000000ull);
+      // all MMAs issued complete before TMEM is released
+      tc_commit_by(one, &sm.drain);
+      mbar_wait_bounded(&sm.drain, 0u, 100000000ull);
+      __syncwarp();
+    } else if (warp == 21 && n > 0 && !producers_stalled()) {  // test control: stalled producers issue nothing
+      // ============================ copies of codes and scales ==================
+      // 16 keys a lane (pages hold a multiple of 16): lanes 0-7 bring K, 8-15 V.
+      const int32_t* pages = p.table + int64_t(g) * p.width;
+      const int part = lane & 7;
+      const bool is_v = lane & 8;
+      const uint8_t* codes = is_v ? p.vc : p.kc;
+      const float* scales = is_v ? p.vs : p.ks;
+      auto page_of = [&](int j) {
+        const int key = (j0 + j) * PX_BN + 16 * part;
+        return lane < 16 && j < n && key < len ? max(pages[key / p.P], 0) : -1;
+      };
+      int page = page_of(0);
+      bool ok = true;
+      int it = 0;
+      for (int j = 0; ok && j < n; ++j) {
+        const int key = (j0 + j) * PX_BN + 16 * part;
+        const int keys = min(PX_BN, (len - (j0 + j) * PX_BN + 15) & ~15);  // of the block, in whole sixteens
+        const int64_t row = (int64_t(page) * p.Hkv + hk) * p.P + key % p.P;
+        const bool have = page >= 0;
+        page = page_of(j + 1);
+        for (int v = 0; ok && v < 2; ++v, ++it) {
+          const int s = it % PX_RAW;
+          ok = it < PX_RAW || __all_sync(0xffffffffu, px_wait(&sm.raw_empty[s], uint32_t((it / PX_RAW - 1) & 1), abort_flag));
+          if (!ok) break;
+          if (lane == 0) mbar_arrive_expect_tx(&sm.raw_full[s], uint32_t(keys) * (RB + DG * 4));
+          __syncwarp();
+          if (have && is_v == bool(v)) {
+            bulk_g2s(sm.raw[s] + 16 * part * RB, codes + row * RB, 16 * RB, &sm.raw_full[s]);
+            bulk_g2s(sm.raw[s] + SM::CODES + 16 * part * DG * 4, scales + row * DG, 16 * DG * 4, &sm.raw_full[s]);
+          }
+        }
+      }
+      // copies already issued land before the CTA goes away
+      for (int k = 1; k <= PX_RAW && it - k >= 0; ++k)
+        mbar_wait_bounded(&sm.raw_full[(it - k) % PX_RAW], uint32_t(((it - k) / PX_RAW) & 1), 100000000ull);
+      __syncwarp();
     }
-    __syncwarp();
-  } else if (warp >= 8) {
+  } else if (warp >= 16) {
     // ============================ codes -> fp16 tiles ===========================
     // Lane t has rows t / LPR + (128 / LPR) * k and chunks t % LPR + LPR * c of
-    // each: 64-byte runs of a row in global memory, and stores whose 8 lanes of
-    // a phase hit 8 different 16-byte columns of the swizzled tile.
-    const int t = tid - 256, sub = t % LPR;
-    const int32_t* pages = p.table + int64_t(g) * p.width;
-    const bool stall = producers_stalled();  // test control: nothing is produced
-    uint4 kq[LPR][CPT], vq[LPR][CPT];
-    float kscale[LPR][CPT], vscale[LPR][CPT];
-    int64_t rid[LPR];
-    int page[LPR];
-    auto key_of = [&](int j, int k) { return (j0 + j) * PX_BN + t / LPR + (128 / LPR) * k; };
-    auto load_pages = [&](int j) {
-#pragma unroll
-      for (int k = 0; k < LPR; ++k) {
-        const int key = key_of(j, k);
-        page[k] = j < n && key < len ? pages[key / p.P] : -1;
-      }
-    };
-    auto load = [&](const uint8_t* codes, const float* scales, uint4 (&w)[LPR][CPT], float (&s)[LPR][CPT]) {
-#pragma unroll
-      for (int k = 0; k < LPR; ++k)
-#pragma unroll
-        for (int c = 0; c < CPT; ++c) {
-          const int chunk = sub + LPR * c;
-          const bool in = rid[k] >= 0;
-          w[k][c] = in ? *reinterpret_cast<const uint4*>(codes + rid[k] * RB + chunk * 16) : make_uint4(0u, 0u, 0u, 0u);
-          s[k][c] = in ? scales[rid[k] * DG + chunk * (128 / BITS) / 64] : 0.f;
-        }
-    };
-    auto rows_of = [&](int j) {
-#pragma unroll
-      for (int k = 0; k < LPR; ++k)
-        rid[k] = page[k] < 0 ? -1 : (int64_t(page[k]) * p.Hkv + hk) * p.P + key_of(j, k) % p.P;
-    };
+    // each: the stores of a phase's 8 lanes hit 8 different 16-byte columns of
+    // the swizzled tile.
+    const int t = tid - 512, sub = t % LPR;
     constexpr uint32_t OFF = 0x64006400u + uint32_t(TOP) * 0x00010001u;  // 1024 + TOP, twice
-    auto store = [&](int it, const uint4 (&w)[LPR][CPT], const float (&s)[LPR][CPT], float norm) {
-      const int st = it % NST;
-      bool ok = it < NST || px_wait(&empty[st], uint32_t((it / NST - 1) & 1), abort_flag);
-      ok = __all_sync(0xffffffffu, ok) && !stall;
-      if (!ok) return false;
+    float norm[2] = {1.f, 1.f};  // K, V
+    bool ok = true;
+    for (int it = 0; ok && it < 2 * n; ++it) {
+      const int s = it % PX_RAW, st = it % NST, j = it >> 1;
+      if (it == 0) {
+        // references from the first block: its largest scales of K and of V
+        // (PX_RAW blocks are in flight: V's has been asked for too)
+        float top[2] = {0.f, 0.f};
+        for (int v = 0; v < 2; ++v) {
+          ok = ok && __all_sync(0xffffffffu, px_wait(&sm.raw_full[v], 0u, abort_flag));
+          const float* sc = reinterpret_cast<const float*>(sm.raw[v] + SM::CODES);
+          if (ok && t < len - j0 * PX_BN)
+            for (int e = 0; e < DG; ++e)
+              if (sc[t * DG + e] < INFINITY) top[v] = fmaxf(top[v], sc[t * DG + e]);
+          top[v] = warp_max<32>(top[v]);
+          if (lane == 0) sm.largest[v][warp - 16] = top[v];
+        }
+        bar_all(3, 128);
+        // the largest value of the first block lands in [2^(BITS-8), 2^(BITS-6))
+        for (int v = 0; v < 2; ++v)
+          norm[v] = pow2_inverse(fmaxf(fmaxf(sm.largest[v][0], sm.largest[v][1]),
+                                       fmaxf(sm.largest[v][2], sm.largest[v][3])), -7);
+      } else {
+        ok = __all_sync(0xffffffffu, px_wait(&sm.raw_full[s], uint32_t((it / PX_RAW) & 1), abort_flag));
+      }
+      ok = ok && (it < NST || __all_sync(0xffffffffu, px_wait(&sm.empty[st], uint32_t((it / NST - 1) & 1), abort_flag)));
+      if (!ok) break;
+      const int valid = len - (j0 + j) * PX_BN;  // keys of the block (128 or more: all)
+      const float* scales = reinterpret_cast<const float*>(sm.raw[s] + SM::CODES);
 #pragma unroll
       for (int k = 0; k < LPR; ++k) {
         const int row = t / LPR + (128 / LPR) * k;
 #pragma unroll
         for (int c = 0; c < CPT; ++c) {
-          const float sc = s[k][c] * norm;
-          const float sat = sc > 256.f ? 256.f : sc;  // 255 * 256 is the last fp16 value; NaN stays
-          const __half2 h2 = __float2half2_rn(sat);
+          const int chunk = sub + LPR * c;
+          const bool in = row < valid;
+          const uint4 w = *reinterpret_cast<const uint4*>(sm.raw[s] + row * RB + chunk * 16);
+          const float sc = in ? scales[row * DG + chunk * (128 / BITS) / 64] * norm[it & 1] : 0.f;
+          const __half2 h2 = __float2half2_rn(sc > 256.f ? 256.f : sc);  // 255 * 256 is the last fp16 value; NaN stays
           const uint32_t s2 = *reinterpret_cast<const uint32_t*>(&h2);
           uint32_t b[32 / BITS];
-          spread_codes<BITS>(w[k][c], b);
-          const int col = (sub + LPR * c) * (16 / BITS);  // first 8-value column of the chunk
+          spread_codes<BITS>(w, b);
+          const int col = chunk * (16 / BITS);  // first 8-value column of the chunk
 #pragma unroll
           for (int x = 0; x < 16 / BITS; ++x) {
             const uint2 lo = codes_to_f16(b[2 * x], OFF, s2), hi = codes_to_f16(b[2 * x + 1], OFF, s2);
             const int cc = col + x;
-            *reinterpret_cast<uint4*>(ring + st * TILE + (cc >> 3) * HALF + row * 128 + (((cc & 7) ^ (row & 7)) << 4)) =
+            *reinterpret_cast<uint4*>(sm.ring[st] + (cc >> 3) * HALF + row * 128 + (((cc & 7) ^ (row & 7)) << 4)) =
                 make_uint4(lo.x, lo.y, hi.x, hi.y);
           }
         }
       }
       fence_proxy_async_smem();
       __syncwarp();
-      if (lane == 0) mbar_arrive(&full[st]);
-      return true;
-    };
-    load_pages(0);
-    rows_of(0);
-    load(p.kc, p.ks, kq, kscale);
-    load(p.vc, p.vs, vq, vscale);
-    load_pages(1);
-    float km = 0.f, vm = 0.f;
-#pragma unroll
-    for (int k = 0; k < LPR; ++k)
-#pragma unroll
-      for (int c = 0; c < CPT; ++c) {
-        if (kscale[k][c] < INFINITY) km = fmaxf(km, kscale[k][c]);
-        if (vscale[k][c] < INFINITY) vm = fmaxf(vm, vscale[k][c]);
+      if (lane == 0) {
+        mbar_arrive(&sm.raw_empty[s]);
+        mbar_arrive(&sm.full[st]);
       }
-    km = warp_max<32>(km);
-    vm = warp_max<32>(vm);
-    if (lane == 0) {
-      red[warp - 8] = km;
-      red[4 + warp - 8] = vm;
-    }
-    named_sync(128);
-    // the largest value of the first block lands in [2^(BITS-8), 2^(BITS-6))
-    const float kn = pow2_inverse(fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3])), -7);
-    const float vn = pow2_inverse(fmaxf(fmaxf(red[4], red[5]), fmaxf(red[6], red[7])), -7);
-    for (int j = 0; j < n; ++j) {
-      if (!store(2 * j, kq, kscale, kn)) break;
-      rows_of(j + 1);
-      load(p.kc, p.ks, kq, kscale);
-      load_pages(j + 2);
-      if (!store(2 * j + 1, vq, vscale, vn)) break;
-      load(p.vc, p.vs, vq, vscale);
     }
     __syncwarp();
   } else {
     // ============================ queries, softmax, partials ====================
-    float zs = 0.f;  // scores in base 2 = S * zs
-    if (i < n_tiles) {
-      // this thread's query row, scaled by a power of two into fp16
-      uint4 w[DP / 8];
+    // Two threads a row, 64 keys (and half the columns of O) each; threads of
+    // a tile leave its loops together: what a wait that gave up says goes
+    // through the tile's barrier first.
+    const int i = warp >> 3, h = (warp >> 2) & 1, r = tid & 127;  // tile, half of the keys, MMA row
+    const int bar = 1 + i;
+    // MMA row r of tile i: request row0 + i * tpt + r / G, query head hk * G + r % G
+    const int req = i * p.tpt + r / p.G;
+    const bool live = g >= 0 && r < p.tpt * p.G && req < rows;
+    const int64_t bh = int64_t(row0 + req) * p.Hq + hk * p.G + r % p.G;
+    const int64_t part = bh * p.part_stride + split;
+    auto wait_all = [&](uint64_t* b, uint32_t parity) {
+      return bool(__all_sync(0xffffffffu, px_wait(b, parity, abort_flag)));
+    };
+    if (n <= 0) {  // fewer blocks than splits
+      if (live && h == 0) *reinterpret_cast<float2*>(p.ml_part + part * 2) = make_float2(-INFINITY, 0.f);
+    } else if (i < n_tiles) {
+      // ---- this row's query, scaled by a power of two into fp16; a half of its columns each ----
+      constexpr int QC = DP / 16;  // 16-byte pieces of a half
+      uint4 w[QC];
 #pragma unroll
-      for (int c = 0; c < DP / 8; ++c)
-        w[c] = live ? reinterpret_cast<const uint4*>(p.q + bh * DP)[c] : make_uint4(0u, 0u, 0u, 0u);
+      for (int c = 0; c < QC; ++c)
+        w[c] = live ? reinterpret_cast<const uint4*>(p.q + bh * DP)[h * QC + c] : make_uint4(0u, 0u, 0u, 0u);
       float top = 0.f;
 #pragma unroll
-      for (int c = 0; c < DP / 8; ++c) {
-        const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(&w[c]);
+      for (int c = 0; c < QC; ++c) {
+        const __nv_bfloat162* e = reinterpret_cast<const __nv_bfloat162*>(&w[c]);
 #pragma unroll
-        for (int k = 0; k < 4; ++k) top = fmaxf(top, fmaxf(fabsf(__low2float(h[k])), fabsf(__high2float(h[k]))));
+        for (int k = 0; k < 4; ++k) top = fmaxf(top, fmaxf(fabsf(__low2float(e[k])), fabsf(__high2float(e[k]))));
       }
-      const float qn = pow2_inverse(top, 0);
-      zs = p.scale2 / qn;
+      // max (or sum) with the row's other thread
+      auto join = [&](float v, bool add) {
+        if (h) sm.exchange[i][r] = v;
+        bar_all(bar, 256);
+        if (!h) {
+          const float o = sm.exchange[i][r];
+          v = add ? v + o : fmaxf(v, o);
+          sm.exchange[i][r] = v;
+        }
+        bar_all(bar, 256);
+        return h ? sm.exchange[i][r] : v;
+      };
+      const float qn = pow2_inverse(join(top, false), 0);
 #pragma unroll
-      for (int c = 0; c < DP / 8; ++c) {
-        const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(&w[c]);
+      for (int c = 0; c < QC; ++c) {
+        const __nv_bfloat162* e = reinterpret_cast<const __nv_bfloat162*>(&w[c]);
         uint32_t x[4];
 #pragma unroll
-        for (int k = 0; k < 4; ++k) x[k] = pack_f16x2(__low2float(h[k]) * qn, __high2float(h[k]) * qn);
-        *reinterpret_cast<uint4*>(sq + i * TILE + (c >> 3) * HALF + r * 128 + (((c & 7) ^ (r & 7)) << 4)) =
+        for (int k = 0; k < 4; ++k) x[k] = pack_f16x2(__low2float(e[k]) * qn, __high2float(e[k]) * qn);
+        const int cc = h * QC + c;
+        *reinterpret_cast<uint4*>(sm.q[i] + (cc >> 3) * HALF + r * 128 + (((cc & 7) ^ (r & 7)) << 4)) =
             make_uint4(x[0], x[1], x[2], x[3]);
       }
-    }
-    fence_proxy_async_smem();
-    __syncwarp();
-    if (lane == 0) mbar_arrive(q_full);
-    const uint32_t lane_at = uint32_t(32 * (warp & 3)) << 16;
-    const uint32_t s_at = tmem + lane_at + 128 * i, o_at = tmem + lane_at + 256 + DP * i;
-    float m = -INFINITY, l = 0.f;  // m: reference of the exponents
-    bool ok = true;
-    if (i < n_tiles) {
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&sm.q_full);
+      const uint32_t lane_at = uint32_t(32 * (warp & 3)) << 16;
+      const uint32_t s_at = tmem + lane_at + 128 * i + 64 * h, o_at = tmem + lane_at + 256 + DP * i + DP / 2 * h;
+      float zs = p.scale2 / qn;  // scores in base 2 = S * zs, once K's reference is known
+      float m = -INFINITY, l = 0.f;  // m: reference of the exponents
+      bool ok = true, quit = false;
       for (int j = 0; j < n; ++j) {
-        ok = __all_sync(0xffffffffu, px_wait(&s_full[i], uint32_t(j & 1), abort_flag));
-        if (!ok) break;
+        ok = ok && wait_all(&sm.s_full[i], uint32_t(j & 1));
         tc_fence_after();
-        if (j == 0) zs /= pow2_inverse(fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3])), -7);
-        const int valid = len - (j0 + j) * PX_BN;  // keys of the block (128 or more: all)
-        float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+        if (j == 0)
+          zs /= pow2_inverse(fmaxf(fmaxf(sm.largest[0][0], sm.largest[0][1]), fmaxf(sm.largest[0][2], sm.largest[0][3])), -7);
+        const int valid = len - (j0 + j) * PX_BN - 64 * h;  // keys of this half (64 or more: all)
+        const bool masked = valid < 64;
+        // the scores are read twice, 32 at a time: 64 at once and P do not fit 80 registers
+        auto scores = [&](int c, uint32_t (&s)[32]) {
+          tmem_ld32(s_at + c, s);
+          if (masked) {
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          uint32_t s[64];
-          tmem_ld64(s_at + 64 * h, s);
-#pragma unroll
-          for (int c = 0; c < 64; ++c) {
-            const float z = __uint_as_float(s[c]) * zs;
-            if (64 * h + c < valid) mx[c & 3] = fmaxf(mx[c & 3], z);
+            for (int k = 0; k < 32; ++k)
+              if (c + k >= valid) s[k] = 0xFF800000u;
           }
+        };
+        float mx = -INFINITY;
+#pragma unroll
+        for (int c = 0; c < 64; c += 32) {
+          uint32_t s[32];
+          scores(c, s);
+          mx = fmaxf(mx, row_max(s));
         }
-        const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
-        if (j == 0) {
-          m = top;
-        } else {
-          const bool move = top > m + 8.f;
-          if (__any_sync(0xffffffffu, move)) {
-            ok = __all_sync(0xffffffffu, px_wait(&pv_done[i], uint32_t((j - 1) & 1), abort_flag));
-            if (!ok) break;
+        mx *= zs;
+        if (bar_or(bar, 256, !ok || j == 0 || mx > m + 8.f)) {
+          if (bar_or(bar, 256, !ok)) {
+            quit = true;
+            break;
+          }
+          const float both = join(mx, false);
+          const bool move = j == 0 || both > m + 8.f;
+          if (j > 0) {
+            // O holds blocks up to j - 1 once their product is done
+            ok = wait_all(&sm.pv_done[i], uint32_t((j - 1) & 1));
             tc_fence_after();
-            const float f = move ? ex2(m - top) : 1.f;
-            if (move) m = top;
+            const float f = move ? ex2(m - both) : 1.f;
             l *= f;
+            if (__any_sync(0xffffffffu, move)) {
 #pragma unroll
-            for (int c = 0; c < DP; c += 32) {
-              uint32_t o[32];
-              tmem_ld32(o_at + c, o);
+              for (int c = 0; c < DP / 2; c += 16) {
+                uint32_t o[16];
+                tmem_ld16(o_at + c, o);
 #pragma unroll
-              for (int k = 0; k < 32; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * f);
-              tmem_st32(o_at + c, o);
+                for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
+                tmem_st16(o_at + c, o);
+              }
             }
           }
+          if (move) m = both;
         }
         const float ref = m == -INFINITY ? 0.f : m;
-        float sum[4] = {0.f, 0.f, 0.f, 0.f};
-        uint32_t pk[2][32];
+        uint64_t sum[2] = {0ull, 0ull};
+        uint32_t pk[2][16];
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          uint32_t s[64];
-          tmem_ld64(s_at + 64 * h, s);
-#pragma unroll
-          for (int k = 0; k < 32; ++k) {
-            float e[2];
-#pragma unroll
-            for (int x = 0; x < 2; ++x) {
-              const int c = 2 * k + x;
-              e[x] = 64 * h + c < valid ? ex2(fmaf(__uint_as_float(s[c]), zs, -ref)) : 0.f;
-              sum[c & 3] += e[x];
-            }
-            pk[h][k] = pack_f16x2(e[0], e[1]);
-          }
+        for (int c = 0; c < 2; ++c) {
+          uint32_t s[32];
+          scores(32 * c, s);
+          if (masked) exp_row<false, false>(s, zs, ref, sum, pk[c]);  // exact zeros
+          else exp_row<false, true>(s, zs, ref, sum, pk[c]);
         }
-        // P goes over S once every column of S has been read
-        tmem_st32(s_at, pk[0]);
-        tmem_st32(s_at + 32, pk[1]);
-        l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+        // P goes over this thread's own scores
+        tmem_st16(s_at, pk[0]);
+        tmem_st16(s_at + 16, pk[1]);
+        const float2 l2 = f32x2_parts(add_x2(sum[0], sum[1]));
+        l += l2.x + l2.y;
         tmem_wait_st();
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(&p_full[i]);
+        if (lane == 0) mbar_arrive(&sm.p_full[2 * i + h]);
       }
+      // ---- the partial: rows of O through shared memory, then one copy each ----
+      // (the operands have been used up once both tiles' products are done)
+      if (!quit) l = join(l, true);
+      ok = ok && !quit && wait_all(&sm.drain, 0u);
+      tc_fence_after();
       if (ok) {
-        ok = __all_sync(0xffffffffu, px_wait(&pv_done[i], uint32_t((n - 1) & 1), abort_flag));
-        tc_fence_after();
-      }
-      if (ok) {
-        const float back = 1.f / pow2_inverse(fmaxf(fmaxf(red[4], red[5]), fmaxf(red[6], red[7])), -7);
+        const float back = 1.f / pow2_inverse(fmaxf(fmaxf(sm.largest[1][0], sm.largest[1][1]),
+                                                    fmaxf(sm.largest[1][2], sm.largest[1][3])), -7);
+        uint8_t* out = sm.q[0] + (i * 128 + r) * SM::PITCH;
 #pragma unroll
-        for (int c = 0; c < DP; c += 32) {
-          uint32_t o[32];
-          tmem_ld32(o_at + c, o);
-          if (live) {
+        for (int c = 0; c < DP / 2; c += 16) {
+          uint32_t o[16];
+          tmem_ld16(o_at + c, o);
 #pragma unroll
-            for (int k = 0; k < 32; k += 4)
-              *reinterpret_cast<float4*>(p.o_part + part * DP + c + k) =
-                  make_float4(__uint_as_float(o[k]) * back, __uint_as_float(o[k + 1]) * back,
-                              __uint_as_float(o[k + 2]) * back, __uint_as_float(o[k + 3]) * back);
-          }
-          __syncwarp();
+          for (int e = 0; e < 16; e += 4)
+            *reinterpret_cast<float4*>(out + (DP / 2 * h + c + e) * 4) =
+                make_float4(__uint_as_float(o[e]) * back, __uint_as_float(o[e + 1]) * back,
+                            __uint_as_float(o[e + 2]) * back, __uint_as_float(o[e + 3]) * back);
         }
-        if (live) *reinterpret_cast<float2*>(p.ml_part + part * 2) = make_float2(m, l);
+        fence_proxy_async_smem();
       }
+      bar_all(bar, 256);
+      if (ok && live && h == 0) {
+        bulk_s2g(p.o_part + part * DP, sm.q[0] + (i * 128 + r) * SM::PITCH, DP * 4);
+        *reinterpret_cast<float2*>(p.ml_part + part * 2) = make_float2(m, l);
+        bulk_s2g_wait();
+      }
+      tc_fence_before();
+    } else {
+      if (lane == 0) mbar_arrive(&sm.q_full);  // the tile is not used
     }
-    tc_fence_before();
   }
   __syncthreads();
-  if (warp == 12) {
+  if (warp == 20) {
     tc_fence_after();
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
   }
   if (tid == 0 && *abort_flag) report_timeout(nullptr);
+  if (p.beside) pdl_wait();  // this kernel completes after the one it ran beside
 }
 
 // Splits n_prefix.. are the request's own tokens; the first n_prefix hold
-// something only where the request is in a group.  One CTA per (request,
-// head), one thread per value; the splits are summed in order.
-__global__ void prefix_combine_kernel(const float* __restrict__ o_part, const float* __restrict__ ml_part,
-                                      const int32_t* __restrict__ off, int Ng, int Hq, int n_prefix, int n, int D,
-                                      __nv_bfloat16* __restrict__ out) {
+// something only where the request is in a group.  One warp per (request,
+// head), D / 32 values a lane; the splits are summed in order, 8 loads ahead.
+template <int D>
+__global__ void __launch_bounds__(256) prefix_combine_kernel(const float* __restrict__ o_part,
+                                                             const float* __restrict__ ml_part,
+                                                             const int32_t* __restrict__ off, int Ng, int rows, int Hq,
+                                                             int n_prefix, int n, __nv_bfloat16* __restrict__ out) {
   pdl_enter();
-  const int64_t bh = blockIdx.x;
+  constexpr int V = D / 32;
+  const int64_t bh = int64_t(blockIdx.x) * 8 + (threadIdx.x >> 5);
+  const int lane = threadIdx.x & 31;
+  if (bh >= rows) return;
   const int b = int(bh / Hq);
   bool in = false;
-  for (int g = threadIdx.x & 31; g < Ng; g += 32) in |= b >= off[g] && b < off[g + 1];
+  for (int g = lane; g < Ng; g += 32) in |= b >= off[g] && b < off[g + 1];
   const int s0 = __any_sync(0xffffffffu, in) ? 0 : n_prefix;
   const float2* ml = reinterpret_cast<const float2*>(ml_part) + bh * n;
+  const float* o = o_part + bh * n * D + lane * V;
   float top = -INFINITY;
-  for (int s = s0; s < n; ++s) top = fmaxf(top, ml[s].x);
-  float o = 0.f, l = 0.f;
-  const int d = threadIdx.x;
-  for (int s = s0; s < n; ++s) {
-    const float2 x = ml[s];
-    if (x.y == 0.f) continue;  // an empty split wrote no partial
-    const float f = top == -INFINITY ? 1.f : ex2(x.x - top);
-    o += f * o_part[(bh * n + s) * D + d];
-    l += f * x.y;
+  for (int s = s0 + lane; s < n; s += 32) top = fmaxf(top, ml[s].x);
+  top = warp_max<32>(top);
+  float acc[V], l = 0.f;
+#pragma unroll
+  for (int v = 0; v < V; ++v) acc[v] = 0.f;
+  for (int c0 = s0; c0 < n; c0 += 32) {
+    const float2 x = c0 + lane < n ? ml[c0 + lane] : make_float2(0.f, 0.f);
+    // an empty split wrote no partial; NaN sums stay
+    const float f = x.y == 0.f ? 0.f : top == -INFINITY ? 1.f : ex2(x.x - top);
+    const unsigned some = __ballot_sync(0xffffffffu, x.y != 0.f);
+    l += warp_sum<32>(x.y == 0.f ? 0.f : f * x.y);
+    for (int k0 = 0; k0 < min(32, n - c0); k0 += 8) {
+      float v[8][V];
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        const float* src = o + int64_t(c0 + k0 + k) * D;
+        const bool on = (some >> (k0 + k)) & 1;
+        if constexpr (V == 4) {
+          const float4 y = on ? *reinterpret_cast<const float4*>(src) : make_float4(0.f, 0.f, 0.f, 0.f);
+          v[k][0] = y.x, v[k][1] = y.y, v[k][2] = y.z, v[k][3] = y.w;
+        } else {
+          const float2 y = on ? *reinterpret_cast<const float2*>(src) : make_float2(0.f, 0.f);
+          v[k][0] = y.x, v[k][1] = y.y;
+        }
+      }
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        const float w = __shfl_sync(0xffffffffu, f, k0 + k);
+#pragma unroll
+        for (int e = 0; e < V; ++e) acc[e] = fmaf(w, v[k][e], acc[e]);
+      }
+    }
   }
-  out[bh * D + d] = __float2bfloat16_rn(l != 0.f ? o / l : 0.f);
+  const float inv = l != 0.f ? 1.f / l : 0.f;
+  uint32_t y[V / 2];
+#pragma unroll
+  for (int e = 0; e < V / 2; ++e) y[e] = pack_bf16x2(acc[2 * e] * inv, acc[2 * e + 1] * inv);
+  if constexpr (V == 4) *reinterpret_cast<uint2*>(out + bh * D + lane * V) = make_uint2(y[0], y[1]);
+  else *reinterpret_cast<uint32_t*>(out + bh * D + lane * V) = y[0];
 }
 
+template <int D>
+static int launch_combine(const float* o_part, const float* ml_part, const int32_t* off, int Ng, int64_t rows, int Hq,
+                          int n_prefix, int n, __nv_bfloat16* out, cudaStream_t st) {
+  return launch_kernel(prefix_combine_kernel<D>, dim3{unsigned((rows + 7) / 8)}, dim3{256}, 0, st, o_part, ml_part, off,
+                       Ng, int(rows), Hq, n_prefix, n, out);
+}
+
+// With `beside` the kernel follows the requests' own-token kernel, whose
+// results it does not need: it is let onto the SMs as that one's CTAs leave
+// them (programmatic launch without the wait at the start).  That kernel's
+// CTAs have all passed their own wait by then, so what came before it is
+// complete; the wait at this kernel's end makes its completion cover both.
 template <int DP, int BITS>
 static int launch_prefix(const PrefixParams& p, unsigned grid, cudaStream_t st) {
+  using SM = PrefixSmem<DP, BITS>;
+  static_assert(sizeof(SM) <= 227 * 1024, "one CTA's shared memory");
+  static_assert(2 * 128 * SM::PITCH <= (2 + PX_RING) * SM::TILE, "room for the output rows");
   auto kern = prefix_attn_kernel<DP, BITS>;
-  const int smem = 1024 + (2 + PX_STAGES) * 128 * DP * 2 + 256;
-  const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, int(sizeof(SM)));
   if (e != cudaSuccess) {
     set_last_cuda_error(e);
     return B2F_ERR_CUDA;
   }
-  return launch_kernel(kern, dim3{grid}, dim3{PX_THREADS}, size_t(smem), st, p);
+  int& policy = launch_pdl_policy();
+  const int before = policy;
+  if (p.beside) policy = 1;
+  const int rc = launch_kernel(kern, dim3{grid}, dim3{PX_THREADS}, sizeof(SM), st, p);
+  policy = before;
+  return rc;
 }
 
 template <int DP>
@@ -556,7 +681,7 @@ int b2f_shared_prefix_attn(const void* q, const uint8_t* k_pages, const float* k
   if (!(bits == 2 || bits == 4 || bits == 8)) return B2F_ERR_UNSUPPORTED;
   if (!(D == 64 || D == 128) || group_size != 64) return B2F_ERR_UNSUPPORTED;
   if (B < 0 || n_groups < 0 || Hq <= 0 || Hkv <= 0 || Hq % Hkv != 0) return B2F_ERR_INVALID;
-  if (Hq / Hkv > 16 || B > 65535 || Hkv > 4096 || n_groups > 65535) return B2F_ERR_UNSUPPORTED;
+  if (Hq / Hkv > 16 || B > 65535 || Hkv > 4096 || B * Hq > (1 << 30) || n_groups > 65535) return B2F_ERR_UNSUPPORTED;
   if (page_size <= 0 || page_size % 16 != 0 || prefix_pages <= 0 || max_pages <= 0 || max_prefix < 0 || max_own < 0)
     return B2F_ERR_INVALID;
   if (page_size > (1 << 20) || prefix_pages * page_size > (int64_t(1) << 30) || max_pages * page_size > (int64_t(1) << 30))
@@ -565,8 +690,8 @@ int b2f_shared_prefix_attn(const void* q, const uint8_t* k_pages, const float* k
   if (!q || !k_pages || !k_scales || !v_pages || !v_scales || !block_table || !seq_lens || !out ||
       (n_groups > 0 && (!prefix_table || !prefix_lens || !group_offsets)))
     return B2F_ERR_INVALID;
-  if (!aligned(q, 16) || !aligned(k_pages, 16) || !aligned(v_pages, 16) || !aligned(k_scales, 8) ||
-      !aligned(v_scales, 8) || !aligned(out, 16))
+  if (!aligned(q, 16) || !aligned(k_pages, 16) || !aligned(v_pages, 16) || !aligned(k_scales, 16) ||
+      !aligned(v_scales, 16) || !aligned(out, 16))
     return B2F_ERR_ALIGN;
   const int64_t G = Hq / Hkv, tpt = 128 / G;
   if (max_prefix > prefix_pages * page_size) max_prefix = prefix_pages * page_size;
@@ -581,26 +706,28 @@ int b2f_shared_prefix_attn(const void* q, const uint8_t* k_pages, const float* k
   const __nv_bfloat16* qb = static_cast<const __nv_bfloat16*>(q);
   cudaStream_t st = as_stream(stream);
   int rc;
-  if (np > 0) {
-    // items: at most one partial pair of tiles per group
-    const int64_t grid = (B / (2 * tpt) + n_groups) * Hkv * np;
-    if (grid > 0x7fffffff) return B2F_ERR_UNSUPPORTED;
-    PrefixParams p{qb, k_pages, v_pages, k_scales, v_scales, prefix_table, prefix_lens, group_offsets, prefix_pages,
-                   o_part, ml_part, softmax_scale * kLog2e, int(B), int(n_groups), int(Hq), int(Hkv), int(G),
-                   int(page_size), int(tpt), np, n, int(max_prefix)};
-    rc = D == 64 ? launch_prefix_bits<64>(p, bits, unsigned(grid), st)
-                 : launch_prefix_bits<128>(p, bits, unsigned(grid), st);
-    if (rc != B2F_OK) return rc;
-  }
   if (no > 0) {
     rc = launch_own_partials(qb, k_pages, k_scales, v_pages, v_scales, block_table, max_pages, seq_lens, int(B), int(Hq),
                              int(Hkv), int(D), int(page_size), bits, softmax_scale, no, int(max_own), o_part, ml_part, n,
                              np, st);
     if (rc != B2F_OK) return rc;
   }
-  return launch_kernel(prefix_combine_kernel, dim3{unsigned(B * Hq)}, dim3{unsigned(D)}, 0, st,
-                       static_cast<const float*>(o_part), static_cast<const float*>(ml_part), group_offsets,
-                       np > 0 ? int(n_groups) : 0, int(Hq), np, n, int(D), static_cast<__nv_bfloat16*>(out));
+  if (np > 0) {
+    // items: at most one partial pair of tiles per group
+    const int64_t grid = (B / (2 * tpt) + n_groups) * Hkv * np;
+    if (grid > 0x7fffffff) return B2F_ERR_UNSUPPORTED;
+    const float s2 = fabsf(softmax_scale) * kLog2e;
+    PrefixParams p{qb, k_pages, v_pages, k_scales, v_scales, prefix_table, prefix_lens, group_offsets, prefix_pages,
+                   o_part, ml_part, s2 > 1e-30f ? s2 : 1e-30f, softmax_scale < 0.f, int(B), int(n_groups), int(Hq),
+                   int(Hkv), int(G), int(page_size), int(tpt), np, n, int(max_prefix), no > 0};
+    rc = D == 64 ? launch_prefix_bits<64>(p, bits, unsigned(grid), st)
+                 : launch_prefix_bits<128>(p, bits, unsigned(grid), st);
+    if (rc != B2F_OK) return rc;
+  }
+  __nv_bfloat16* ob = static_cast<__nv_bfloat16*>(out);
+  const int Ng = np > 0 ? int(n_groups) : 0;
+  return D == 64 ? launch_combine<64>(o_part, ml_part, group_offsets, Ng, B * Hq, int(Hq), np, n, ob, st)
+                 : launch_combine<128>(o_part, ml_part, group_offsets, Ng, B * Hq, int(Hq), np, n, ob, st);
 }
 
 }  // extern "C"

@@ -55,6 +55,18 @@ __device__ __forceinline__ float v_reference(const AttnParams& p, int b, int hkv
   for (int g = 0; g < DG; ++g) top = fmaxf(top, p.vs[row * DG + g]);
   return pow2_inverse(top, shift);
 }
+// largest magnitude of 16 consecutive values (32-byte aligned)
+__device__ __forceinline__ float absmax16(const __nv_bfloat16* x) {
+  float top = 0.f;
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const uint4 v = reinterpret_cast<const uint4*>(x)[i];
+    const __nv_bfloat162* e = reinterpret_cast<const __nv_bfloat162*>(&v);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) top = fmaxf(top, fmaxf(fabsf(__low2float(e[k])), fabsf(__high2float(e[k]))));
+  }
+  return top;
+}
 __device__ __forceinline__ float scaled_up_to(float s, float f, float top) {
   const float x = s * f;
   return x > top ? top : x;  // NaN stays
@@ -123,8 +135,9 @@ __global__ void __launch_bounds__(RING ? 160 : 128) qkv_decode_attn_kernel(const
     float qn = p.qscale;
     if constexpr (PART) {
       float top = 0.f;
-      for (int d = 0; hv && d < 16 * DG; ++d)
-        top = fmaxf(top, fabsf(__bfloat162float(qrow[64 * (d >> 4) + 16 * c + (d & 15)])));
+#pragma unroll
+      for (int g = 0; g < DG; ++g)
+        if (hv) top = fmaxf(top, absmax16(qrow + 64 * g + 16 * c));
       top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
       top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
       qn = pow2_inverse(top, 0);
@@ -711,8 +724,9 @@ __global__ void __launch_bounds__(160, 2) qkv_decode_attn_t8_kernel(const AttnPa
       float qn = p.qscale;
       if constexpr (PART) {
         float top = 0.f;
-        for (int d = 0; hv && d < 16 * DG; ++d)
-          top = fmaxf(top, fabsf(__bfloat162float(qrow[64 * (d >> 4) + 16 * c + (d & 15)])));
+#pragma unroll
+        for (int grp = 0; grp < DG; ++grp)
+          if (hv) top = fmaxf(top, absmax16(qrow + 64 * grp + 16 * c));
         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
         qn = pow2_inverse(top, 0);
