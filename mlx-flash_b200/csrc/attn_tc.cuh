@@ -167,7 +167,7 @@ __device__ __forceinline__ void bulk_s2g(void* dst, const void* src, uint32_t by
                : "memory");
 }
 __device__ __forceinline__ void bulk_s2g_wait() {
-  asm volatile("cp.async.bulk.commit_group;\n cp.async.bulk.wait_group 0;" ::: "memory");
+  asm volatile("cp.async.bulk.commit_group;\n cp.async.bulk.wait_group.read 0;" ::: "memory");
 }
 
 // OR of a predicate over the `n` threads of named barrier `id`

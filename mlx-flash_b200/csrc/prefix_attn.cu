@@ -29,10 +29,14 @@ int launch_own_partials(const __nv_bfloat16* q, const uint8_t* kc, const float* 
                         int bits, float scale, int n_splits, int max_len, float* o_part, float* ml_part,
                         int part_stride, int part_base, cudaStream_t st);
 
-constexpr int PX_THREADS = 768;  // warps 0-15 softmax, 16-19 decode the codes, 20 issues the MMAs, 21 the copies
-constexpr int PX_BN = 128;       // keys per block
-constexpr int PX_RAW = 3;        // blocks of codes in flight (K and V count apart)
-constexpr int PX_RING = 3;       // decoded tiles
+// warps 0-15 softmax, 16-19 decode K, 20-23 V, 24 issues the MMAs, 25 the copies
+constexpr int PX_THREADS = 832;
+constexpr int PX_MMA = 24, PX_COPY = 25;
+constexpr int PX_BN = 128;  // keys per block
+// Stages alternate K and V (it = 2 j, 2 j + 1): an even number, so that a
+// stage holds one of the two only and its readers see its phases in turn.
+constexpr int PX_RAW = 2;   // blocks of codes in flight
+constexpr int PX_RING = 4;  // decoded tiles
 struct PrefixParams {
   const __nv_bfloat16* q;
   const uint8_t *kc, *vc;
@@ -54,8 +58,8 @@ struct PrefixSmem {
   uint8_t q[2][TILE];           // at the end, with the ring, the output rows
   uint8_t ring[PX_RING][TILE];  // K_0 V_0 K_1 V_1 ..., fp16
   uint8_t raw[PX_RAW][RAW];     // the same blocks as codes
-  float exchange[2][128];       // between the two threads of a row
-  float largest[2][4];          // scales of the first block, per decoding warp
+  __nv_bfloat16 exchange[2][128];  // between the two threads of a row
+  float largest[2][4];             // scales of the first block (K, V), per decoding warp
   uint64_t raw_full[PX_RAW], raw_empty[PX_RAW], full[PX_RING], empty[PX_RING], q_full, s_full[2], p_full[4], pv_done[2],
       drain;
   int item[4];  // group, first request, requests from there, prefix length
@@ -178,7 +182,7 @@ __global__ void __launch_bounds__(PX_THREADS, 1) prefix_attn_kernel(const Prefix
     mbar_init(&sm.drain, 1);
     sm.abort_flag = 0;
     fence_mbarrier_init();
-  } else if (warp == 20) {
+  } else if (warp == PX_MMA) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&sm.tmem)), "r"(512u)
                  : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
@@ -194,8 +198,8 @@ __global__ void __launch_bounds__(PX_THREADS, 1) prefix_attn_kernel(const Prefix
   const int n = g < 0 ? 0 : min(blocks, j0 + per) - j0;  // this split's blocks (g < 0: a spare CTA of the grid)
   const int n_tiles = rows > p.tpt ? 2 : 1;
 
-  if (warp >= 20) {
-    if (warp == 20 && n > 0) {
+  if (warp >= PX_MMA) {
+    if (warp == PX_MMA && n > 0) {
       // ============================ MMA issuer ==================================
       const uint32_t one = elect_lane();
       const uint32_t id_s = mma_idesc(PX_BN, false, false, p.negate), id_o = mma_idesc(DP, false, true, false);
@@ -260,7 +264,7 @@ __global__ void __launch_bounds__(PX_THREADS, 1) prefix_attn_kernel(const Prefix
       tc_commit_by(one, &sm.drain);
       mbar_wait_bounded(&sm.drain, 0u, 100000000ull);
       __syncwarp();
-    } else if (warp == 21 && n > 0 && !producers_stalled()) {  // test control: stalled producers issue nothing
+    } else if (warp == PX_COPY && n > 0 && !producers_stalled()) {  // test control: stalled producers issue nothing
       // ============================ copies of codes and scales ==================
       // 16 keys a lane (pages hold a multiple of 16): lanes 0-7 bring K, 8-15 V.
       const int32_t* pages = p.table + int64_t(g) * p.width;
@@ -303,32 +307,26 @@ __global__ void __launch_bounds__(PX_THREADS, 1) prefix_attn_kernel(const Prefix
     // Lane t has rows t / LPR + (128 / LPR) * k and chunks t % LPR + LPR * c of
     // each: the stores of a phase's 8 lanes hit 8 different 16-byte columns of
     // the swizzled tile.
-    const int t = tid - 512, sub = t % LPR;
+    const int v = (warp - 16) >> 2;  // K or V
+    const int t = tid - 512 - 128 * v, sub = t % LPR;
     constexpr uint32_t OFF = 0x64006400u + uint32_t(TOP) * 0x00010001u;  // 1024 + TOP, twice
-    float norm[2] = {1.f, 1.f};  // K, V
+    float norm = 1.f;
     bool ok = true;
-    for (int it = 0; ok && it < 2 * n; ++it) {
-      const int s = it % PX_RAW, st = it % NST, j = it >> 1;
-      if (it == 0) {
-        // references from the first block: its largest scales of K and of V
-        // (PX_RAW blocks are in flight: V's has been asked for too)
-        float top[2] = {0.f, 0.f};
-        for (int v = 0; v < 2; ++v) {
-          ok = ok && __all_sync(0xffffffffu, px_wait(&sm.raw_full[v], 0u, abort_flag));
-          const float* sc = reinterpret_cast<const float*>(sm.raw[v] + SM::CODES);
-          if (ok && t < len - j0 * PX_BN)
-            for (int e = 0; e < DG; ++e)
-              if (sc[t * DG + e] < INFINITY) top[v] = fmaxf(top[v], sc[t * DG + e]);
-          top[v] = warp_max<32>(top[v]);
-          if (lane == 0) sm.largest[v][warp - 16] = top[v];
-        }
-        bar_all(3, 128);
-        // the largest value of the first block lands in [2^(BITS-8), 2^(BITS-6))
-        for (int v = 0; v < 2; ++v)
-          norm[v] = pow2_inverse(fmaxf(fmaxf(sm.largest[v][0], sm.largest[v][1]),
-                                       fmaxf(sm.largest[v][2], sm.largest[v][3])), -7);
-      } else {
-        ok = __all_sync(0xffffffffu, px_wait(&sm.raw_full[s], uint32_t((it / PX_RAW) & 1), abort_flag));
+    for (int j = 0; j < n; ++j) {
+      const int it = 2 * j + v, s = it % PX_RAW, st = it % NST;
+      ok = __all_sync(0xffffffffu, ok && px_wait(&sm.raw_full[s], uint32_t((it / PX_RAW) & 1), abort_flag));
+      if (j == 0) {
+        // the reference: the first block's largest scale, which puts its
+        // largest value in [2^(BITS-8), 2^(BITS-6))
+        float top = 0.f;
+        const float* sc = reinterpret_cast<const float*>(sm.raw[s] + SM::CODES);
+        if (ok && t < len - j0 * PX_BN)
+          for (int e = 0; e < DG; ++e)
+            if (sc[t * DG + e] < INFINITY) top = fmaxf(top, sc[t * DG + e]);
+        top = warp_max<32>(top);
+        if (lane == 0) sm.largest[v][warp & 3] = top;
+        bar_all(3 + v, 128);
+        norm = pow2_inverse(fmaxf(fmaxf(sm.largest[v][0], sm.largest[v][1]), fmaxf(sm.largest[v][2], sm.largest[v][3])), -7);
       }
       ok = ok && (it < NST || __all_sync(0xffffffffu, px_wait(&sm.empty[st], uint32_t((it / NST - 1) & 1), abort_flag)));
       if (!ok) break;
@@ -342,7 +340,7 @@ __global__ void __launch_bounds__(PX_THREADS, 1) prefix_attn_kernel(const Prefix
           const int chunk = sub + LPR * c;
           const bool in = row < valid;
           const uint4 w = *reinterpret_cast<const uint4*>(sm.raw[s] + row * RB + chunk * 16);
-          const float sc = in ? scales[row * DG + chunk * (128 / BITS) / 64] * norm[it & 1] : 0.f;
+          const float sc = in ? scales[row * DG + chunk * (128 / BITS) / 64] * norm : 0.f;
           const __half2 h2 = __float2half2_rn(sc > 256.f ? 256.f : sc);  // 255 * 256 is the last fp16 value; NaN stays
           const uint32_t s2 = *reinterpret_cast<const uint32_t*>(&h2);
           uint32_t b[32 / BITS];
@@ -396,19 +394,16 @@ __global__ void __launch_bounds__(PX_THREADS, 1) prefix_attn_kernel(const Prefix
 #pragma unroll
         for (int k = 0; k < 4; ++k) top = fmaxf(top, fmaxf(fabsf(__low2float(e[k])), fabsf(__high2float(e[k]))));
       }
-      // max (or sum) with the row's other thread
-      auto join = [&](float v, bool add) {
-        if (h) sm.exchange[i][r] = v;
+      // max with the row's other thread, to 8 bits: both take the same value, and
+      // a reference need not be exact
+      auto join = [&](float v) {
+        if (h) sm.exchange[i][r] = __float2bfloat16_rn(v);
         bar_all(bar, 256);
-        if (!h) {
-          const float o = sm.exchange[i][r];
-          v = add ? v + o : fmaxf(v, o);
-          sm.exchange[i][r] = v;
-        }
+        if (!h) sm.exchange[i][r] = __float2bfloat16_rn(fmaxf(v, __bfloat162float(sm.exchange[i][r])));
         bar_all(bar, 256);
-        return h ? sm.exchange[i][r] : v;
+        return __bfloat162float(sm.exchange[i][r]);
       };
-      const float qn = pow2_inverse(join(top, false), 0);
+      const float qn = pow2_inverse(join(top), 0);
 #pragma unroll
       for (int c = 0; c < QC; ++c) {
         const __nv_bfloat162* e = reinterpret_cast<const __nv_bfloat162*>(&w[c]);
@@ -434,7 +429,7 @@ __global__ void __launch_bounds__(PX_THREADS, 1) prefix_attn_kernel(const Prefix
           zs /= pow2_inverse(fmaxf(fmaxf(sm.largest[0][0], sm.largest[0][1]), fmaxf(sm.largest[0][2], sm.largest[0][3])), -7);
         const int valid = len - (j0 + j) * PX_BN - 64 * h;  // keys of this half (64 or more: all)
         const bool masked = valid < 64;
-        // the scores are read twice, 32 at a time: 64 at once and P do not fit 80 registers
+        // the scores are read twice, 32 at a time: 64 at once and P do not fit 72 registers
         auto scores = [&](int c, uint32_t (&s)[32]) {
           tmem_ld32(s_at + c, s);
           if (masked) {
@@ -456,7 +451,7 @@ __global__ void __launch_bounds__(PX_THREADS, 1) prefix_attn_kernel(const Prefix
             quit = true;
             break;
           }
-          const float both = join(mx, false);
+          const float both = join(mx);
           const bool move = j == 0 || both > m + 8.f;
           if (j > 0) {
             // O holds blocks up to j - 1 once their product is done
@@ -479,17 +474,14 @@ __global__ void __launch_bounds__(PX_THREADS, 1) prefix_attn_kernel(const Prefix
         }
         const float ref = m == -INFINITY ? 0.f : m;
         uint64_t sum[2] = {0ull, 0ull};
-        uint32_t pk[2][16];
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
-          uint32_t s[32];
+          uint32_t s[32], pk[16];
           scores(32 * c, s);
-          if (masked) exp_row<false, false>(s, zs, ref, sum, pk[c]);  // exact zeros
-          else exp_row<false, true>(s, zs, ref, sum, pk[c]);
+          if (masked) exp_row<false, false>(s, zs, ref, sum, pk);  // exact zeros
+          else exp_row<false, true>(s, zs, ref, sum, pk);
+          tmem_st16(s_at + 16 * c, pk);  // P goes over this thread's own scores, behind their reading
         }
-        // P goes over this thread's own scores
-        tmem_st16(s_at, pk[0]);
-        tmem_st16(s_at + 16, pk[1]);
         const float2 l2 = f32x2_parts(add_x2(sum[0], sum[1]));
         l += l2.x + l2.y;
         tmem_wait_st();
@@ -499,13 +491,13 @@ __global__ void __launch_bounds__(PX_THREADS, 1) prefix_attn_kernel(const Prefix
       }
       // ---- the partial: rows of O through shared memory, then one copy each ----
       // (the operands have been used up once both tiles' products are done)
-      if (!quit) l = join(l, true);
       ok = ok && !quit && wait_all(&sm.drain, 0u);
       tc_fence_after();
+      uint8_t* out = sm.q[0] + (i * 128 + r) * SM::PITCH;
       if (ok) {
         const float back = 1.f / pow2_inverse(fmaxf(fmaxf(sm.largest[1][0], sm.largest[1][1]),
                                                     fmaxf(sm.largest[1][2], sm.largest[1][3])), -7);
-        uint8_t* out = sm.q[0] + (i * 128 + r) * SM::PITCH;
+        if (h) *reinterpret_cast<float*>(out + DP * 4) = l;  // behind the row: this thread's sum
 #pragma unroll
         for (int c = 0; c < DP / 2; c += 16) {
           uint32_t o[16];
@@ -520,8 +512,8 @@ __global__ void __launch_bounds__(PX_THREADS, 1) prefix_attn_kernel(const Prefix
       }
       bar_all(bar, 256);
       if (ok && live && h == 0) {
-        bulk_s2g(p.o_part + part * DP, sm.q[0] + (i * 128 + r) * SM::PITCH, DP * 4);
-        *reinterpret_cast<float2*>(p.ml_part + part * 2) = make_float2(m, l);
+        bulk_s2g(p.o_part + part * DP, out, DP * 4);
+        *reinterpret_cast<float2*>(p.ml_part + part * 2) = make_float2(m, l + *reinterpret_cast<const float*>(out + DP * 4));
         bulk_s2g_wait();
       }
       tc_fence_before();
@@ -530,7 +522,7 @@ __global__ void __launch_bounds__(PX_THREADS, 1) prefix_attn_kernel(const Prefix
     }
   }
   __syncthreads();
-  if (warp == 20) {
+  if (warp == PX_MMA) {
     tc_fence_after();
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
   }
