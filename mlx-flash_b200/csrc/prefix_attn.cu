@@ -29,8 +29,8 @@ int launch_own_partials(const __nv_bfloat16* q, const uint8_t* kc, const float* 
                         int bits, float scale, int n_splits, int max_len, float* o_part, float* ml_part,
                         int part_stride, int part_base, cudaStream_t st);
 
-// warps 0-15 softmax, 16-19 decode K, 20-23 V, 24 issues the MMAs, 25 the copies
-constexpr int PX_THREADS = 832;
+// warps 0-15 softmax, 16-19 decode K, 20-23 V, 24 issues the MMAs, 25 copies K, 26 V
+constexpr int PX_THREADS = 864;
 constexpr int PX_MMA = 24, PX_COPY = 25;
 constexpr int PX_BN = 128;  // keys per block
 // Stages alternate K and V (it = 2 j, 2 j + 1): an even number, so that a
@@ -264,42 +264,39 @@ __global__ void __launch_bounds__(PX_THREADS, 1) prefix_attn_kernel(const Prefix
       tc_commit_by(one, &sm.drain);
       mbar_wait_bounded(&sm.drain, 0u, 100000000ull);
       __syncwarp();
-    } else if (warp == PX_COPY && n > 0 && !producers_stalled()) {  // test control: stalled producers issue nothing
+    } else if (warp >= PX_COPY && n > 0 && !producers_stalled()) {  // test control: stalled producers issue nothing
       // ============================ copies of codes and scales ==================
-      // 16 keys a lane (pages hold a multiple of 16): lanes 0-7 bring K, 8-15 V.
+      // 16 keys a lane (pages hold a multiple of 16)
+      const int v = warp - PX_COPY, part = lane;  // K or V
       const int32_t* pages = p.table + int64_t(g) * p.width;
-      const int part = lane & 7;
-      const bool is_v = lane & 8;
-      const uint8_t* codes = is_v ? p.vc : p.kc;
-      const float* scales = is_v ? p.vs : p.ks;
+      const uint8_t* codes = v ? p.vc : p.kc;
+      const float* scales = v ? p.vs : p.ks;
       auto page_of = [&](int j) {
         const int key = (j0 + j) * PX_BN + 16 * part;
-        return lane < 16 && j < n && key < len ? max(pages[key / p.P], 0) : -1;
+        return part < 8 && j < n && key < len ? max(pages[key / p.P], 0) : -1;
       };
-      int page = page_of(0);
-      bool ok = true;
-      int it = 0;
-      for (int j = 0; ok && j < n; ++j) {
-        const int key = (j0 + j) * PX_BN + 16 * part;
+      int page = page_of(0), j = 0;
+      for (; j < n; ++j) {
+        const int key = (j0 + j) * PX_BN + 16 * part, it = 2 * j + v, s = it % PX_RAW;
         const int keys = min(PX_BN, (len - (j0 + j) * PX_BN + 15) & ~15);  // of the block, in whole sixteens
         const int64_t row = (int64_t(page) * p.Hkv + hk) * p.P + key % p.P;
         const bool have = page >= 0;
         page = page_of(j + 1);
-        for (int v = 0; ok && v < 2; ++v, ++it) {
-          const int s = it % PX_RAW;
-          ok = it < PX_RAW || __all_sync(0xffffffffu, px_wait(&sm.raw_empty[s], uint32_t((it / PX_RAW - 1) & 1), abort_flag));
-          if (!ok) break;
-          if (lane == 0) mbar_arrive_expect_tx(&sm.raw_full[s], uint32_t(keys) * (RB + DG * 4));
-          __syncwarp();
-          if (have && is_v == bool(v)) {
-            bulk_g2s(sm.raw[s] + 16 * part * RB, codes + row * RB, 16 * RB, &sm.raw_full[s]);
-            bulk_g2s(sm.raw[s] + SM::CODES + 16 * part * DG * 4, scales + row * DG, 16 * DG * 4, &sm.raw_full[s]);
-          }
+        if (it >= PX_RAW &&
+            !__all_sync(0xffffffffu, px_wait(&sm.raw_empty[s], uint32_t((it / PX_RAW - 1) & 1), abort_flag)))
+          break;
+        if (lane == 0) mbar_arrive_expect_tx(&sm.raw_full[s], uint32_t(keys) * (RB + DG * 4));
+        __syncwarp();
+        if (have) {
+          bulk_g2s(sm.raw[s] + 16 * part * RB, codes + row * RB, 16 * RB, &sm.raw_full[s]);
+          bulk_g2s(sm.raw[s] + SM::CODES + 16 * part * DG * 4, scales + row * DG, 16 * DG * 4, &sm.raw_full[s]);
         }
       }
-      // copies already issued land before the CTA goes away
-      for (int k = 1; k <= PX_RAW && it - k >= 0; ++k)
-        mbar_wait_bounded(&sm.raw_full[(it - k) % PX_RAW], uint32_t(((it - k) / PX_RAW) & 1), 100000000ull);
+      // the last copy issued lands before the CTA goes away (those before it were waited for)
+      if (j > 0) {
+        const int it = 2 * (j - 1) + v;
+        mbar_wait_bounded(&sm.raw_full[it % PX_RAW], uint32_t((it / PX_RAW) & 1), 100000000ull);
+      }
       __syncwarp();
     }
   } else if (warp >= 16) {
@@ -328,24 +325,37 @@ __global__ void __launch_bounds__(PX_THREADS, 1) prefix_attn_kernel(const Prefix
         bar_all(3 + v, 128);
         norm = pow2_inverse(fmaxf(fmaxf(sm.largest[v][0], sm.largest[v][1]), fmaxf(sm.largest[v][2], sm.largest[v][3])), -7);
       }
-      ok = ok && (it < NST || __all_sync(0xffffffffu, px_wait(&sm.empty[st], uint32_t((it / NST - 1) & 1), abort_flag)));
       if (!ok) break;
+      // the lane's codes and scales into registers: the stage is free for the next copy
       const int valid = len - (j0 + j) * PX_BN;  // keys of the block (128 or more: all)
       const float* scales = reinterpret_cast<const float*>(sm.raw[s] + SM::CODES);
+      uint4 w[LPR][CPT];
+      float sc[LPR][CPT];
 #pragma unroll
       for (int k = 0; k < LPR; ++k) {
         const int row = t / LPR + (128 / LPR) * k;
 #pragma unroll
         for (int c = 0; c < CPT; ++c) {
           const int chunk = sub + LPR * c;
-          const bool in = row < valid;
-          const uint4 w = *reinterpret_cast<const uint4*>(sm.raw[s] + row * RB + chunk * 16);
-          const float sc = in ? scales[row * DG + chunk * (128 / BITS) / 64] * norm : 0.f;
-          const __half2 h2 = __float2half2_rn(sc > 256.f ? 256.f : sc);  // 255 * 256 is the last fp16 value; NaN stays
+          w[k][c] = *reinterpret_cast<const uint4*>(sm.raw[s] + row * RB + chunk * 16);
+          sc[k][c] = row < valid ? scales[row * DG + chunk * (128 / BITS) / 64] : 0.f;
+        }
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&sm.raw_empty[s]);
+      ok = it < NST || __all_sync(0xffffffffu, px_wait(&sm.empty[st], uint32_t((it / NST - 1) & 1), abort_flag));
+      if (!ok) break;
+#pragma unroll
+      for (int k = 0; k < LPR; ++k) {
+        const int row = t / LPR + (128 / LPR) * k;
+#pragma unroll
+        for (int c = 0; c < CPT; ++c) {
+          const float x0 = sc[k][c] * norm;
+          const __half2 h2 = __float2half2_rn(x0 > 256.f ? 256.f : x0);  // 255 * 256 is the last fp16 value; NaN stays
           const uint32_t s2 = *reinterpret_cast<const uint32_t*>(&h2);
           uint32_t b[32 / BITS];
-          spread_codes<BITS>(w, b);
-          const int col = chunk * (16 / BITS);  // first 8-value column of the chunk
+          spread_codes<BITS>(w[k][c], b);
+          const int col = (sub + LPR * c) * (16 / BITS);  // first 8-value column of the chunk
 #pragma unroll
           for (int x = 0; x < 16 / BITS; ++x) {
             const uint2 lo = codes_to_f16(b[2 * x], OFF, s2), hi = codes_to_f16(b[2 * x + 1], OFF, s2);
@@ -357,10 +367,7 @@ __global__ void __launch_bounds__(PX_THREADS, 1) prefix_attn_kernel(const Prefix
       }
       fence_proxy_async_smem();
       __syncwarp();
-      if (lane == 0) {
-        mbar_arrive(&sm.raw_empty[s]);
-        mbar_arrive(&sm.full[st]);
-      }
+      if (lane == 0) mbar_arrive(&sm.full[st]);
     }
     __syncwarp();
   } else {
