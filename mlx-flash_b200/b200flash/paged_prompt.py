@@ -35,15 +35,17 @@ class PagePlan(NamedTuple):
     counts: torch.Tensor  # [2] tokens in the batch, pages it takes
 
 
-def _int32(name, t, *shape):
-    """``t`` contiguous, after checking that it is int32 of ``shape`` (None: any extent)."""
-    ok = t.dtype is torch.int32 and t.dim() == len(shape)
-    if ok:
-        for want, got in zip(shape, t.shape):
-            ok = ok and (want is None or want == got)
-    if not ok:
-        want = ", ".join("*" if s is None else str(s) for s in shape)
-        raise ValueError(f"{name} must be int32 [{want}], got {t.dtype} {list(t.shape)}")
+def _int32(name, t, n=None):
+    """``t`` contiguous, after checking that it is int32 ``[n]`` (None: any length)."""
+    if t.dtype is not torch.int32 or t.dim() != 1 or (n is not None and t.shape[0] != n):
+        raise ValueError(f"{name} must be int32 [{'*' if n is None else n}], got {t.dtype} {list(t.shape)}")
+    return t if t.is_contiguous() else t.contiguous()
+
+
+def _table(name, t, n=None):
+    """``t`` contiguous, after checking that it is int32 ``[n, *]``."""
+    if t.dtype is not torch.int32 or t.dim() != 2 or (n is not None and t.shape[0] != n):
+        raise ValueError(f"{name} must be int32 [{'*' if n is None else n}, *], got {t.dtype} {list(t.shape)}")
     return t if t.is_contiguous() else t.contiguous()
 
 
@@ -63,21 +65,23 @@ def plan_pages(new_lens: torch.Tensor, free_pages: torch.Tensor, page_size: int,
         raise ValueError(f"page_size must be positive, got {page_size}")
     if total_tokens < 0:
         raise ValueError(f"total_tokens must be non-negative, got {total_tokens}")
-    n = _int32("new_lens", new_lens, None)
+    n = _int32("new_lens", new_lens)
     B, T = n.shape[0], int(total_tokens)
     if context_lens is not None:
         context_lens = _int32("context_lens", context_lens, B)
-    free = _int32("free_pages", free_pages, None)
+    free = _int32("free_pages", free_pages)
     if not block_table.is_contiguous():
         raise ValueError("block_table is extended in place: it must be contiguous")
-    _int32("block_table", block_table, B, None)
+    _table("block_table", block_table, B)
     # one allocation for the int32 outputs, positions and rows on 16-byte boundaries
     pad = -T % 4
     ints = torch.empty(2 * (T + pad) + 2 * B + 3, dtype=torch.int32, device=dev)
-    positions, _, rows, _, cu, lens, counts = ints.split((T, pad, T, pad, B + 1, B, 2))
+    positions, _, rows, _, cu, lens, counts = ints.split_with_sizes((T, pad, T, pad, B + 1, B, 2))
     out = PagePlan(cu, positions, torch.empty(T, dtype=torch.int64, device=dev), rows, lens, counts)
-    ws_bytes = int(_capi.lib().b2f_page_plan_workspace_bytes(B))
-    ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev) if ws_bytes else None
+    ws, ws_bytes = None, 0
+    if B > 2048:  # more requests than every CTA scans for itself
+        ws_bytes = int(_capi.lib().b2f_page_plan_workspace_bytes(B))
+        ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev)
     call("b2f_page_plan", ptr(n), ptr(context_lens), B, ptr(free), free.shape[0], page_size, ptr(block_table),
          max(1, block_table.shape[1]), T, ptr(out.cu_seqlens), ptr(out.positions), ptr(out.slots), ptr(out.rows),
          ptr(out.seq_lens), ptr(out.counts), ptr(ws), ws_bytes, stream_of(dev))
@@ -115,21 +119,22 @@ def qk_norm_rope(qkv: torch.Tensor, n_heads: int, n_kv_heads: int, positions: to
     if Hq <= 0 or Hkv <= 0 or qkv.dim() != 2 or qkv.shape[1] % (Hq + 2 * Hkv):
         raise ValueError(f"qkv {list(qkv.shape)} does not hold {Hq} + 2 * {Hkv} heads a row")
     T, D = qkv.shape[0], qkv.shape[1] // (Hq + 2 * Hkv)
-    for name, w in (("q_norm", q_norm), ("k_norm", k_norm)):
-        if tuple(w.shape) != (D,) or w.dtype != qkv.dtype:
-            raise ValueError(f"{name} must be {qkv.dtype} [{D}], got {w.dtype} {list(w.shape)}")
+    for w in (q_norm, k_norm):
+        if w.dim() != 1 or w.shape[0] != D or w.dtype is not qkv.dtype:
+            raise ValueError(f"q_norm and k_norm must be {qkv.dtype} [{D}], got {w.dtype} {list(w.shape)}")
     positions = _int32("positions", positions, T)
     if inv_freq is None:
         inv_freq = rope_frequencies(D, float(theta), dev)
     elif inv_freq.dtype != torch.float64 or inv_freq.dim() != 1 or inv_freq.shape[0] * 2 > D or inv_freq.shape[0] % 8:
         raise ValueError(f"inv_freq must be float64 with a multiple of 8 up to {D // 2} values")
-    inv_freq = inv_freq.contiguous()
+    else:
+        inv_freq = inv_freq.contiguous()
     if (cache is None) != (slots is None):
         raise ValueError("cache and slots go together")
-    x = qkv
-    if x.stride(1) != 1 or x.stride(0) % 8 or x.stride(0) < x.shape[1] or x.data_ptr() % 16:
-        x = aligned_contiguous(x)
-    ld = x.stride(0) if T > 1 else x.shape[1]
+    x, width = qkv, qkv.shape[1]
+    ld, last = x.stride()
+    if last != 1 or ld % 8 or ld < width or x.data_ptr() % 16:
+        x, ld = aligned_contiguous(x), width
     kc = ks = vc = vs = None
     page_size = 0
     if cache is not None:
@@ -153,7 +158,7 @@ def qk_norm_rope(qkv: torch.Tensor, n_heads: int, n_kv_heads: int, positions: to
     call("b2f_qk_norm_rope_rows", ptr(x), ld, DTYPE_CODES[qkv.dtype], T, Hq, Hkv, D, ptr(qw), ptr(kw), float(eps),
          ptr(inv_freq), 2 * inv_freq.shape[0], ptr(positions), ptr(q), ptr(k), ptr(slots), ptr(kc), ptr(ks), ptr(vc),
          ptr(vs), page_size, bits, stream_of(dev))
-    return q, k, qkv[:, (Hq + Hkv) * D:].unflatten(1, (Hkv, D))
+    return q, k, qkv[:, (Hq + Hkv) * D:].view(T, Hkv, D)
 
 
 def _rows_of_heads(t):
@@ -185,7 +190,7 @@ def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqle
     Hkv = k.shape[1]
     if Hkv == 0 or Hq == 0 or Hq % Hkv:
         raise ValueError(f"num_kv_heads {Hkv} must divide the {Hq} query heads")
-    cu = _int32("cu_seqlens", cu_seqlens, None)
+    cu = _int32("cu_seqlens", cu_seqlens)
     if cu.shape[0] < 1:
         raise ValueError("cu_seqlens must hold at least one offset")
     if softmax_scale is None:
@@ -193,8 +198,9 @@ def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqle
     (q, q_row, q_head), (k, k_row, k_head), (v, v_row, v_head) = (_rows_of_heads(t) for t in (q, k, v))
     out = torch.empty(T, Hq, D, dtype=q.dtype, device=dev)
     lse = torch.empty(T, Hq, dtype=torch.float32, device=dev) if return_lse else None
-    call("b2f_prompt_attn", ptr(q), q_row, q_head, ptr(k), k_row, k_head, ptr(v), v_row, v_head, DTYPE_CODES[q.dtype], ptr(cu), cu.shape[0] - 1, T, Hq, Hkv, D, int(bool(causal)),
-         float(softmax_scale), ptr(out), ptr(lse), stream_of(dev))
+    call("b2f_prompt_attn", ptr(q), q_row, q_head, ptr(k), k_row, k_head, ptr(v), v_row, v_head, DTYPE_CODES[q.dtype],
+         ptr(cu), cu.shape[0] - 1, T, Hq, Hkv, D, int(bool(causal)), float(softmax_scale), ptr(out), ptr(lse),
+         stream_of(dev))
     return (out, lse) if return_lse else out
 
 
@@ -228,17 +234,20 @@ def shared_prefix_attention(q: torch.Tensor, k_pages: torch.Tensor, k_scales: to
         raise ValueError(f"group_size must be 64, got {group_size}")
     if page_size <= 0 or page_size % 16:
         raise ValueError(f"page_size must be a positive multiple of 16, got {page_size}")
-    row = packed_len(D, bits, group_size)
-    for name, t, dt, w in (("k_pages", k_pages, torch.uint8, row), ("v_pages", v_pages, torch.uint8, row),
-                           ("k_scales", k_scales, torch.float32, D // 64),
-                           ("v_scales", v_scales, torch.float32, D // 64)):
-        if t.dtype != dt or not t.is_contiguous() or t.numel() % (Hkv * page_size * max(1, w)):
-            raise ValueError(f"{name} must be contiguous {dt} pages of {Hkv} x {page_size} rows of {w}")
-    prefix_table = _int32("prefix_table", prefix_table, None, None)
+    if D not in (64, 128):
+        raise ValueError(f"head_dim must be 64 or 128, got {D}")
+    page = Hkv * page_size * D  # values of a page
+    for codes, scales in ((k_pages, k_scales), (v_pages, v_scales)):
+        if (codes.dtype is not torch.uint8 or scales.dtype is not torch.float32 or not codes.is_contiguous()
+                or not scales.is_contiguous() or codes.numel() * 8 != scales.numel() * 64 * bits
+                or scales.numel() % (page // 64)):
+            raise ValueError(f"K and V must be contiguous pages of {Hkv} x {page_size} rows: uint8 codes and float32 "
+                             f"scales, one per 64 values of {bits} bits")
+    prefix_table = _table("prefix_table", prefix_table)
     Ng = prefix_table.shape[0]
     prefix_lens = _int32("prefix_lens", prefix_lens, Ng)
     group_offsets = _int32("group_offsets", group_offsets, Ng + 1)
-    block_table = _int32("block_table", block_table, B, None)
+    block_table = _table("block_table", block_table, B)
     seq_lens = _int32("seq_lens", seq_lens, B)
     cap_p, cap_o = prefix_table.shape[1] * page_size, block_table.shape[1] * page_size
     max_p = cap_p if max_prefix_len is None else min(int(max_prefix_len), cap_p)

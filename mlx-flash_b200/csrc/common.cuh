@@ -6,6 +6,8 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <atomic>
+
 #include "b2f.h"
 
 namespace b2f {
@@ -66,6 +68,23 @@ inline int launch_kernel(void (*kern)(P...), dim3 grid, dim3 block, size_t smem,
     return B2F_ERR_CUDA;
   }
   return check_launch();
+}
+
+// The dynamic shared memory above 48 KB that `kern` is launched with, set on
+// its first launch on each device (Kern: one flag word per kernel).
+template <auto Kern>
+inline int allow_smem(int bytes) {
+  static std::atomic<uint64_t> done{0};
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e == cudaSuccess && dev < 64 && (done.load(std::memory_order_relaxed) >> dev & 1)) return B2F_OK;
+  if (e == cudaSuccess) e = cudaFuncSetAttribute(Kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (e != cudaSuccess) {
+    set_last_cuda_error(e);
+    return B2F_ERR_CUDA;
+  }
+  if (dev < 64) done.fetch_or(uint64_t(1) << dev, std::memory_order_relaxed);
+  return B2F_OK;
 }
 
 inline bool aligned(const void* p, uintptr_t a) {

@@ -615,12 +615,9 @@ static int launch_prefix(const PrefixParams& p, unsigned grid, cudaStream_t st) 
   using SM = PrefixSmem<DP, BITS>;
   static_assert(sizeof(SM) <= 227 * 1024, "one CTA's shared memory");
   static_assert(2 * 128 * SM::PITCH <= (2 + PX_RING) * SM::TILE, "room for the output rows");
-  auto kern = prefix_attn_kernel<DP, BITS>;
-  const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, int(sizeof(SM)));
-  if (e != cudaSuccess) {
-    set_last_cuda_error(e);
-    return B2F_ERR_CUDA;
-  }
+  constexpr auto kern = prefix_attn_kernel<DP, BITS>;
+  const int set = allow_smem<kern>(int(sizeof(SM)));
+  if (set != B2F_OK) return set;
   int& policy = launch_pdl_policy();
   const int before = policy;
   if (p.beside) policy = 1;

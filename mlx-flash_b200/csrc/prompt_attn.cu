@@ -613,14 +613,11 @@ static int make_rows_map(CUtensorMap* map, const void* base, bool bf16, int64_t 
 template <int DP, bool BF16>
 static int launch_prompt(const PromptParams& p, const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv,
                          unsigned grid, cudaStream_t st) {
-  auto kern = prompt_attn_kernel<DP, BF16>;
+  constexpr auto kern = prompt_attn_kernel<DP, BF16>;
   const int smem = int(sizeof(PromptSmem<DP>));
   static_assert(sizeof(PromptSmem<DP>) <= 227 * 1024, "one CTA's shared memory");
-  const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-  if (e != cudaSuccess) {
-    set_last_cuda_error(e);
-    return B2F_ERR_CUDA;
-  }
+  const int set = allow_smem<kern>(smem);
+  if (set != B2F_OK) return set;
   return launch_kernel(kern, dim3{grid}, dim3{PA_THREADS}, size_t(smem), st, p, mq, mk, mv);
 }
 

@@ -505,13 +505,10 @@ static int launch_norm_rope(const NormRopeParams& p, cudaStream_t st) {
   // a CTA each up to 4 per SM: measured for 36 heads of 128 at 592 tokens, few F1, stream F2
   if (p.T <= 4 * 148)
     return launch_kernel(qk_norm_rope_few_kernel<Tag, D, APPEND>, dim3{unsigned(p.T)}, dim3{256}, 0, st, p);
-  auto kern = qk_norm_rope_stream_kernel<Tag, D, APPEND>;
+  constexpr auto kern = qk_norm_rope_stream_kernel<Tag, D, APPEND>;
   constexpr int smem = NR_WARPS * NR_STAGES * NR_CHUNK;
-  const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-  if (e != cudaSuccess) {
-    set_last_cuda_error(e);
-    return B2F_ERR_CUDA;
-  }
+  const int set = allow_smem<kern>(smem);
+  if (set != B2F_OK) return set;
   const int want = p.T, most = NR_CTAS * 148;
   return launch_kernel(kern, dim3{unsigned(want < most ? want : most)}, dim3{32 * NR_WARPS}, smem, st, p);
 }
