@@ -16,12 +16,14 @@
 // maximum: it moves, and O is rescaled, only where a row's new maximum passes
 // it by more than 8 (P stays below 2^8), which after the first blocks is rare.
 // So a row's two threads have to agree on one bit per block (a reduction in
-// the barrier that keeps P off the scores still being read), and the rescale
-// needs no warps of its own.
+// the barrier that keeps P off the scores still being read; each leaves its
+// maximum for the other before it), and the rescale needs no warps of its own.
 //
 // Warps: 0-7 softmax of tile 0, 8-15 of tile 1 (also the epilogue), 16 issues
 // the MMAs, 17 plans the items and issues the TMA loads, 18-19 mend value
-// tiles (below).  The two tiles alternate on the tensor core: while it works
+// tiles (below) and store the output of whole tiles, which the epilogue leaves
+// in a ring stage (rows of a tile written by their threads cost a shared-memory
+// port cycle per 128-byte line: 4500 cycles a tile).  The two tiles alternate on the tensor core: while it works
 // on one, the other's softmax runs.  One thread per row left a warp of each
 // tile on a scheduler, 2400 cycles a block of softmax and 1250 of MMA in a
 // chain (1.17 PFLOP/s at 16384 tokens); two threads shorten the former.
@@ -53,11 +55,25 @@ struct PromptParams {
   int negate;     // softmax_scale < 0: the MMA negates Q
   int B, T, Hq, Hkv, G, D, causal;
   int tpt;        // tokens per tile
-  int wide;       // out takes 32-byte stores
 };
 
-struct PromptItem {
+// What the planner hands to the other warps, worked out once.
+struct __align__(16) PromptItem {
   int row0, len, tok0, hk;  // first row and tokens of the sequence, first token of the item, KV head
+  int n0, n1;               // blocks of the tiles
+  int mask;                 // first block in which anything is masked: at most 3 from there, as two tiles span <= 256 tokens
+  int whole;                // bit i: the rows of tile i are all there; it leaves through a ring stage of its own
+
+  __device__ __forceinline__ int blocks() const { return max(n0, n1); }
+  // ring stages of the item: K and V of each block, then those of whole tiles
+  __device__ __forceinline__ int stages() const { return 2 * blocks() + (whole & 1) + (whole >> 1); }
+  __device__ __forceinline__ void plan(const PromptParams& p) {
+    const int t1 = tok0 + p.tpt, e0 = p.causal ? min(len, t1) : len, e1 = t1 >= len ? 0 : p.causal ? min(len, t1 + p.tpt) : len;
+    n0 = (e0 + PA_BN - 1) / PA_BN;
+    n1 = (e1 + PA_BN - 1) / PA_BN;
+    mask = (p.causal ? tok0 : len) / PA_BN;
+    whole = int(t1 <= len) | int(t1 + p.tpt <= len) << 1;
+  }
 };
 
 template <int DP>
@@ -66,13 +82,17 @@ struct PromptSmem {
   static constexpr int STAGES = DP == 128 ? 5 : 8;
   uint8_t q[2][TILE];
   uint8_t ring[STAGES][TILE];  // K_0 V_0 K_1 V_1 ...
-  float exchange[2][128];      // between the two threads of a row
+  union {                      // between the two threads of a row
+    __nv_bfloat16 top[2][2][128];
+    float sum[2][128];
+  } exchange;
+  int quit[2][2];              // per tile and parity of the block: a wait gave up
   uint32_t bad[2][DP];         // per column: first key that is NaN | +inf | -inf, from the first masked block on
   int any_bad[2];
   PromptItem item[2];
   uint4 next;  // the answer of next_cta_ask
   uint64_t full[STAGES], empty[STAGES], q_full, q_empty, s_full[2], p_full[4], pv_done[2], v_raw[PA_MEND],
-      v_fix[PA_MEND], item_full[2], item_empty[2], asked, drain;
+      v_fix[PA_MEND], o_full[2], item_full[2], item_empty[2], asked, drain;
   uint32_t tmem;
   int abort_flag;
 };
@@ -85,28 +105,12 @@ __device__ __forceinline__ bool wait_or_abort(uint64_t* bar, uint32_t parity, vo
   return false;
 }
 
-// Blocks of the item's tiles and the first block in which anything is masked.
-struct PromptBlocks {
-  int n[2], all, kend, mask;
-  __device__ __forceinline__ PromptBlocks(const PromptParams& p, const PromptItem& x) {
-    kend = 0;
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const int t = x.tok0 + i * p.tpt;
-      const int e = t >= x.len ? 0 : p.causal ? min(x.len, t + p.tpt) : x.len;
-      n[i] = (e + PA_BN - 1) / PA_BN;
-      kend = max(kend, e);
-    }
-    all = max(n[0], n[1]);
-    mask = p.causal ? x.tok0 / PA_BN : x.len / PA_BN;  // at most 3 blocks from there: two tiles span <= 256 tokens
-  }
-};
-
 template <int DP, bool BF16>
 __global__ void __launch_bounds__(PA_THREADS, 1) prompt_attn_kernel(const PromptParams p,
                                                                     const __grid_constant__ CUtensorMap tmq,
                                                                     const __grid_constant__ CUtensorMap tmk,
-                                                                    const __grid_constant__ CUtensorMap tmv) {
+                                                                    const __grid_constant__ CUtensorMap tmv,
+                                                                    const __grid_constant__ CUtensorMap tmo) {
   pdl_enter();
   using SM = PromptSmem<DP>;
   constexpr int NST = SM::STAGES, TILE = SM::TILE, HALF = 128 * 128;  // HALF: 64 columns of a tile
@@ -132,9 +136,11 @@ __global__ void __launch_bounds__(PA_THREADS, 1) prompt_attn_kernel(const Prompt
       mbar_init(&sm.p_full[2 * i], 4);
       mbar_init(&sm.p_full[2 * i + 1], 4);
       mbar_init(&sm.pv_done[i], 1);
+      mbar_init(&sm.o_full[i], 8);
       mbar_init(&sm.item_full[i], 1);
       mbar_init(&sm.item_empty[i], 19);  // the warps but the planner's
       sm.any_bad[i] = 0;
+      sm.quit[i][0] = sm.quit[i][1] = 0;
     }
     for (int i = 0; i < PA_MEND; ++i) {
       mbar_init(&sm.v_raw[i], 1);
@@ -185,7 +191,7 @@ __global__ void __launch_bounds__(PA_THREADS, 1) prompt_attn_kernel(const Prompt
         next_cta_ask(&sm.next, &sm.asked);
       }
       // ---- the item of `cta`; sequence B: the rows past the last sequence ----
-      PromptItem x{0, 0, 0, cta % p.Hkv};
+      PromptItem x{0, 0, 0, cta % p.Hkv, 0, 0, 0, 0};
       int left = cta / p.Hkv;
       for (int b0 = 0; b0 <= p.B; b0 += 32) {
         const int b = b0 + lane;
@@ -212,17 +218,22 @@ __global__ void __launch_bounds__(PA_THREADS, 1) prompt_attn_kernel(const Prompt
         }
         left -= __shfl_sync(0xffffffffu, s, 31);
       }
+      if (x.len > 0) x.plan(p);
       if (x.len != 0) publish(x);  // 0: a spare CTA of the grid
       if (ok && x.len > 0) {
-        const PromptBlocks blk(p, x);
+        const int all = x.blocks(), stages = x.stages();
         if (lane == 0 && !producers_stalled()) {  // test control: stalled producers issue nothing
-          auto load = [&](int i) {  // K (even i) or V of block i / 2
+          auto load = [&](int i) {  // K (even i) or V of block i / 2; then the stages of whole tiles
             const int n = it + i, s = n % NST;
             if (n >= NST && !wait_or_abort(&sm.empty[s], uint32_t((n / NST - 1) & 1), abort_flag)) return false;
+            if (i >= 2 * all) {
+              mbar_arrive(&sm.full[s]);
+              return true;
+            }
             // a value block with masked rows lands on a barrier of its own, for warps 18-19
             const int j = i >> 1;
-            const bool mend = (i & 1) && j >= blk.mask;
-            uint64_t* bar = mend ? &sm.v_raw[(mends + j - blk.mask) % PA_MEND] : &sm.full[s];
+            const bool mend = (i & 1) && j >= x.mask;
+            uint64_t* bar = mend ? &sm.v_raw[(mends + j - x.mask) % PA_MEND] : &sm.full[s];
             if (mend) mbar_arrive(&sm.full[s]);
             mbar_arrive_expect_tx(bar, uint32_t(TILE));
             for (int h = 0; h < DP / 64; ++h)
@@ -233,13 +244,13 @@ __global__ void __launch_bounds__(PA_THREADS, 1) prompt_attn_kernel(const Prompt
           ok = load(i++) && load(i++);
           ok = ok && (loads == 0 || wait_or_abort(&sm.q_empty, uint32_t((loads - 1) & 1), abort_flag));
           if (ok) {
-            const int tiles = blk.n[1] ? 2 : 1;
+            const int tiles = x.n1 ? 2 : 1;
             mbar_arrive_expect_tx(&sm.q_full, uint32_t(tiles * (DP / 64) * p.tpt * p.G * 128));
             for (int t = 0; t < tiles; ++t)
               for (int h = 0; h < DP / 64; ++h)
                 tma_load_4d(sm.q[t] + h * HALF, &tmq, 64 * h, 0, x.hk, x.row0 + x.tok0 + t * p.tpt, &sm.q_full);
           }
-          while (ok && i < 2 * blk.all) ok = load(i++);
+          while (ok && i < stages) ok = load(i++);
           if (!ok) {
             // copies already issued land before the CTA goes away
             mbar_wait_bounded(&sm.q_full, uint32_t(loads & 1), 100000000ull);
@@ -247,15 +258,15 @@ __global__ void __launch_bounds__(PA_THREADS, 1) prompt_attn_kernel(const Prompt
               const int n = it + i - k;
               mbar_wait_bounded(&sm.full[n % NST], uint32_t((n / NST) & 1), 100000000ull);
             }
-            for (int j = blk.mask; 2 * j + 1 < i; ++j) {
-              const int m = mends + j - blk.mask;
+            for (int j = x.mask; 2 * j + 1 < min(i, 2 * all); ++j) {
+              const int m = mends + j - x.mask;
               mbar_wait_bounded(&sm.v_raw[m % PA_MEND], uint32_t((m / PA_MEND) & 1), 100000000ull);
             }
           }
         }
         ok = __shfl_sync(0xffffffffu, int(ok), 0) != 0;
-        it += 2 * blk.all;
-        mends += max(0, blk.all - blk.mask);
+        it += stages;
+        mends += max(0, all - x.mask);
         ++loads;
       }
       // the answer lands whatever happened (a bounded wait)
@@ -269,9 +280,11 @@ __global__ void __launch_bounds__(PA_THREADS, 1) prompt_attn_kernel(const Prompt
       __syncwarp();
       if (cta < 0) break;
     }
-    if (ok) publish(PromptItem{0, PA_STOP, 0, 0});
+    if (ok) publish(PromptItem{0, PA_STOP, 0, 0, 0, 0, 0, 0});
   } else if (warp >= 18) {
-    // ============================ value tiles with masked rows ==================
+    // ================ value tiles with masked rows; whole tiles' output ==========
+    const int tile = warp - 18;
+    int stored = 0;
     int it = 0, mends = 0;
     for (int k = 0;; ++k) {
       const int slot = k & 1;
@@ -280,13 +293,14 @@ __global__ void __launch_bounds__(PA_THREADS, 1) prompt_attn_kernel(const Prompt
       if (x.len == PA_STOP) break;
       bool ok = true;
       if (x.len > 0) {
-        const PromptBlocks blk(p, x);
-        for (int j = blk.mask; j < blk.all; ++j, ++mends) {
+        const int all = x.blocks();
+        const int kend = p.causal ? min(x.len, x.tok0 + 2 * p.tpt) : x.len;  // keys of the item
+        for (int j = x.mask; j < all; ++j, ++mends) {
           const int b = mends % PA_MEND;
           ok = __all_sync(0xffffffffu, wait_or_abort(&sm.v_raw[b], uint32_t((mends / PA_MEND) & 1), abort_flag));
           if (!ok) break;
           uint8_t* v = sm.ring[(it + 2 * j + 1) % NST];
-          const int valid = min(PA_BN, blk.kend - j * PA_BN);
+          const int valid = min(PA_BN, kend - j * PA_BN);
           // a line = 64 columns of one key; the two warps take four lines each in turn
           for (int line = (warp - 18) * 4 + (lane >> 3); line < 128 * (DP / 64); line += 8) {
             const int key = line & 127, h = line >> 7, c = lane & 7;
@@ -305,7 +319,7 @@ __global__ void __launch_bounds__(PA_THREADS, 1) prompt_attn_kernel(const Prompt
                   const uint32_t y = (u[e >> 1] >> (16 * (e & 1))) & 0xFFFFu;
                   if ((y & expo) != expo) continue;
                   const int at10 = (y & ~expo & 0x7FFFu) ? 0 : (y & 0x8000u) ? 20 : 10;  // NaN, +inf, -inf
-                  const uint32_t off = uint32_t((j - blk.mask) * PA_BN + key);
+                  const uint32_t off = uint32_t((j - x.mask) * PA_BN + key);
                   uint32_t* word = &sm.bad[slot][64 * h + 8 * c + e];
                   uint32_t old = *word, seen;
                   do {
@@ -324,7 +338,18 @@ __global__ void __launch_bounds__(PA_THREADS, 1) prompt_attn_kernel(const Prompt
           __syncwarp();
           if (lane == 0) mbar_arrive(&sm.v_fix[b]);
         }
-        it += 2 * blk.all;
+        if (ok && (x.whole >> tile & 1)) {
+          const int s = (it + 2 * all + tile) % NST;  // (a whole second tile follows a whole first)
+          ok = __all_sync(0xffffffffu, wait_or_abort(&sm.o_full[tile], uint32_t(stored++ & 1), abort_flag));
+          if (ok && lane == 0) {
+            for (int c = 0; c < DP / 64; ++c)
+              if (64 * c < p.D) tma_store_4d(&tmo, sm.ring[s] + c * HALF, 64 * c, 0, x.hk, x.row0 + x.tok0 + tile * p.tpt);
+            bulk_s2g_wait();
+            mbar_arrive(&sm.empty[s]);
+          }
+          __syncwarp();
+        }
+        it += x.stages();
       }
       if (!ok) break;
       if (lane == 0) mbar_arrive(&sm.item_empty[slot]);
@@ -364,33 +389,33 @@ __global__ void __launch_bounds__(PA_THREADS, 1) prompt_attn_kernel(const Prompt
       const int slot = k & 1;
       ok = wait_all(&sm.item_full[slot], uint32_t((k / 2) & 1));
       if (!ok) break;
-      PromptItem x = sm.item[slot];
-      x.row0 = __shfl_sync(0xffffffffu, x.row0, 0);
-      x.len = __shfl_sync(0xffffffffu, x.len, 0);
-      x.tok0 = __shfl_sync(0xffffffffu, x.tok0, 0);
-      if (x.len == PA_STOP) break;
-      if (x.len > 0) {
-        const PromptBlocks blk(p, x);
+      const PromptItem& x = sm.item[slot];
+      const int len = __shfl_sync(0xffffffffu, x.len, 0);
+      if (len == PA_STOP) break;
+      if (len > 0) {
+        const int nb[2] = {__shfl_sync(0xffffffffu, x.n0, 0), __shfl_sync(0xffffffffu, x.n1, 0)};
+        const int mask = __shfl_sync(0xffffffffu, x.mask, 0), whole = __shfl_sync(0xffffffffu, x.whole, 0);
+        const int all = max(nb[0], nb[1]);
         ok = wait_all(&sm.q_full, uint32_t(loads++ & 1)) && full_of(ring);
         if (!ok) break;
         tc_fence_after();
         for (int i = 0; i < 2; ++i)
-          if (blk.n[i]) score(i, ring.s);
+          if (nb[i]) score(i, ring.s);
         tc_commit_by(one, &sm.empty[ring.s]);
-        if (blk.all == 1) tc_commit_by(one, &sm.q_empty);
-        for (int j = 0; ok && j < blk.all; ++j) {
+        if (all == 1) tc_commit_by(one, &sm.q_empty);
+        for (int j = 0; ok && j < all; ++j) {
           ring.next();
           const Ring rv = ring;  // V_j
-          if (j < blk.mask) {
+          if (j < mask) {
             ok = full_of(rv);
           } else {
             ok = wait_all(&sm.v_fix[mends % PA_MEND], uint32_t((mends / PA_MEND) & 1));
             ++mends;
           }
-          if (j + 1 < blk.all) ring.next();  // K_{j+1}
+          if (j + 1 < all) ring.next();  // K_{j+1}
           bool next = false;                 // it has landed
           for (int i = 0; ok && i < 2; ++i) {
-            if (j >= blk.n[i]) continue;
+            if (j >= nb[i]) continue;
             const uint64_t v = v_desc + uint64_t(rv.s * (TILE >> 4));
             for (int h = 0; ok && h < 2; ++h) {  // O_i += P_i V_j
               ok = wait_all(&sm.p_full[2 * i + h], uint32_t(done[i] & 1));
@@ -404,17 +429,17 @@ __global__ void __launch_bounds__(PA_THREADS, 1) prompt_attn_kernel(const Prompt
             if (!ok) break;
             ++done[i];
             tc_commit_by(one, &sm.pv_done[i]);
-            if (j + 1 < blk.n[i]) {
+            if (j + 1 < nb[i]) {
               if (!next) ok = next = full_of(ring);
               if (ok) score(i, ring.s);
             }
           }
           if (!ok) break;
           tc_commit_by(one, &sm.empty[rv.s]);
-          if (j + 1 < blk.all) tc_commit_by(one, &sm.empty[ring.s]);
-          if (j + 2 == blk.all) tc_commit_by(one, &sm.q_empty);  // the last scores are issued
+          if (j + 1 < all) tc_commit_by(one, &sm.empty[ring.s]);
+          if (j + 2 == all) tc_commit_by(one, &sm.q_empty);  // the last scores are issued
         }
-        ring.next();
+        for (int i = 0; i <= (whole & 1) + (whole >> 1); ++i) ring.next();
       }
       if (ok && lane == 0) mbar_arrive(&sm.item_empty[slot]);
     }
@@ -433,18 +458,17 @@ __global__ void __launch_bounds__(PA_THREADS, 1) prompt_attn_kernel(const Prompt
     auto wait_all = [&](uint64_t* b, uint32_t parity) {
       return bool(__all_sync(0xffffffffu, wait_or_abort(b, parity, abort_flag)));
     };
-    // max (or sum) with the row's other thread
-    auto join = [&](float v, bool add) {
-      if (h) sm.exchange[i][r] = v;
+    // sum over the row's two threads
+    auto joined = [&](float v) {
+      if (h) sm.exchange.sum[i][r] = v;
       bar_all(bar, 256);
-      if (!h) {
-        const float o = sm.exchange[i][r];
-        v = add ? v + o : fmaxf(v, o);
-        sm.exchange[i][r] = v;
-      }
+      if (!h) sm.exchange.sum[i][r] = v += sm.exchange.sum[i][r];
       bar_all(bar, 256);
-      return h ? sm.exchange[i][r] : v;
+      return h ? sm.exchange.sum[i][r] : v;
     };
+    const int rt = r / p.G, rh = r - rt * p.G;  // token of the tile, head of the group
+    const bool row_of_tile = r < p.tpt * p.G;
+    int it = 0;
     int done = 0;  // blocks of this tile so far
     for (int k = 0;; ++k) {
       const int slot = k & 1;
@@ -465,10 +489,9 @@ __global__ void __launch_bounds__(PA_THREADS, 1) prompt_attn_kernel(const Prompt
         if (lane == 0) mbar_arrive(&sm.item_empty[slot]);
         continue;
       }
-      const PromptBlocks blk(p, x);
-      const int nb = blk.n[i];
-      const int t = x.tok0 + i * p.tpt + r / p.G;
-      const bool live = r < p.tpt * p.G && t < x.len;
+      const int nb = i ? x.n1 : x.n0;
+      const int t = x.tok0 + i * p.tpt + rt;
+      const bool live = row_of_tile && t < x.len;
       const int last = !live ? -1 : p.causal ? t : x.len - 1;  // last key the row sees
       float m = -INFINITY, l = 0.f;  // m: reference of the exponents (scaled scores)
       bool quit = false;
@@ -477,7 +500,7 @@ __global__ void __launch_bounds__(PA_THREADS, 1) prompt_attn_kernel(const Prompt
         tc_fence_after();
         uint32_t s[64];
         tmem_ld64(s_at + 64 * h, s);
-        const bool masked = j >= blk.mask;
+        const bool masked = j >= x.mask;
         if (masked) {
           const int rel = last - j * PA_BN - 64 * h;
 #pragma unroll
@@ -485,13 +508,18 @@ __global__ void __launch_bounds__(PA_THREADS, 1) prompt_attn_kernel(const Prompt
             if (c > rel) s[c] = 0xFF800000u;
         }
         const float top = row_max(s) * p.scale2;
-        // every score of the tile has been read past this barrier
+        // every score of the tile has been read past this barrier, and what a
+        // thread leaves before it can be read by the others: its maximum (to 8
+        // bits: both take the same value, a reference need not be exact)
+        const __nv_bfloat16 top8 = __float2bfloat16_rn(top);
+        sm.exchange.top[i][h][r] = top8;
+        if (!ok) sm.quit[i][j & 1] = 1;
         if (bar_or(bar, 256, !ok || j == 0 || top > m + 8.f)) {
-          if (bar_or(bar, 256, !ok)) {
+          if (*const_cast<volatile int*>(&sm.quit[i][j & 1])) {
             quit = true;
             break;
           }
-          const float both = join(top, false);
+          const float both = fmaxf(__bfloat162float(top8), __bfloat162float(sm.exchange.top[i][1 - h][r]));
           const bool move = j == 0 || both > m + 8.f;
           if (j > 0) {
             // O holds blocks up to j - 1 once their product is done
@@ -527,13 +555,18 @@ __global__ void __launch_bounds__(PA_THREADS, 1) prompt_attn_kernel(const Prompt
       }
       if (quit) break;
       if (nb) {
-        l = join(l, true);
         ok = ok && wait_all(&sm.pv_done[i], uint32_t((done - 1) & 1));
         tc_fence_after();
-        const int64_t row = int64_t(x.row0 + t) * p.Hq + x.hk * p.G + r % p.G;
+        l = joined(l);  // (the last product needed every thread's P: all maxima have been read)
+        const int64_t row = int64_t(x.row0 + t) * p.Hq + x.hk * p.G + rh;
         const float inv = l > 0.f ? 1.f / l : l;  // l is NaN where a score is
         const bool any_bad = *const_cast<volatile int*>(&sm.any_bad[slot]) != 0;
-        const int seen = t - blk.mask * PA_BN;  // keys up to here, from the first masked block
+        const int seen = t - x.mask * PA_BN;  // keys up to here, from the first masked block
+        // a whole tile leaves through the ring stage that the planner grants it
+        const bool staged = x.whole >> i & 1;
+        const int n = it + 2 * x.blocks() + i;  // (a whole second tile follows a whole first)
+        uint8_t* stage = sm.ring[n % NST];
+        if (staged) ok = ok && wait_all(&sm.full[n % NST], uint32_t((n / NST) & 1));
         if (ok) {
 #pragma unroll
           for (int c = 0; c < DP / 2; c += 32) {
@@ -557,11 +590,15 @@ __global__ void __launch_bounds__(PA_THREADS, 1) prompt_attn_kernel(const Prompt
               w[e] = BF16 ? pack_bf16x2(y0, y1) : pack_f16x2(y0, y1);
             }
             const int d = DP / 2 * h + c;
-            uint16_t* dst = static_cast<uint16_t*>(p.out) + row * p.D + d;
-            if (live && p.wide && d + 32 <= p.D) {  // whole 32-byte sectors
-              store_32b(dst, &w[0]);
-              store_32b(dst + 16, &w[8]);
+            if (staged) {
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                const int col = d / 8 + e;  // 16-byte column of the row
+                *reinterpret_cast<uint4*>(stage + (col >> 3) * HALF + r * 128 + (((col & 7) ^ (r & 7)) << 4)) =
+                    make_uint4(w[4 * e], w[4 * e + 1], w[4 * e + 2], w[4 * e + 3]);
+              }
             } else if (live) {
+              uint16_t* dst = static_cast<uint16_t*>(p.out) + row * p.D + d;
 #pragma unroll
               for (int e = 0; e < 4; ++e)
                 if (d + 8 * e < p.D)
@@ -569,11 +606,15 @@ __global__ void __launch_bounds__(PA_THREADS, 1) prompt_attn_kernel(const Prompt
             }
             __syncwarp();
           }
+          if (staged) fence_proxy_async_smem();
           if (live && p.lse && h == 0)
             p.lse[row] = l > 0.f ? (m + log2f(l)) * 0.6931471805599453f : l == 0.f ? -INFINITY : l;
         }
         tc_fence_before();
+        __syncwarp();
+        if (staged && ok && lane == 0) mbar_arrive(&sm.o_full[i]);  // warp 18 or 19 stores it
       }
+      it += x.stages();
       __syncwarp();
       if (lane == 0) mbar_arrive(&sm.item_empty[slot]);
       // a wait that gave up is told at the next item's barrier (the flag makes that wait fail too)
@@ -612,13 +653,13 @@ static int make_rows_map(CUtensorMap* map, const void* base, bool bf16, int64_t 
 
 template <int DP, bool BF16>
 static int launch_prompt(const PromptParams& p, const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv,
-                         unsigned grid, cudaStream_t st) {
+                         const CUtensorMap& mo, unsigned grid, cudaStream_t st) {
   constexpr auto kern = prompt_attn_kernel<DP, BF16>;
   const int smem = int(sizeof(PromptSmem<DP>));
   static_assert(sizeof(PromptSmem<DP>) <= 227 * 1024, "one CTA's shared memory");
   const int set = allow_smem<kern>(smem);
   if (set != B2F_OK) return set;
-  return launch_kernel(kern, dim3{grid}, dim3{PA_THREADS}, size_t(smem), st, p, mq, mk, mv);
+  return launch_kernel(kern, dim3{grid}, dim3{PA_THREADS}, size_t(smem), st, p, mq, mk, mv, mo);
 }
 
 B2F_DEFINE_WAIT_CONTROLS(prompt_attn)
@@ -648,16 +689,17 @@ extern "C" int b2f_prompt_attn(const void* q, int64_t q_row, int64_t q_head, con
   const int64_t items = (T / (2 * tpt) + B + 1) * Hkv;
   if (items > 0x7fffffff) return B2F_ERR_UNSUPPORTED;
   const bool bf16 = dtype == B2F_BF16;
-  CUtensorMap mq, mk, mv;
+  CUtensorMap mq, mk, mv, mo;
   if ((rc = make_rows_map(&mq, q, bf16, D, G, Hkv, T, q_head, q_row, int(G), int(tpt))) != B2F_OK ||
       (rc = make_rows_map(&mk, k, bf16, D, 0, Hkv, T, k_head, k_row, 0, PA_BN)) != B2F_OK ||
-      (rc = make_rows_map(&mv, v, bf16, D, 0, Hkv, T, v_head, v_row, 0, PA_BN)) != B2F_OK)
+      (rc = make_rows_map(&mv, v, bf16, D, 0, Hkv, T, v_head, v_row, 0, PA_BN)) != B2F_OK ||
+      (rc = make_rows_map(&mo, out, bf16, D, G, Hkv, T, D, Hq * D, int(G), int(tpt))) != B2F_OK)
     return rc;
   const float s2 = fabsf(softmax_scale) * kLog2e;
   PromptParams p{cu_seqlens, out, lse, s2 > 1e-30f ? s2 : 1e-30f, softmax_scale < 0.f, int(B), int(T), int(Hq),
-                 int(Hkv), int(G), int(D), causal != 0, int(tpt), aligned(out, 32) && D % 16 == 0};
+                 int(Hkv), int(G), int(D), causal != 0, int(tpt)};
   cudaStream_t st = as_stream(stream);
   const unsigned n = unsigned(items);
-  if (bf16) return D <= 64 ? launch_prompt<64, true>(p, mq, mk, mv, n, st) : launch_prompt<128, true>(p, mq, mk, mv, n, st);
-  return D <= 64 ? launch_prompt<64, false>(p, mq, mk, mv, n, st) : launch_prompt<128, false>(p, mq, mk, mv, n, st);
+  if (bf16) return D <= 64 ? launch_prompt<64, true>(p, mq, mk, mv, mo, n, st) : launch_prompt<128, true>(p, mq, mk, mv, mo, n, st);
+  return D <= 64 ? launch_prompt<64, false>(p, mq, mk, mv, mo, n, st) : launch_prompt<128, false>(p, mq, mk, mv, mo, n, st);
 }
