@@ -33,6 +33,7 @@ int launch_own_partials(const __nv_bfloat16* q, const uint8_t* kc, const float* 
 constexpr int PX_THREADS = 864;
 constexpr int PX_MMA = 24, PX_COPY = 25;
 constexpr int PX_BN = 128;  // keys per block
+constexpr int PX_SMS = 148;
 // Stages alternate K and V (it = 2 j, 2 j + 1): an even number, so that a
 // stage holds one of the two only and its readers see its phases in turn.
 constexpr int PX_RAW = 2;   // blocks of codes in flight
@@ -46,7 +47,7 @@ struct PrefixParams {
   float *o_part, *ml_part;
   float scale2;   // |softmax_scale| * log2(e)
   int negate;     // softmax_scale < 0: the MMA negates Q
-  int B, Ng, Hq, Hkv, G, P, tpt, n_splits, part_stride, max_prefix;
+  int B, Ng, Hq, Hkv, G, P, tpt, max_splits, part_stride, max_prefix;
   int beside;     // launched to run beside the previous kernel (see launch_prefix)
 };
 
@@ -62,7 +63,8 @@ struct PrefixSmem {
   float largest[2][4];             // scales of the first block (K, V), per decoding warp
   uint64_t raw_full[PX_RAW], raw_empty[PX_RAW], full[PX_RING], empty[PX_RING], q_full, s_full[2], p_full[4], pv_done[2],
       drain;
-  int item[4];  // group, first request, requests from there, prefix length
+  int item[6];  // group, first request, requests from there, prefix length, KV head, split
+  int splits;
   uint32_t tmem;
   int abort_flag;
 };
@@ -101,6 +103,19 @@ __device__ __forceinline__ void spread_codes(const uint4& q, uint32_t (&w)[32 / 
   }
 }
 
+// Splits of each prefix: enough for one CTA per SM (a CTA takes the whole SM's
+// shared memory), by how many pairs of tiles the groups make -- which only the
+// device knows.  Called by whole warps.
+__device__ __forceinline__ int splits_of(const int32_t* off, int Ng, int B, int span, int Hkv, int max_splits) {
+  int pairs = 0;
+  for (int g = threadIdx.x & 31; g < Ng; g += 32) {
+    const int lo = min(max(off[g], 0), B), hi = min(max(off[g + 1], lo), B);
+    pairs += (hi - lo + span - 1) / span;
+  }
+  pairs = __reduce_add_sync(0xffffffffu, pairs);
+  return max(1, min(max_splits, PX_SMS / max(1, pairs * Hkv)));
+}
+
 __device__ __forceinline__ bool px_wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag) {
   if (*abort_flag) return false;
   if (mbar_wait_bounded(bar, parity)) return true;
@@ -127,10 +142,11 @@ __global__ void __launch_bounds__(PX_THREADS, 1) prefix_attn_kernel(const Prefix
     return;
   }
 
-  const int split = blockIdx.x % p.n_splits, hk = blockIdx.x / p.n_splits % p.Hkv;
   if (warp == 0) {
-    int left = blockIdx.x / p.n_splits / p.Hkv, g = -1, row0 = 0, rows = 0, len = 0;
     const int span = 2 * p.tpt;
+    const int splits = splits_of(p.off, p.Ng, p.B, span, p.Hkv, p.max_splits);
+    const int split = blockIdx.x % splits, hk = blockIdx.x / splits % p.Hkv;
+    int left = blockIdx.x / splits / p.Hkv, g = -1, row0 = 0, rows = 0, len = 0;
     for (int g0 = 0; g0 < p.Ng && g < 0; g0 += 32) {
       int lo = 0, hi = 0, n = 0;
       if (g0 + lane < p.Ng) {
@@ -162,6 +178,9 @@ __global__ void __launch_bounds__(PX_THREADS, 1) prefix_attn_kernel(const Prefix
       sm.item[1] = row0;
       sm.item[2] = rows;
       sm.item[3] = len;
+      sm.item[4] = hk;
+      sm.item[5] = split;
+      sm.splits = splits;
     }
   } else if (tid == 32) {
     for (int s = 0; s < PX_RAW; ++s) {
@@ -193,7 +212,9 @@ __global__ void __launch_bounds__(PX_THREADS, 1) prefix_attn_kernel(const Prefix
   const uint32_t tmem = __shfl_sync(0xffffffffu, sm.tmem, 0);
   const int g = __shfl_sync(0xffffffffu, sm.item[0], 0), row0 = __shfl_sync(0xffffffffu, sm.item[1], 0);
   const int rows = __shfl_sync(0xffffffffu, sm.item[2], 0), len = __shfl_sync(0xffffffffu, sm.item[3], 0);
-  const int blocks = (len + PX_BN - 1) / PX_BN, per = (blocks + p.n_splits - 1) / p.n_splits;
+  const int hk = __shfl_sync(0xffffffffu, sm.item[4], 0), split = __shfl_sync(0xffffffffu, sm.item[5], 0);
+  const int splits = __shfl_sync(0xffffffffu, sm.splits, 0);
+  const int blocks = (len + PX_BN - 1) / PX_BN, per = (blocks + splits - 1) / splits;
   const int j0 = split * per;
   const int n = g < 0 ? 0 : min(blocks, j0 + per) - j0;  // this split's blocks (g < 0: a spare CTA of the grid)
   const int n_tiles = rows > p.tpt ? 2 : 1;
@@ -543,8 +564,9 @@ __global__ void __launch_bounds__(PX_THREADS, 1) prefix_attn_kernel(const Prefix
 template <int D>
 __global__ void __launch_bounds__(256) prefix_combine_kernel(const float* __restrict__ o_part,
                                                              const float* __restrict__ ml_part,
-                                                             const int32_t* __restrict__ off, int Ng, int rows, int Hq,
-                                                             int n_prefix, int n, __nv_bfloat16* __restrict__ out) {
+                                                             const int32_t* __restrict__ off, int Ng, int rows, int B, int Hq,
+                                                             int Hkv, int span, int n_prefix, int n,
+                                                             __nv_bfloat16* __restrict__ out) {
   pdl_enter();
   constexpr int V = D / 32;
   const int64_t bh = int64_t(blockIdx.x) * 8 + (threadIdx.x >> 5);
@@ -553,26 +575,31 @@ __global__ void __launch_bounds__(256) prefix_combine_kernel(const float* __rest
   const int b = int(bh / Hq);
   bool in = false;
   for (int g = lane; g < Ng; g += 32) in |= b >= off[g] && b < off[g + 1];
-  const int s0 = __any_sync(0xffffffffu, in) ? 0 : n_prefix;
+  // partials: splits 0..sp of the prefix, then n_prefix.. of the own tokens
+  const int sp = __any_sync(0xffffffffu, in) ? splits_of(off, Ng, B, span, Hkv, n_prefix) : 0;
+  const int count = sp + n - n_prefix;
+  const int gap = n_prefix - sp;
   const float2* ml = reinterpret_cast<const float2*>(ml_part) + bh * n;
   const float* o = o_part + bh * n * D + lane * V;
   float top = -INFINITY;
-  for (int s = s0 + lane; s < n; s += 32) top = fmaxf(top, ml[s].x);
+  for (int s = lane; s < count; s += 32) top = fmaxf(top, ml[s < sp ? s : s + gap].x);
   top = warp_max<32>(top);
   float acc[V], l = 0.f;
 #pragma unroll
   for (int v = 0; v < V; ++v) acc[v] = 0.f;
-  for (int c0 = s0; c0 < n; c0 += 32) {
-    const float2 x = c0 + lane < n ? ml[c0 + lane] : make_float2(0.f, 0.f);
+  for (int c0 = 0; c0 < count; c0 += 32) {
+    const int s = c0 + lane;
+    const float2 x = s < count ? ml[s < sp ? s : s + gap] : make_float2(0.f, 0.f);
     // an empty split wrote no partial; NaN sums stay
     const float f = x.y == 0.f ? 0.f : top == -INFINITY ? 1.f : ex2(x.x - top);
     const unsigned some = __ballot_sync(0xffffffffu, x.y != 0.f);
     l += warp_sum<32>(x.y == 0.f ? 0.f : f * x.y);
-    for (int k0 = 0; k0 < min(32, n - c0); k0 += 8) {
+    for (int k0 = 0; k0 < min(32, count - c0); k0 += 8) {
       float v[8][V];
 #pragma unroll
       for (int k = 0; k < 8; ++k) {
-        const float* src = o + int64_t(c0 + k0 + k) * D;
+        const int at = c0 + k0 + k;
+        const float* src = o + int64_t(at < sp ? at : at + gap) * D;
         const bool on = (some >> (k0 + k)) & 1;
         if constexpr (V == 4) {
           const float4 y = on ? *reinterpret_cast<const float4*>(src) : make_float4(0.f, 0.f, 0.f, 0.f);
@@ -599,10 +626,10 @@ __global__ void __launch_bounds__(256) prefix_combine_kernel(const float* __rest
 }
 
 template <int D>
-static int launch_combine(const float* o_part, const float* ml_part, const int32_t* off, int Ng, int64_t rows, int Hq,
-                          int n_prefix, int n, __nv_bfloat16* out, cudaStream_t st) {
-  return launch_kernel(prefix_combine_kernel<D>, dim3{unsigned((rows + 7) / 8)}, dim3{256}, 0, st, o_part, ml_part, off,
-                       Ng, int(rows), Hq, n_prefix, n, out);
+static int launch_combine(const float* o_part, const float* ml_part, const int32_t* off, int Ng, int64_t B, int Hq,
+                          int Hkv, int span, int n_prefix, int n, __nv_bfloat16* out, cudaStream_t st) {
+  return launch_kernel(prefix_combine_kernel<D>, dim3{unsigned((B * Hq + 7) / 8)}, dim3{256}, 0, st, o_part, ml_part, off,
+                       Ng, int(B * Hq), int(B), Hq, Hkv, span, n_prefix, n, out);
 }
 
 // With `beside` the kernel follows the requests' own-token kernel, whose
@@ -633,13 +660,11 @@ static int launch_prefix_bits(const PrefixParams& p, int bits, unsigned grid, cu
   return launch_prefix<DP, 2>(p, grid, st);
 }
 
-// Splits of the prefix: enough for one CTA per SM (a CTA takes the whole
-// SM's shared memory), at most one per block of keys.
-static int prefix_splits(int64_t B, int64_t G, int64_t Hkv, int64_t Ng, int64_t max_prefix) {
+// Most splits that a prefix can get (one pair of tiles in all; a split has a
+// block of keys at least): the partials' room.
+static int prefix_splits(int64_t B, int64_t Hkv, int64_t Ng, int64_t max_prefix) {
   if (Ng <= 0 || max_prefix <= 0 || B <= 0) return 0;
-  const int64_t span = 2 * (128 / G), per_group = (B + Ng - 1) / Ng;
-  const int64_t ctas = Ng * ((per_group + span - 1) / span) * Hkv, blocks = (max_prefix + PX_BN - 1) / PX_BN;
-  const int64_t want = 148 / ctas > 1 ? 148 / ctas : 1;
+  const int64_t blocks = (max_prefix + PX_BN - 1) / PX_BN, want = PX_SMS / Hkv > 1 ? PX_SMS / Hkv : 1;
   return int(want < blocks ? want : blocks);
 }
 
@@ -663,7 +688,7 @@ extern "C" {
 int64_t b2f_shared_prefix_attn_workspace_bytes(int64_t B, int64_t Hq, int64_t Hkv, int64_t D, int64_t n_groups,
                                                int64_t max_prefix, int64_t max_own) {
   if (B <= 0 || Hq <= 0 || Hkv <= 0 || D <= 0 || Hq / Hkv > 16) return 0;
-  const int64_t n = prefix_splits(B, Hq / Hkv, Hkv, n_groups, max_prefix) + own_splits(B, Hkv, max_own);
+  const int64_t n = prefix_splits(B, Hkv, n_groups, max_prefix) + own_splits(B, Hkv, max_own);
   return B * Hq * n * (D + 2) * int64_t(sizeof(float));
 }
 
@@ -692,7 +717,7 @@ int b2f_shared_prefix_attn(const void* q, const uint8_t* k_pages, const float* k
   const int64_t G = Hq / Hkv, tpt = 128 / G;
   if (max_prefix > prefix_pages * page_size) max_prefix = prefix_pages * page_size;
   if (max_own > max_pages * page_size) max_own = max_pages * page_size;
-  const int np = prefix_splits(B, G, Hkv, n_groups, max_prefix), no = own_splits(B, Hkv, max_own), n = np + no;
+  const int np = prefix_splits(B, Hkv, n_groups, max_prefix), no = own_splits(B, Hkv, max_own), n = np + no;
   if (n > 0) {
     if (!workspace || workspace_bytes < B * Hq * n * (D + 2) * int64_t(sizeof(float))) return B2F_ERR_WORKSPACE;
     if (!aligned(workspace, 16)) return B2F_ERR_ALIGN;
@@ -709,8 +734,8 @@ int b2f_shared_prefix_attn(const void* q, const uint8_t* k_pages, const float* k
     if (rc != B2F_OK) return rc;
   }
   if (np > 0) {
-    // items: at most one partial pair of tiles per group
-    const int64_t grid = (B / (2 * tpt) + n_groups) * Hkv * np;
+    // pairs of tiles: at most one partial pair per group; more splits than one only while they fit the SMs
+    const int64_t pairs = (B / (2 * tpt) + n_groups) * Hkv, grid = pairs > PX_SMS ? pairs : PX_SMS;
     if (grid > 0x7fffffff) return B2F_ERR_UNSUPPORTED;
     const float s2 = fabsf(softmax_scale) * kLog2e;
     PrefixParams p{qb, k_pages, v_pages, k_scales, v_scales, prefix_table, prefix_lens, group_offsets, prefix_pages,
@@ -722,8 +747,8 @@ int b2f_shared_prefix_attn(const void* q, const uint8_t* k_pages, const float* k
   }
   __nv_bfloat16* ob = static_cast<__nv_bfloat16*>(out);
   const int Ng = np > 0 ? int(n_groups) : 0;
-  return D == 64 ? launch_combine<64>(o_part, ml_part, group_offsets, Ng, B * Hq, int(Hq), np, n, ob, st)
-                 : launch_combine<128>(o_part, ml_part, group_offsets, Ng, B * Hq, int(Hq), np, n, ob, st);
+  return D == 64 ? launch_combine<64>(o_part, ml_part, group_offsets, Ng, B, int(Hq), int(Hkv), int(2 * tpt), np, n, ob, st)
+                 : launch_combine<128>(o_part, ml_part, group_offsets, Ng, B, int(Hq), int(Hkv), int(2 * tpt), np, n, ob, st);
 }
 
 }  // extern "C"
