@@ -106,14 +106,13 @@ __device__ __forceinline__ void spread_codes(const uint4& q, uint32_t (&w)[32 / 
 // Splits of each prefix: enough for one CTA per SM (a CTA takes the whole SM's
 // shared memory), by how many pairs of tiles the groups make -- which only the
 // device knows.  Called by whole warps.
-__device__ __forceinline__ int splits_of(const int32_t* off, int Ng, int B, int span, int Hkv, int max_splits) {
-  int pairs = 0;
-  for (int g = threadIdx.x & 31; g < Ng; g += 32) {
-    const int lo = min(max(off[g], 0), B), hi = min(max(off[g + 1], lo), B);
-    pairs += (hi - lo + span - 1) / span;
-  }
-  pairs = __reduce_add_sync(0xffffffffu, pairs);
+__device__ __forceinline__ int splits_for(int lane_pairs, int Hkv, int max_splits) {
+  const int pairs = __reduce_add_sync(0xffffffffu, lane_pairs);
   return max(1, min(max_splits, PX_SMS / max(1, pairs * Hkv)));
+}
+__device__ __forceinline__ int group_pairs(const int32_t* off, int g, int B, int span) {
+  const int lo = min(max(off[g], 0), B), hi = min(max(off[g + 1], lo), B);
+  return (hi - lo + span - 1) / span;
 }
 
 __device__ __forceinline__ bool px_wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag) {
@@ -144,16 +143,22 @@ __global__ void __launch_bounds__(PX_THREADS, 1) prefix_attn_kernel(const Prefix
 
   if (warp == 0) {
     const int span = 2 * p.tpt;
-    const int splits = splits_of(p.off, p.Ng, p.B, span, p.Hkv, p.max_splits);
+    int lo = 0, hi = 0, n = 0;  // this lane's group
+    auto look = [&](int g) {
+      lo = hi = n = 0;
+      if (g >= p.Ng) return;
+      lo = min(max(p.off[g], 0), p.B);
+      hi = min(max(p.off[g + 1], lo), p.B);
+      n = min(max(p.lens[g], 0), p.max_prefix);
+    };
+    look(lane);
+    int pairs = (hi - lo + span - 1) / span;
+    for (int x = 32 + lane; x < p.Ng; x += 32) pairs += group_pairs(p.off, x, p.B, span);
+    const int splits = splits_for(pairs, p.Hkv, p.max_splits);
     const int split = blockIdx.x % splits, hk = blockIdx.x / splits % p.Hkv;
     int left = blockIdx.x / splits / p.Hkv, g = -1, row0 = 0, rows = 0, len = 0;
     for (int g0 = 0; g0 < p.Ng && g < 0; g0 += 32) {
-      int lo = 0, hi = 0, n = 0;
-      if (g0 + lane < p.Ng) {
-        lo = min(max(p.off[g0 + lane], 0), p.B);
-        hi = min(max(p.off[g0 + lane + 1], lo), p.B);
-        n = min(max(p.lens[g0 + lane], 0), p.max_prefix);
-      }
+      if (g0) look(g0 + lane);
       int s = (hi - lo + span - 1) / span;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
@@ -574,9 +579,14 @@ __global__ void __launch_bounds__(256) prefix_combine_kernel(const float* __rest
   if (bh >= rows) return;
   const int b = int(bh / Hq);
   bool in = false;
-  for (int g = lane; g < Ng; g += 32) in |= b >= off[g] && b < off[g + 1];
+  int pairs = 0;
+  for (int g = lane; g < Ng; g += 32) {
+    in |= b >= off[g] && b < off[g + 1];
+    pairs += group_pairs(off, g, B, span);
+  }
   // partials: splits 0..sp of the prefix, then n_prefix.. of the own tokens
-  const int sp = __any_sync(0xffffffffu, in) ? splits_of(off, Ng, B, span, Hkv, n_prefix) : 0;
+  const int splits = splits_for(pairs, Hkv, n_prefix);
+  const int sp = __any_sync(0xffffffffu, in) ? splits : 0;
   const int count = sp + n - n_prefix;
   const int gap = n_prefix - sp;
   const float2* ml = reinterpret_cast<const float2*>(ml_part) + bh * n;
