@@ -23,11 +23,11 @@
 namespace b2f {
 
 // qkv_attn.cu: decode attention of B rows over their own pages, as partials
-// (o [B * Hq][part_stride][D], then m, l pairs) at splits part_base...
+// (o [B * Hq][n_splits][D], then m, l pairs).
 int launch_own_partials(const __nv_bfloat16* q, const uint8_t* kc, const float* ks, const uint8_t* vc, const float* vs,
                         const int32_t* table, int64_t width, const int32_t* lens, int B, int Hq, int Hkv, int D, int P,
                         int bits, float scale, int n_splits, int max_len, float* o_part, float* ml_part,
-                        int part_stride, int part_base, cudaStream_t st);
+                        cudaStream_t st);
 
 // warps 0-15 softmax, 16-19 decode K, 20-23 V, 24 issues the MMAs, 25 copies K, 26 V
 constexpr int PX_THREADS = 864;
@@ -44,10 +44,10 @@ struct PrefixParams {
   const float *ks, *vs;
   const int32_t *table, *lens, *off;
   int64_t width;
-  float *o_part, *ml_part;
+  float *o_part, *ml_part;  // [CTA][256 rows][DP], [CTA][256 rows] of (m, l)
   float scale2;   // |softmax_scale| * log2(e)
   int negate;     // softmax_scale < 0: the MMA negates Q
-  int B, Ng, Hq, Hkv, G, P, tpt, max_splits, part_stride, max_prefix;
+  int B, Ng, Hq, Hkv, G, P, tpt, max_splits, max_prefix;
   int beside;     // launched to run beside the previous kernel (see launch_prefix)
 };
 
@@ -105,9 +105,8 @@ __device__ __forceinline__ void spread_codes(const uint4& q, uint32_t (&w)[32 / 
 
 // Splits of each prefix: enough for one CTA per SM (a CTA takes the whole SM's
 // shared memory), by how many pairs of tiles the groups make -- which only the
-// device knows.  Called by whole warps.
-__device__ __forceinline__ int splits_for(int lane_pairs, int Hkv, int max_splits) {
-  const int pairs = __reduce_add_sync(0xffffffffu, lane_pairs);
+// device knows.
+__device__ __forceinline__ int splits_for(int pairs, int Hkv, int max_splits) {
   return max(1, min(max_splits, PX_SMS / max(1, pairs * Hkv)));
 }
 __device__ __forceinline__ int group_pairs(const int32_t* off, int g, int B, int span) {
@@ -154,7 +153,7 @@ __global__ void __launch_bounds__(PX_THREADS, 1) prefix_attn_kernel(const Prefix
     look(lane);
     int pairs = (hi - lo + span - 1) / span;
     for (int x = 32 + lane; x < p.Ng; x += 32) pairs += group_pairs(p.off, x, p.B, span);
-    const int splits = splits_for(pairs, p.Hkv, p.max_splits);
+    const int splits = splits_for(__reduce_add_sync(0xffffffffu, pairs), p.Hkv, p.max_splits);
     const int split = blockIdx.x % splits, hk = blockIdx.x / splits % p.Hkv;
     int left = blockIdx.x / splits / p.Hkv, g = -1, row0 = 0, rows = 0, len = 0;
     for (int g0 = 0; g0 < p.Ng && g < 0; g0 += 32) {
@@ -407,7 +406,7 @@ __global__ void __launch_bounds__(PX_THREADS, 1) prefix_attn_kernel(const Prefix
     const int req = i * p.tpt + r / p.G;
     const bool live = g >= 0 && r < p.tpt * p.G && req < rows;
     const int64_t bh = int64_t(row0 + req) * p.Hq + hk * p.G + r % p.G;
-    const int64_t part = bh * p.part_stride + split;
+    const int64_t part = int64_t(blockIdx.x) * 256 + i * 128 + r;
     auto wait_all = [&](uint64_t* b, uint32_t parity) {
       return bool(__all_sync(0xffffffffu, px_wait(b, parity, abort_flag)));
     };
@@ -563,43 +562,65 @@ __global__ void __launch_bounds__(PX_THREADS, 1) prefix_attn_kernel(const Prefix
   if (p.beside) pdl_wait();  // this kernel completes after the one it ran beside
 }
 
-// Splits n_prefix.. are the request's own tokens; the first n_prefix hold
-// something only where the request is in a group.  One warp per (request,
-// head), D / 32 values a lane; the splits are summed in order, 8 loads ahead.
+// One warp per (request, head), D / 32 values a lane, over the partials of its
+// prefix (if it is in a group) and of its own tokens: summed in order, 8 loads
+// ahead.
+struct CombineParams {
+  const float *o_prefix, *ml_prefix;  // [CTA][256][D] and (m, l), as prefix_attn_kernel leaves them
+  const float *o_own, *ml_own;        // [B * Hq][n_own][D] and (m, l)
+  const int32_t* off;
+  __nv_bfloat16* out;
+  int Ng, B, Hq, Hkv, tpt, max_splits, n_own;
+};
+
 template <int D>
-__global__ void __launch_bounds__(256) prefix_combine_kernel(const float* __restrict__ o_part,
-                                                             const float* __restrict__ ml_part,
-                                                             const int32_t* __restrict__ off, int Ng, int rows, int B, int Hq,
-                                                             int Hkv, int span, int n_prefix, int n,
-                                                             __nv_bfloat16* __restrict__ out) {
+__global__ void __launch_bounds__(256) prefix_combine_kernel(const CombineParams p) {
   pdl_enter();
   constexpr int V = D / 32;
   const int64_t bh = int64_t(blockIdx.x) * 8 + (threadIdx.x >> 5);
   const int lane = threadIdx.x & 31;
-  if (bh >= rows) return;
-  const int b = int(bh / Hq);
-  bool in = false;
-  int pairs = 0;
-  for (int g = lane; g < Ng; g += 32) {
-    in |= b >= off[g] && b < off[g + 1];
-    pairs += group_pairs(off, g, B, span);
+  if (bh >= int64_t(p.B) * p.Hq) return;
+  const int b = int(bh / p.Hq), h = int(bh - int64_t(b) * p.Hq), G = p.Hq / p.Hkv, span = 2 * p.tpt;
+  // the request's pair of tiles (over all groups) and its place in the group
+  int pairs = 0, pair = -1, rel = 0;
+  for (int g0 = 0; g0 < p.Ng; g0 += 32) {
+    const int g = g0 + lane;
+    const int lo = g < p.Ng ? min(max(p.off[g], 0), p.B) : 0, hi = g < p.Ng ? min(max(p.off[g + 1], lo), p.B) : 0;
+    const int n = (hi - lo + span - 1) / span;
+    int s = n;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int a = __shfl_up_sync(0xffffffffu, s, o);
+      if (lane >= o) s += a;
+    }
+    const unsigned hit = __ballot_sync(0xffffffffu, b >= lo && b < hi);
+    if (hit && pair < 0) {
+      const int w = __ffs(hit) - 1;
+      rel = b - __shfl_sync(0xffffffffu, lo, w);
+      pair = pairs + __shfl_sync(0xffffffffu, s - n, w) + rel / span;
+    }
+    pairs += __shfl_sync(0xffffffffu, s, 31);
   }
-  // partials: splits 0..sp of the prefix, then n_prefix.. of the own tokens
-  const int splits = splits_for(pairs, Hkv, n_prefix);
-  const int sp = __any_sync(0xffffffffu, in) ? splits : 0;
-  const int count = sp + n - n_prefix;
-  const int gap = n_prefix - sp;
-  const float2* ml = reinterpret_cast<const float2*>(ml_part) + bh * n;
-  const float* o = o_part + bh * n * D + lane * V;
+  const int splits = splits_for(pairs, p.Hkv, p.max_splits), sp = pair < 0 ? 0 : splits;
+  const int count = sp + p.n_own;
+  // partial s of the row: the prefix's splits, then the own tokens'
+  const int64_t at = ((int64_t(pair) * p.Hkv + h / G) * splits) * 256 + rel % span / p.tpt * 128 + rel % p.tpt * G + h % G;
+  auto ml_of = [&](int s) {
+    return s < sp ? reinterpret_cast<const float2*>(p.ml_prefix)[at + s * 256]
+                  : reinterpret_cast<const float2*>(p.ml_own)[bh * p.n_own + s - sp];
+  };
+  auto row_of = [&](int s) {
+    return (s < sp ? p.o_prefix + (at + s * 256) * D : p.o_own + (bh * p.n_own + s - sp) * D) + lane * V;
+  };
   float top = -INFINITY;
-  for (int s = lane; s < count; s += 32) top = fmaxf(top, ml[s < sp ? s : s + gap].x);
+  for (int s = lane; s < count; s += 32) top = fmaxf(top, ml_of(s).x);
   top = warp_max<32>(top);
   float acc[V], l = 0.f;
 #pragma unroll
   for (int v = 0; v < V; ++v) acc[v] = 0.f;
   for (int c0 = 0; c0 < count; c0 += 32) {
     const int s = c0 + lane;
-    const float2 x = s < count ? ml[s < sp ? s : s + gap] : make_float2(0.f, 0.f);
+    const float2 x = s < count ? ml_of(s) : make_float2(0.f, 0.f);
     // an empty split wrote no partial; NaN sums stay
     const float f = x.y == 0.f ? 0.f : top == -INFINITY ? 1.f : ex2(x.x - top);
     const unsigned some = __ballot_sync(0xffffffffu, x.y != 0.f);
@@ -608,9 +629,8 @@ __global__ void __launch_bounds__(256) prefix_combine_kernel(const float* __rest
       float v[8][V];
 #pragma unroll
       for (int k = 0; k < 8; ++k) {
-        const int at = c0 + k0 + k;
-        const float* src = o + int64_t(at < sp ? at : at + gap) * D;
         const bool on = (some >> (k0 + k)) & 1;
+        const float* src = row_of(c0 + k0 + k);
         if constexpr (V == 4) {
           const float4 y = on ? *reinterpret_cast<const float4*>(src) : make_float4(0.f, 0.f, 0.f, 0.f);
           v[k][0] = y.x, v[k][1] = y.y, v[k][2] = y.z, v[k][3] = y.w;
@@ -631,15 +651,8 @@ __global__ void __launch_bounds__(256) prefix_combine_kernel(const float* __rest
   uint32_t y[V / 2];
 #pragma unroll
   for (int e = 0; e < V / 2; ++e) y[e] = pack_bf16x2(acc[2 * e] * inv, acc[2 * e + 1] * inv);
-  if constexpr (V == 4) *reinterpret_cast<uint2*>(out + bh * D + lane * V) = make_uint2(y[0], y[1]);
-  else *reinterpret_cast<uint32_t*>(out + bh * D + lane * V) = y[0];
-}
-
-template <int D>
-static int launch_combine(const float* o_part, const float* ml_part, const int32_t* off, int Ng, int64_t B, int Hq,
-                          int Hkv, int span, int n_prefix, int n, __nv_bfloat16* out, cudaStream_t st) {
-  return launch_kernel(prefix_combine_kernel<D>, dim3{unsigned((B * Hq + 7) / 8)}, dim3{256}, 0, st, o_part, ml_part, off,
-                       Ng, int(B * Hq), int(B), Hq, Hkv, span, n_prefix, n, out);
+  if constexpr (V == 4) *reinterpret_cast<uint2*>(p.out + bh * D + lane * V) = make_uint2(y[0], y[1]);
+  else *reinterpret_cast<uint32_t*>(p.out + bh * D + lane * V) = y[0];
 }
 
 // With `beside` the kernel follows the requests' own-token kernel, whose
@@ -671,7 +684,7 @@ static int launch_prefix_bits(const PrefixParams& p, int bits, unsigned grid, cu
 }
 
 // Most splits that a prefix can get (one pair of tiles in all; a split has a
-// block of keys at least): the partials' room.
+// block of keys at least).
 static int prefix_splits(int64_t B, int64_t Hkv, int64_t Ng, int64_t max_prefix) {
   if (Ng <= 0 || max_prefix <= 0 || B <= 0) return 0;
   const int64_t blocks = (max_prefix + PX_BN - 1) / PX_BN, want = PX_SMS / Hkv > 1 ? PX_SMS / Hkv : 1;
@@ -687,6 +700,21 @@ static int own_splits(int64_t B, int64_t Hkv, int64_t max_own) {
   return int(n < 64 ? n : 64);
 }
 
+// CTAs of the prefix kernel, each with room for the partials of its two tiles:
+// a partial pair of tiles per group at most, and more splits than one only
+// while they fit the SMs.
+static int64_t prefix_ctas(int64_t B, int64_t G, int64_t Hkv, int64_t Ng, int64_t max_prefix) {
+  if (prefix_splits(B, Hkv, Ng, max_prefix) == 0) return 0;
+  const int64_t n = (B / (2 * (128 / G)) + Ng) * Hkv;
+  return n > PX_SMS ? n : PX_SMS;
+}
+
+// Floats of the partials: prefix, own tokens.
+static int64_t partial_floats(int64_t B, int64_t Hq, int64_t Hkv, int64_t D, int64_t Ng, int64_t max_prefix,
+                              int64_t max_own) {
+  return (prefix_ctas(B, Hq / Hkv, Hkv, Ng, max_prefix) * 256 + B * Hq * own_splits(B, Hkv, max_own)) * (D + 2);
+}
+
 B2F_DEFINE_WAIT_CONTROLS(prefix_attn)
 
 }  // namespace b2f
@@ -698,8 +726,7 @@ extern "C" {
 int64_t b2f_shared_prefix_attn_workspace_bytes(int64_t B, int64_t Hq, int64_t Hkv, int64_t D, int64_t n_groups,
                                                int64_t max_prefix, int64_t max_own) {
   if (B <= 0 || Hq <= 0 || Hkv <= 0 || D <= 0 || Hq / Hkv > 16) return 0;
-  const int64_t n = prefix_splits(B, Hkv, n_groups, max_prefix) + own_splits(B, Hkv, max_own);
-  return B * Hq * n * (D + 2) * int64_t(sizeof(float));
+  return partial_floats(B, Hq, Hkv, D, n_groups, max_prefix, max_own) * int64_t(sizeof(float));
 }
 
 int b2f_shared_prefix_attn(const void* q, const uint8_t* k_pages, const float* k_scales, const uint8_t* v_pages,
@@ -727,38 +754,39 @@ int b2f_shared_prefix_attn(const void* q, const uint8_t* k_pages, const float* k
   const int64_t G = Hq / Hkv, tpt = 128 / G;
   if (max_prefix > prefix_pages * page_size) max_prefix = prefix_pages * page_size;
   if (max_own > max_pages * page_size) max_own = max_pages * page_size;
-  const int np = prefix_splits(B, Hkv, n_groups, max_prefix), no = own_splits(B, Hkv, max_own), n = np + no;
-  if (n > 0) {
-    if (!workspace || workspace_bytes < B * Hq * n * (D + 2) * int64_t(sizeof(float))) return B2F_ERR_WORKSPACE;
+  const int np = prefix_splits(B, Hkv, n_groups, max_prefix), no = own_splits(B, Hkv, max_own);
+  const int64_t ctas = prefix_ctas(B, G, Hkv, n_groups, max_prefix);
+  if (ctas > 0x7fffffff) return B2F_ERR_UNSUPPORTED;
+  if (np + no > 0) {
+    if (!workspace || workspace_bytes < partial_floats(B, Hq, Hkv, D, n_groups, max_prefix, max_own) * 4)
+      return B2F_ERR_WORKSPACE;
     if (!aligned(workspace, 16)) return B2F_ERR_ALIGN;
   }
-  float* o_part = static_cast<float*>(workspace);
-  float* ml_part = o_part + B * Hq * n * D;
+  float* o_prefix = static_cast<float*>(workspace);
+  float* o_own = o_prefix + ctas * 256 * D;
+  float* ml_prefix = o_own + B * Hq * no * D;
+  float* ml_own = ml_prefix + ctas * 256 * 2;
   const __nv_bfloat16* qb = static_cast<const __nv_bfloat16*>(q);
   cudaStream_t st = as_stream(stream);
   int rc;
   if (no > 0) {
     rc = launch_own_partials(qb, k_pages, k_scales, v_pages, v_scales, block_table, max_pages, seq_lens, int(B), int(Hq),
-                             int(Hkv), int(D), int(page_size), bits, softmax_scale, no, int(max_own), o_part, ml_part, n,
-                             np, st);
+                             int(Hkv), int(D), int(page_size), bits, softmax_scale, no, int(max_own), o_own, ml_own, st);
     if (rc != B2F_OK) return rc;
   }
   if (np > 0) {
-    // pairs of tiles: at most one partial pair per group; more splits than one only while they fit the SMs
-    const int64_t pairs = (B / (2 * tpt) + n_groups) * Hkv, grid = pairs > PX_SMS ? pairs : PX_SMS;
-    if (grid > 0x7fffffff) return B2F_ERR_UNSUPPORTED;
     const float s2 = fabsf(softmax_scale) * kLog2e;
     PrefixParams p{qb, k_pages, v_pages, k_scales, v_scales, prefix_table, prefix_lens, group_offsets, prefix_pages,
-                   o_part, ml_part, s2 > 1e-30f ? s2 : 1e-30f, softmax_scale < 0.f, int(B), int(n_groups), int(Hq),
-                   int(Hkv), int(G), int(page_size), int(tpt), np, n, int(max_prefix), no > 0};
-    rc = D == 64 ? launch_prefix_bits<64>(p, bits, unsigned(grid), st)
-                 : launch_prefix_bits<128>(p, bits, unsigned(grid), st);
+                   o_prefix, ml_prefix, s2 > 1e-30f ? s2 : 1e-30f, softmax_scale < 0.f, int(B), int(n_groups), int(Hq),
+                   int(Hkv), int(G), int(page_size), int(tpt), np, int(max_prefix), no > 0};
+    rc = D == 64 ? launch_prefix_bits<64>(p, bits, unsigned(ctas), st)
+                 : launch_prefix_bits<128>(p, bits, unsigned(ctas), st);
     if (rc != B2F_OK) return rc;
   }
-  __nv_bfloat16* ob = static_cast<__nv_bfloat16*>(out);
-  const int Ng = np > 0 ? int(n_groups) : 0;
-  return D == 64 ? launch_combine<64>(o_part, ml_part, group_offsets, Ng, B, int(Hq), int(Hkv), int(2 * tpt), np, n, ob, st)
-                 : launch_combine<128>(o_part, ml_part, group_offsets, Ng, B, int(Hq), int(Hkv), int(2 * tpt), np, n, ob, st);
+  const CombineParams c{o_prefix, ml_prefix, o_own, ml_own, group_offsets, static_cast<__nv_bfloat16*>(out),
+                        np > 0 ? int(n_groups) : 0, int(B), int(Hq), int(Hkv), int(tpt), np, no};
+  return launch_kernel(D == 64 ? prefix_combine_kernel<64> : prefix_combine_kernel<128>,
+                       dim3{unsigned((B * Hq + 7) / 8)}, dim3{256}, 0, st, c);
 }
 
 }  // extern "C"

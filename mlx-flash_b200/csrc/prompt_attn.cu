@@ -166,6 +166,7 @@ __global__ void __launch_bounds__(PA_THREADS, 1) prompt_attn_kernel(const Prompt
     // ============================ items and TMA loads ===========================
     const int span = 2 * p.tpt;
     int cta = blockIdx.x, asks = 0, items = 0, it = 0, mends = 0, loads = 0;
+    int b_from = 0, pairs_before = 0;  // sequences looked through, their pairs: CTAs are taken over in rising order
     bool ok = true;
     // hands `x` to the other warps
     auto publish = [&](const PromptItem& x) {
@@ -192,9 +193,10 @@ __global__ void __launch_bounds__(PA_THREADS, 1) prompt_attn_kernel(const Prompt
       }
       // ---- the item of `cta`; sequence B: the rows past the last sequence ----
       PromptItem x{0, 0, 0, cta % p.Hkv, 0, 0, 0, 0};
-      int left = cta / p.Hkv;
-      for (int b0 = 0; b0 <= p.B; b0 += 32) {
-        const int b = b0 + lane;
+      const int want = cta / p.Hkv;  // pair of tiles, over all sequences
+      if (want < pairs_before) b_from = pairs_before = 0;
+      for (; b_from <= p.B; b_from += 32) {
+        const int b = b_from + lane;
         int lo = 0, hi = 0;
         if (b <= p.B) {
           lo = min(max(p.cu[b], 0), p.T);
@@ -207,16 +209,16 @@ __global__ void __launch_bounds__(PA_THREADS, 1) prompt_attn_kernel(const Prompt
           const int a = __shfl_up_sync(0xffffffffu, s, o);
           if (lane >= o) s += a;
         }
-        const unsigned hit = __ballot_sync(0xffffffffu, s > left);
+        const unsigned hit = __ballot_sync(0xffffffffu, s > want - pairs_before);
         if (hit) {
           const int w = __ffs(hit) - 1;
           x.row0 = __shfl_sync(0xffffffffu, lo, w);
-          x.len = __shfl_sync(0xffffffffu, b0 + w < p.B ? hi - lo : lo - hi, w);  // negative: rows of no sequence
+          x.len = __shfl_sync(0xffffffffu, b_from + w < p.B ? hi - lo : lo - hi, w);  // negative: rows of no sequence
           // the longest rows of a sequence first: they set the tail of the grid
-          x.tok0 = (__shfl_sync(0xffffffffu, s, w) - 1 - left) * span;
+          x.tok0 = (__shfl_sync(0xffffffffu, s, w) - 1 - (want - pairs_before)) * span;
           break;
         }
-        left -= __shfl_sync(0xffffffffu, s, 31);
+        pairs_before += __shfl_sync(0xffffffffu, s, 31);
       }
       if (x.len > 0) x.plan(p);
       if (x.len != 0) publish(x);  // 0: a spare CTA of the grid

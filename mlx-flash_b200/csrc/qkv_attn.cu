@@ -38,9 +38,7 @@ struct AttnParams {
   __nv_bfloat16* out;
   int ring_bytes;  // ring path: shared-memory bytes of the page ring (the merge area follows)
   int slot_bytes;  // ring path: bytes of one ring slot
-  // PART kernels only: where the partials of this call's splits go, the
-  // longest sequence read
-  int part_stride, part_base, max_len;
+  int max_len;     // PART kernels: the longest sequence read
 };
 
 // The kernels' PART form writes partials for a combine with other splits of
@@ -568,7 +566,7 @@ __global__ void __launch_bounds__(RING ? 160 : 128) qkv_decode_attn_kernel(const
     }
     const int64_t bh = int64_t(b) * p.Hq + hq0 + head;
     if constexpr (PART) {
-      const int64_t part = bh * p.part_stride + p.part_base + split;
+      const int64_t part = bh * p.n_splits + split;
       p.o_part[part * D + d] = o / vn;
       if (d == 0) {
         p.ml_part[part * 2 + 0] = mstar;
@@ -968,7 +966,7 @@ __global__ void __launch_bounds__(160, 2) qkv_decode_attn_t8_kernel(const AttnPa
       }
       const int64_t bh = int64_t(b) * p.Hq + hq0 + head;
       if constexpr (PART) {
-        const int64_t part = bh * p.part_stride + p.part_base + int(blockIdx.x);
+        const int64_t part = bh * p.n_splits + int(blockIdx.x);
         p.o_part[part * D + d] = o / vn;
         if (d == 0) {
           p.ml_part[part * 2 + 0] = mstar;
@@ -1078,12 +1076,12 @@ static int launch_part_bits(const AttnParams& p, int bits, cudaStream_t st) {
   return launch_attn<2, D, true>(p, st);
 }
 
-// Decode attention over head-major pages as partials of splits part_base ..
-// part_base + n_splits - 1 of part_stride (prefix_attn.cu joins them).
+// Decode attention over head-major pages as partials, one of n_splits splits
+// too (prefix_attn.cu joins them with those of the prefix).
 int launch_own_partials(const __nv_bfloat16* q, const uint8_t* kc, const float* ks, const uint8_t* vc, const float* vs,
                         const int32_t* table, int64_t width, const int32_t* lens, int B, int Hq, int Hkv, int D, int P,
                         int bits, float scale, int n_splits, int max_len, float* o_part, float* ml_part,
-                        int part_stride, int part_base, cudaStream_t st) {
+                        cudaStream_t st) {
   AttnParams p{};
   p.q = q;
   p.kp = kc;
@@ -1104,8 +1102,6 @@ int launch_own_partials(const __nv_bfloat16* q, const uint8_t* kc, const float* 
   p.qscale = scale * 1.4426950408889634f;
   p.o_part = o_part;
   p.ml_part = ml_part;
-  p.part_stride = part_stride;
-  p.part_base = part_base;
   p.max_len = max_len;
   return D == 64 ? launch_part_bits<64>(p, bits, st) : launch_part_bits<128>(p, bits, st);
 }
