@@ -13,7 +13,7 @@
 //   3. combine: out = sum 2^(m_s - m) O_s / sum 2^(m_s - m) l_s over splits.
 //
 // fp16 operands: a code is exact in 11 bits, and scale * code costs one
-// rounding of 2^-12, where bf16 would cost 2^-9 on K, V and P each -- more than
+// rounding of 2^-11, where bf16 would cost 2^-8 on K, V and P each -- more than
 // the output's own rounding.  fp16's range is made up for by powers of two,
 // which are exact: each query row is scaled by its own absmax, K and V by the
 // largest scale of the CTA's first block (2^14 up to saturation, 2^14 down to
@@ -777,7 +777,7 @@ int b2f_shared_prefix_attn(const void* q, const uint8_t* k_pages, const float* k
   if (np > 0) {
     const float s2 = fabsf(softmax_scale) * kLog2e;
     PrefixParams p{qb, k_pages, v_pages, k_scales, v_scales, prefix_table, prefix_lens, group_offsets, prefix_pages,
-                   o_prefix, ml_prefix, s2 > 1e-30f ? s2 : 1e-30f, softmax_scale < 0.f, int(B), int(n_groups), int(Hq),
+                   o_prefix, ml_prefix, s2 <= 1e-30f ? 1e-30f : s2, softmax_scale < 0.f, int(B), int(n_groups), int(Hq),
                    int(Hkv), int(G), int(page_size), int(tpt), np, int(max_prefix), no > 0};
     rc = D == 64 ? launch_prefix_bits<64>(p, bits, unsigned(ctas), st)
                  : launch_prefix_bits<128>(p, bits, unsigned(ctas), st);

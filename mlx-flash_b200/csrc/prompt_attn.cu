@@ -12,12 +12,15 @@
 //   O += P V         tcgen05.mma with P read from TMEM, V as it lies (MN-major)
 // Softmax in base 2, m and l and O in float32; P is rounded to the inputs'
 // type because the tensor core takes both operands alike (its relative error
-// is that of the output's own rounding).  m is a reference, not the exact
-// maximum: it moves, and O is rescaled, only where a row's new maximum passes
-// it by more than 8 (P stays below 2^8), which after the first blocks is rare.
-// So a row's two threads have to agree on one bit per block (a reduction in
-// the barrier that keeps P off the scores still being read; each leaves its
-// maximum for the other before it), and the rescale needs no warps of its own.
+// is that of the output's own rounding).  m moves, and O is rescaled, only
+// where a row's new maximum passes it by more than 8 (P stays below 2^8),
+// which after the first blocks is rare.  So a row's two threads have to agree
+// on one bit per block (a reduction in the barrier that keeps P off the scores
+// still being read; each leaves half of its maximum for the other before it),
+// and the rescale needs no warps of its own.  Where m moves it is the exact
+// maximum: the largest P of a row of up to 128 keys is 1, which 16 bits hold
+// (m rounded to 8 bits costs such rows 1.5 to 2.3 times the error of the
+// output's rounding, against 1.1 to 1.2, and a row of one key is not its V).
 //
 // Warps: 0-7 softmax of tile 0, 8-15 of tile 1 (also the epilogue), 16 issues
 // the MMAs, 17 plans the items and issues the TMA loads, 18-19 mend value
@@ -83,7 +86,7 @@ struct PromptSmem {
   uint8_t q[2][TILE];
   uint8_t ring[STAGES][TILE];  // K_0 V_0 K_1 V_1 ...
   union {                      // between the two threads of a row
-    __nv_bfloat16 top[2][2][128];
+    uint16_t top[2][2][128];
     float sum[2][128];
   } exchange;
   int quit[2][2];              // per tile and parity of the block: a wait gave up
@@ -511,17 +514,20 @@ __global__ void __launch_bounds__(PA_THREADS, 1) prompt_attn_kernel(const Prompt
         }
         const float top = row_max(s) * p.scale2;
         // every score of the tile has been read past this barrier, and what a
-        // thread leaves before it can be read by the others: its maximum (to 8
-        // bits: both take the same value, a reference need not be exact)
-        const __nv_bfloat16 top8 = __float2bfloat16_rn(top);
-        sm.exchange.top[i][h][r] = top8;
+        // thread leaves before it can be read by the others: the upper half of
+        // its maximum's bits
+        sm.exchange.top[i][h][r] = uint16_t(__float_as_uint(top) >> 16);
         if (!ok) sm.quit[i][j & 1] = 1;
         if (bar_or(bar, 256, !ok || j == 0 || top > m + 8.f)) {
           if (*const_cast<volatile int*>(&sm.quit[i][j & 1])) {
             quit = true;
             break;
           }
-          const float both = fmaxf(__bfloat162float(top8), __bfloat162float(sm.exchange.top[i][1 - h][r]));
+          const uint32_t upper = sm.exchange.top[i][1 - h][r];
+          bar_all(bar, 256);
+          sm.exchange.top[i][h][r] = uint16_t(__float_as_uint(top));  // then the lower half
+          bar_all(bar, 256);
+          const float both = fmaxf(top, __uint_as_float(upper << 16 | sm.exchange.top[i][1 - h][r]));
           const bool move = j == 0 || both > m + 8.f;
           if (j > 0) {
             // O holds blocks up to j - 1 once their product is done
@@ -698,7 +704,7 @@ extern "C" int b2f_prompt_attn(const void* q, int64_t q_row, int64_t q_head, con
       (rc = make_rows_map(&mo, out, bf16, D, G, Hkv, T, D, Hq * D, int(G), int(tpt))) != B2F_OK)
     return rc;
   const float s2 = fabsf(softmax_scale) * kLog2e;
-  PromptParams p{cu_seqlens, out, lse, s2 > 1e-30f ? s2 : 1e-30f, softmax_scale < 0.f, int(B), int(T), int(Hq),
+  PromptParams p{cu_seqlens, out, lse, s2 <= 1e-30f ? 1e-30f : s2, softmax_scale < 0.f, int(B), int(T), int(Hq),
                  int(Hkv), int(G), int(D), causal != 0, int(tpt)};
   cudaStream_t st = as_stream(stream);
   const unsigned n = unsigned(items);

@@ -302,6 +302,53 @@ def test_prompt_attention_later_tokens_do_not_leak(dev, bad):
     assert not bool(dirty[at + 60:].isfinite().any())
 
 
+@pytest.mark.parametrize("dt", ["bf16", "f16"])
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("n", [1, 2, 3, 5, 9, 40])
+def test_prompt_attention_few_keys(dev, n, causal, dt):
+    """Rows of one key are that key's values; short sequences lose no more than two roundings do."""
+    from b200flash.paged_prompt import prompt_attention
+
+    lens = [n] * 60
+    q, k, v, cu = packed(dev, lens, 16, 4, 128, dt, seed=n)
+    out = prompt_attention(q, k, v, cu, causal=causal)
+    got, want = [], []
+    for b in range(60):
+        s = slice(b * n, (b + 1) * n)
+        if causal or n == 1:
+            assert torch.equal(out[b * n], v[b * n].repeat_interleave(4, 0))
+        want.append(attend_reference(q[s], k[s], v[s], causal, 128 ** -0.5)[0])
+        got.append(out[s].double())
+    got, want = torch.cat(got), torch.cat(want)
+    # the output's rounding, and as much again (independent of it) from the rounding of P
+    one = (want.to(DT[dt]).double() - want).norm()
+    assert float((got - want).norm()) <= 1.45 * float(one)
+
+
+@pytest.mark.parametrize("scale", [-0.07, 0.0, 1e-12])
+def test_prompt_attention_scales(dev, scale):
+    from b200flash.paged_prompt import prompt_attention
+
+    lens = [140, 1, 300]
+    q, k, v, cu = packed(dev, lens, 8, 2, 128, "bf16", seed=8, pad=3)
+    out, lse = prompt_attention(q, k, v, cu, softmax_scale=scale, return_lse=True)
+    check_prompt(out, lse, q, k, v, lens, True, scale)
+
+
+@pytest.mark.parametrize("seed", [0, 1])
+def test_prompt_attention_many_sequences(dev, seed):
+    """Several hundred sequences, runs of empty ones among them (more than the planner looks at in one go)."""
+    from b200flash.paged_prompt import prompt_attention
+
+    g = torch.Generator().manual_seed(seed)
+    lens = (torch.randint(0, 30, (400,), generator=g) * (torch.rand(400, generator=g) < 0.5)).tolist()
+    lens[100:180] = [0] * 80
+    lens[250], lens[399] = 500, 0
+    q, k, v, cu = packed(dev, lens, 8, 4, 64, "bf16", seed=seed, pad=300)
+    out, lse = prompt_attention(q, k, v, cu, return_lse=True)
+    check_prompt(out, lse, q, k, v, lens, True)
+
+
 # ---- shared prefixes -----------------------------------------------------------------
 
 
@@ -399,6 +446,44 @@ def test_shared_prefix_attention(dev, off, pre, own, Hq, Hkv, D, bits, page, tig
 def test_shared_prefix_attention_ranges(dev, qscale, kscale, vscale):
     """Queries, keys and values far from 1 (beyond what 16-bit floats of five exponent bits hold)."""
     run_prefix(dev, [0, 3], [400], [0, 30, 100], 8, 2, 128, 8, 64, seed=9, qscale=qscale, kscale=kscale, vscale=vscale)
+
+
+def test_shared_prefix_attention_many_groups(dev):
+    """More groups than a warp looks at in one go, empty ones and empty prefixes among them."""
+    off, own = [0], []
+    for i in range(75):
+        n = (i * 7) % 4
+        own += [(i * 13 + j * 5) % 40 for j in range(n)]
+        off.append(off[-1] + n)
+    run_prefix(dev, off, [(i * 37) % 300 for i in range(75)], own, 8, 2, 64, 8, 16, seed=3)
+
+
+@pytest.mark.parametrize("n,Hq,Hkv,pre", [(300, 8, 1, [90]), (260, 16, 4, [513]), (1, 16, 1, [2000]), (9, 14, 2, [64])])
+def test_shared_prefix_attention_rows(dev, n, Hq, Hkv, pre):
+    """Groups of many tiles of rows, and of up to 16 heads to a KV head."""
+    run_prefix(dev, [0, n], pre, [i % 3 for i in range(n)], Hq, Hkv, 128, 8, 16, seed=4)
+
+
+@pytest.mark.parametrize("scale", [-0.07, 0.0])
+def test_shared_prefix_scales(dev, scale):
+    """A negative scale turns every query about; at 0 every token weighs the same."""
+    from b200flash.paged_prompt import shared_prefix_attention
+
+    g = torch.Generator(device=dev).manual_seed(6)
+    kc, ks, table, _ = paged_rows(dev, [200, 40, 7], 2, 128, 8, 16, g)
+    vc, vs, _, _ = paged_rows(dev, [200, 40, 7], 2, 128, 8, 16, g)
+    q = torch.randn(2, 8, 128, device=dev, generator=g).to(torch.bfloat16)
+    i32 = dict(dtype=torch.int32, device=dev)
+
+    def run(q, scale):
+        return shared_prefix_attention(q, kc, ks, vc, vs, table[:1].contiguous(), torch.tensor([200], **i32),
+                                       torch.tensor([0, 2], **i32), table[1:].contiguous(),
+                                       torch.tensor([40, 7], **i32), 8, 16, 2, softmax_scale=scale)
+
+    got = run(q, scale)
+    want = run(-q, -scale) if scale else run(torch.zeros_like(q), 0.1)
+    # the own tokens' kernel rounds its scaled query to 16 bits on either side
+    within(got, want, 2.0 ** -7 * want.double().abs() + 2.0 ** -7)
 
 
 def test_shared_prefix_matches_decode_attention(dev):
