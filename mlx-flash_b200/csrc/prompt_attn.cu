@@ -85,16 +85,16 @@ struct PromptSmem {
   static constexpr int STAGES = DP == 128 ? 5 : 8;
   uint8_t q[2][TILE];
   uint8_t ring[STAGES][TILE];  // K_0 V_0 K_1 V_1 ...
-  union {                      // between the two threads of a row
-    uint16_t top[2][2][128];
-    float sum[2][128];
-  } exchange;
-  int quit[2][2];              // per tile and parity of the block: a wait gave up
+  union {                      // between the two warps of 32 rows
+    uint16_t top[2][32];
+    float sum[32];
+  } exchange[8];
+  int quit[8][2];              // per pair of warps and parity of the block: a wait gave up
   uint32_t bad[2][DP];         // per column: first key that is NaN | +inf | -inf, from the first masked block on
   int any_bad[2];
   PromptItem item[2];
   uint4 next;  // the answer of next_cta_ask
-  uint64_t full[STAGES], empty[STAGES], q_full, q_empty, s_full[2], p_full[4], pv_done[2], v_raw[PA_MEND],
+  uint64_t full[STAGES], empty[STAGES], q_full, q_empty, s_full[2], p_full[2], pv_done[2], v_raw[PA_MEND],
       v_fix[PA_MEND], o_full[2], item_full[2], item_empty[2], asked, drain;
   uint32_t tmem;
   int abort_flag;
@@ -102,6 +102,7 @@ struct PromptSmem {
 
 // Waits with the CTA's abort flag; false once any wait gave up.
 __device__ __forceinline__ bool wait_or_abort(uint64_t* bar, uint32_t parity, volatile int* abort_flag) {
+  if (mbar_try_wait(bar, parity)) return true;
   if (*abort_flag) return false;
   if (mbar_wait_bounded(bar, parity)) return true;
   *abort_flag = 1;
@@ -136,15 +137,14 @@ __global__ void __launch_bounds__(PA_THREADS, 1) prompt_attn_kernel(const Prompt
     mbar_init(&sm.q_empty, 1);
     for (int i = 0; i < 2; ++i) {
       mbar_init(&sm.s_full[i], 1);
-      mbar_init(&sm.p_full[2 * i], 4);
-      mbar_init(&sm.p_full[2 * i + 1], 4);
+      mbar_init(&sm.p_full[i], 8);
       mbar_init(&sm.pv_done[i], 1);
       mbar_init(&sm.o_full[i], 8);
       mbar_init(&sm.item_full[i], 1);
       mbar_init(&sm.item_empty[i], 19);  // the warps but the planner's
       sm.any_bad[i] = 0;
-      sm.quit[i][0] = sm.quit[i][1] = 0;
     }
+    for (int i = 0; i < 16; ++i) sm.quit[i >> 1][i & 1] = 0;
     for (int i = 0; i < PA_MEND; ++i) {
       mbar_init(&sm.v_raw[i], 1);
       mbar_init(&sm.v_fix[i], 2);
@@ -417,27 +417,22 @@ __global__ void __launch_bounds__(PA_THREADS, 1) prompt_attn_kernel(const Prompt
             ok = wait_all(&sm.v_fix[mends % PA_MEND], uint32_t((mends / PA_MEND) & 1));
             ++mends;
           }
-          if (j + 1 < all) ring.next();  // K_{j+1}
-          bool next = false;                 // it has landed
+          if (ok && j + 1 < all) {  // K_{j+1} (before the waits for P, which are what takes time)
+            ring.next();
+            ok = full_of(ring);
+          }
           for (int i = 0; ok && i < 2; ++i) {
             if (j >= nb[i]) continue;
             const uint64_t v = v_desc + uint64_t(rv.s * (TILE >> 4));
-            for (int h = 0; ok && h < 2; ++h) {  // O_i += P_i V_j
-              ok = wait_all(&sm.p_full[2 * i + h], uint32_t(done[i] & 1));
-              if (!ok) break;
-              tc_fence_after();
-#pragma unroll
-              for (int ks = 0; ks < 4; ++ks)
-                tc_mma_ts(one, tmem + 256 + DP * i, tmem + 128 * i + 32 * h + 8 * ks,
-                          v + (4 * h + ks) * (2048 >> 4), id_o, j > 0 || h > 0 || ks > 0);
-            }
+            ok = wait_all(&sm.p_full[i], uint32_t(done[i] & 1));
             if (!ok) break;
+            tc_fence_after();
+#pragma unroll
+            for (int ks = 0; ks < 8; ++ks)  // O_i += P_i V_j
+              tc_mma_ts(one, tmem + 256 + DP * i, tmem + 128 * i + 8 * ks, v + ks * (2048 >> 4), id_o, j > 0 || ks > 0);
             ++done[i];
             tc_commit_by(one, &sm.pv_done[i]);
-            if (j + 1 < nb[i]) {
-              if (!next) ok = next = full_of(ring);
-              if (ok) score(i, ring.s);
-            }
+            if (j + 1 < nb[i]) score(i, ring.s);
           }
           if (!ok) break;
           tc_commit_by(one, &sm.empty[rv.s]);
@@ -454,10 +449,11 @@ __global__ void __launch_bounds__(PA_THREADS, 1) prompt_attn_kernel(const Prompt
     __syncwarp();
   } else {
     // ============================ softmax and epilogue ==========================
-    // Threads of a tile leave its loops together: what a wait that gave up
-    // says goes through the tile's barrier first.
+    // The two warps of 32 rows share a barrier and leave the loops together:
+    // what a wait that gave up says goes through the barrier first.
     const int i = warp >> 3, h = (warp >> 2) & 1, r = tid & 127;  // tile, half of the keys, MMA row
-    const int bar = 1 + i;
+    const int pair = 4 * i + (warp & 3), bar = 1 + pair;
+    auto& exchange = sm.exchange[pair];
     const uint32_t lane_at = uint32_t(32 * (warp & 3)) << 16;
     const uint32_t s_at = tmem + lane_at + 128 * i, o_at = tmem + lane_at + 256 + DP * i + DP / 2 * h;
     auto wait_all = [&](uint64_t* b, uint32_t parity) {
@@ -465,11 +461,11 @@ __global__ void __launch_bounds__(PA_THREADS, 1) prompt_attn_kernel(const Prompt
     };
     // sum over the row's two threads
     auto joined = [&](float v) {
-      if (h) sm.exchange.sum[i][r] = v;
-      bar_all(bar, 256);
-      if (!h) sm.exchange.sum[i][r] = v += sm.exchange.sum[i][r];
-      bar_all(bar, 256);
-      return h ? sm.exchange.sum[i][r] : v;
+      if (h) exchange.sum[lane] = v;
+      bar_all(bar, 64);
+      if (!h) exchange.sum[lane] = v += exchange.sum[lane];
+      bar_all(bar, 64);
+      return h ? exchange.sum[lane] : v;
     };
     const int rt = r / p.G, rh = r - rt * p.G;  // token of the tile, head of the group
     const bool row_of_tile = r < p.tpt * p.G;
@@ -478,7 +474,7 @@ __global__ void __launch_bounds__(PA_THREADS, 1) prompt_attn_kernel(const Prompt
     for (int k = 0;; ++k) {
       const int slot = k & 1;
       bool ok = wait_all(&sm.item_full[slot], uint32_t((k / 2) & 1));
-      if (bar_or(bar, 256, !ok)) break;
+      if (bar_or(bar, 64, !ok)) break;
       const PromptItem x = sm.item[slot];
       if (x.len == PA_STOP) break;
       if (x.len < 0) {
@@ -513,21 +509,21 @@ __global__ void __launch_bounds__(PA_THREADS, 1) prompt_attn_kernel(const Prompt
             if (c > rel) s[c] = 0xFF800000u;
         }
         const float top = row_max(s) * p.scale2;
-        // every score of the tile has been read past this barrier, and what a
-        // thread leaves before it can be read by the others: the upper half of
-        // its maximum's bits
-        sm.exchange.top[i][h][r] = uint16_t(__float_as_uint(top) >> 16);
-        if (!ok) sm.quit[i][j & 1] = 1;
-        if (bar_or(bar, 256, !ok || j == 0 || top > m + 8.f)) {
-          if (*const_cast<volatile int*>(&sm.quit[i][j & 1])) {
+        // every score of the 32 rows has been read past this barrier, and what
+        // a thread leaves before it can be read by the other: the upper half
+        // of its maximum's bits
+        exchange.top[h][lane] = uint16_t(__float_as_uint(top) >> 16);
+        if (!ok) sm.quit[pair][j & 1] = 1;
+        if (bar_or(bar, 64, !ok || j == 0 || top > m + 8.f)) {
+          if (*const_cast<volatile int*>(&sm.quit[pair][j & 1])) {
             quit = true;
             break;
           }
-          const uint32_t upper = sm.exchange.top[i][1 - h][r];
-          bar_all(bar, 256);
-          sm.exchange.top[i][h][r] = uint16_t(__float_as_uint(top));  // then the lower half
-          bar_all(bar, 256);
-          const float both = fmaxf(top, __uint_as_float(upper << 16 | sm.exchange.top[i][1 - h][r]));
+          const uint32_t upper = exchange.top[1 - h][lane];
+          bar_all(bar, 64);
+          exchange.top[h][lane] = uint16_t(__float_as_uint(top));  // then the lower half
+          bar_all(bar, 64);
+          const float both = fmaxf(top, __uint_as_float(upper << 16 | exchange.top[1 - h][lane]));
           const bool move = j == 0 || both > m + 8.f;
           if (j > 0) {
             // O holds blocks up to j - 1 once their product is done
@@ -559,7 +555,7 @@ __global__ void __launch_bounds__(PA_THREADS, 1) prompt_attn_kernel(const Prompt
         tmem_wait_st();
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(&sm.p_full[2 * i + h]);
+        if (lane == 0) mbar_arrive(&sm.p_full[i]);
       }
       if (quit) break;
       if (nb) {
