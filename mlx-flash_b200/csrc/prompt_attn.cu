@@ -83,6 +83,9 @@ template <int DP>
 struct PromptSmem {
   static constexpr int TILE = 128 * DP * 2;  // bytes of a Q tile, of a K or V block
   static constexpr int STAGES = DP == 128 ? 5 : 8;
+  // TMEM columns: scores, P, O.  P lies over the scores where O leaves no other room.
+  static constexpr bool APART = DP == 64;
+  static constexpr int P_AT = APART ? 256 : 0, P_TILE = APART ? 64 : 128, O_AT = APART ? 384 : 256;
   uint8_t q[2][TILE];
   uint8_t ring[STAGES][TILE];  // K_0 V_0 K_1 V_1 ...
   union {                      // between the two warps of 32 rows
@@ -94,7 +97,7 @@ struct PromptSmem {
   int any_bad[2];
   PromptItem item[2];
   uint4 next;  // the answer of next_cta_ask
-  uint64_t full[STAGES], empty[STAGES], q_full, q_empty, s_full[2], p_full[2], pv_done[2], v_raw[PA_MEND],
+  uint64_t full[STAGES], empty[STAGES], q_full, q_empty, s_full[2], s_read[2], p_full[2], pv_done[2], v_raw[PA_MEND],
       v_fix[PA_MEND], o_full[2], item_full[2], item_empty[2], asked, drain;
   uint32_t tmem;
   int abort_flag;
@@ -137,6 +140,7 @@ __global__ void __launch_bounds__(PA_THREADS, 1) prompt_attn_kernel(const Prompt
     mbar_init(&sm.q_empty, 1);
     for (int i = 0; i < 2; ++i) {
       mbar_init(&sm.s_full[i], 1);
+      mbar_init(&sm.s_read[i], 8);
       mbar_init(&sm.p_full[i], 8);
       mbar_init(&sm.pv_done[i], 1);
       mbar_init(&sm.o_full[i], 8);
@@ -170,6 +174,31 @@ __global__ void __launch_bounds__(PA_THREADS, 1) prompt_attn_kernel(const Prompt
     const int span = 2 * p.tpt;
     int cta = blockIdx.x, asks = 0, items = 0, it = 0, mends = 0, loads = 0;
     int b_from = 0, pairs_before = 0;  // sequences looked through, their pairs: CTAs are taken over in rising order
+    // this lane's sequence; sequence B: the rows past the last one
+    int b, lo, hi;
+    auto look = [&](int from) {
+      b = from + lane;
+      lo = hi = 0;
+      if (b <= p.B) {
+        lo = min(max(p.cu[b], 0), p.T);
+        hi = b < p.B ? min(max(p.cu[b + 1], lo), p.T) : p.T;
+      }
+    };
+    look(0);
+    const bool sorted = p.B < 32;
+    if (sorted) {
+      const int key = b < p.B ? hi - lo : -1;
+      int rank = 0, from = 0;
+      for (int o = 0; o < 32; ++o) {
+        const int k = __shfl_sync(0xffffffffu, key, o);
+        rank += k > key || (k == key && o < lane);
+      }
+      for (int o = 0; o < 32; ++o)
+        if (__shfl_sync(0xffffffffu, rank, o) == lane) from = o;
+      b = __shfl_sync(0xffffffffu, b, from);
+      lo = __shfl_sync(0xffffffffu, lo, from);
+      hi = __shfl_sync(0xffffffffu, hi, from);
+    }
     bool ok = true;
     // hands `x` to the other warps
     auto publish = [&](const PromptItem& x) {
@@ -194,17 +223,12 @@ __global__ void __launch_bounds__(PA_THREADS, 1) prompt_attn_kernel(const Prompt
         mbar_arrive_expect_tx(&sm.asked, 16);
         next_cta_ask(&sm.next, &sm.asked);
       }
-      // ---- the item of `cta`; sequence B: the rows past the last sequence ----
+      // ---- the item of `cta` ----
       PromptItem x{0, 0, 0, cta % p.Hkv, 0, 0, 0, 0};
       const int want = cta / p.Hkv;  // pair of tiles, over all sequences
       if (want < pairs_before) b_from = pairs_before = 0;
       for (; b_from <= p.B; b_from += 32) {
-        const int b = b_from + lane;
-        int lo = 0, hi = 0;
-        if (b <= p.B) {
-          lo = min(max(p.cu[b], 0), p.T);
-          hi = b < p.B ? min(max(p.cu[b + 1], lo), p.T) : p.T;
-        }
+        if (!sorted) look(b_from);
         const int n = (hi - lo + span - 1) / span;
         int s = n;
 #pragma unroll
@@ -216,8 +240,8 @@ __global__ void __launch_bounds__(PA_THREADS, 1) prompt_attn_kernel(const Prompt
         if (hit) {
           const int w = __ffs(hit) - 1;
           x.row0 = __shfl_sync(0xffffffffu, lo, w);
-          x.len = __shfl_sync(0xffffffffu, b_from + w < p.B ? hi - lo : lo - hi, w);  // negative: rows of no sequence
-          // the longest rows of a sequence first: they set the tail of the grid
+          x.len = __shfl_sync(0xffffffffu, b < p.B ? hi - lo : lo - hi, w);  // negative: rows of no sequence
+          // the longest sequences, and rows of a sequence, first: they set the tail of the grid
           x.tok0 = (__shfl_sync(0xffffffffu, s, w) - 1 - (want - pairs_before)) * span;
           break;
         }
@@ -411,15 +435,29 @@ __global__ void __launch_bounds__(PA_THREADS, 1) prompt_attn_kernel(const Prompt
         for (int j = 0; ok && j < all; ++j) {
           ring.next();
           const Ring rv = ring;  // V_j
-          if (j < mask) {
-            ok = full_of(rv);
-          } else {
-            ok = wait_all(&sm.v_fix[mends % PA_MEND], uint32_t((mends / PA_MEND) & 1));
-            ++mends;
-          }
-          if (ok && j + 1 < all) {  // K_{j+1} (before the waits for P, which are what takes time)
+          if (j + 1 < all) {  // K_{j+1} (before the waits for P, which are what takes time)
             ring.next();
             ok = full_of(ring);
+          }
+          auto scored = [&]() {  // the scores of the next block are issued
+            if (j + 1 < all) tc_commit_by(one, &sm.empty[ring.s]);
+            if (j + 2 == all) tc_commit_by(one, &sm.q_empty);
+          };
+          if constexpr (SM::APART) {
+            for (int i = 0; ok && i < 2; ++i) {
+              if (j >= nb[i]) continue;
+              ok = wait_all(&sm.s_read[i], uint32_t(done[i] & 1));
+              tc_fence_after();
+              if (ok && j + 1 < nb[i]) score(i, ring.s);
+            }
+            if (!ok) break;
+            scored();
+          }
+          if (j < mask) {
+            ok = ok && full_of(rv);
+          } else {
+            ok = ok && wait_all(&sm.v_fix[mends % PA_MEND], uint32_t((mends / PA_MEND) & 1));
+            ++mends;
           }
           for (int i = 0; ok && i < 2; ++i) {
             if (j >= nb[i]) continue;
@@ -429,15 +467,15 @@ __global__ void __launch_bounds__(PA_THREADS, 1) prompt_attn_kernel(const Prompt
             tc_fence_after();
 #pragma unroll
             for (int ks = 0; ks < 8; ++ks)  // O_i += P_i V_j
-              tc_mma_ts(one, tmem + 256 + DP * i, tmem + 128 * i + 8 * ks, v + ks * (2048 >> 4), id_o, j > 0 || ks > 0);
+              tc_mma_ts(one, tmem + SM::O_AT + DP * i, tmem + SM::P_AT + SM::P_TILE * i + 8 * ks,
+                        v + ks * (2048 >> 4), id_o, j > 0 || ks > 0);
             ++done[i];
             tc_commit_by(one, &sm.pv_done[i]);
-            if (j + 1 < nb[i]) score(i, ring.s);
+            if (!SM::APART && j + 1 < nb[i]) score(i, ring.s);
           }
           if (!ok) break;
           tc_commit_by(one, &sm.empty[rv.s]);
-          if (j + 1 < all) tc_commit_by(one, &sm.empty[ring.s]);
-          if (j + 2 == all) tc_commit_by(one, &sm.q_empty);  // the last scores are issued
+          if (!SM::APART) scored();
         }
         for (int i = 0; i <= (whole & 1) + (whole >> 1); ++i) ring.next();
       }
@@ -455,7 +493,8 @@ __global__ void __launch_bounds__(PA_THREADS, 1) prompt_attn_kernel(const Prompt
     const int pair = 4 * i + (warp & 3), bar = 1 + pair;
     auto& exchange = sm.exchange[pair];
     const uint32_t lane_at = uint32_t(32 * (warp & 3)) << 16;
-    const uint32_t s_at = tmem + lane_at + 128 * i, o_at = tmem + lane_at + 256 + DP * i + DP / 2 * h;
+    const uint32_t s_at = tmem + lane_at + 128 * i + 64 * h, o_at = tmem + lane_at + SM::O_AT + DP * i + DP / 2 * h,
+                   p_at = tmem + lane_at + SM::P_AT + SM::P_TILE * i + 32 * h;
     auto wait_all = [&](uint64_t* b, uint32_t parity) {
       return bool(__all_sync(0xffffffffu, wait_or_abort(b, parity, abort_flag)));
     };
@@ -500,7 +539,12 @@ __global__ void __launch_bounds__(PA_THREADS, 1) prompt_attn_kernel(const Prompt
         ok = ok && wait_all(&sm.s_full[i], uint32_t(done & 1));
         tc_fence_after();
         uint32_t s[64];
-        tmem_ld64(s_at + 64 * h, s);
+        tmem_ld64(s_at, s);
+        if (SM::APART) {  // the next block's scores may come
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&sm.s_read[i]);
+        }
         const bool masked = j >= x.mask;
         if (masked) {
           const int rel = last - j * PA_BN - 64 * h;
@@ -549,7 +593,12 @@ __global__ void __launch_bounds__(PA_THREADS, 1) prompt_attn_kernel(const Prompt
         uint32_t pk[32];
         if (masked) exp_row<BF16, false>(s, p.scale2, ref, sum, pk);  // exact zeros
         else exp_row<BF16, true>(s, p.scale2, ref, sum, pk);
-        tmem_st32(s_at + 32 * h, pk);
+        // P of the block before has been used up
+        if (SM::APART && j > 0) {
+          ok = ok && wait_all(&sm.pv_done[i], uint32_t((done - 1) & 1));
+          tc_fence_after();
+        }
+        tmem_st32(p_at, pk);
         const float2 l2 = f32x2_parts(add_x2(sum[0], sum[1]));
         l += l2.x + l2.y;
         tmem_wait_st();
