@@ -428,10 +428,14 @@ __global__ void __launch_bounds__(PA_THREADS, 1) prompt_attn_kernel(const Prompt
         ok = wait_all(&sm.q_full, uint32_t(loads++ & 1)) && full_of(ring);
         if (!ok) break;
         tc_fence_after();
-        for (int i = 0; i < 2; ++i)
-          if (nb[i]) score(i, ring.s);
-        tc_commit_by(one, &sm.empty[ring.s]);
-        if (all == 1) tc_commit_by(one, &sm.q_empty);
+        const int first = ring.s;  // K_0
+        score(0, first);
+        auto begun = [&]() {
+          if (nb[1]) score(1, first);
+          tc_commit_by(one, &sm.empty[first]);
+          if (all == 1) tc_commit_by(one, &sm.q_empty);
+        };
+        if (!SM::APART) begun();
         for (int j = 0; ok && j < all; ++j) {
           ring.next();
           const Ring rv = ring;  // V_j
@@ -448,6 +452,7 @@ __global__ void __launch_bounds__(PA_THREADS, 1) prompt_attn_kernel(const Prompt
               if (j >= nb[i]) continue;
               ok = wait_all(&sm.s_read[i], uint32_t(done[i] & 1));
               tc_fence_after();
+              if (ok && i == 0 && j == 0) begun();
               if (ok && j + 1 < nb[i]) score(i, ring.s);
             }
             if (!ok) break;
