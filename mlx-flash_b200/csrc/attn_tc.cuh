@@ -209,9 +209,15 @@ __device__ __forceinline__ uint64_t add_x2(uint64_t a, uint64_t b) {
   asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
   return d;
 }
+// maxima that keep NaN
+__device__ __forceinline__ float max2(float a, float b) {
+  float d;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
+  return d;
+}
 __device__ __forceinline__ float max3(float a, float b, float c) {
   float d;
-  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
   return d;
 }
 
@@ -221,13 +227,14 @@ __device__ __forceinline__ float row_max(const uint32_t (&s)[N]) {
 #pragma unroll
   for (int c = 0; c < N; c += 2)
     m[(c >> 1) & 3] = max3(m[(c >> 1) & 3], __uint_as_float(s[c]), __uint_as_float(s[c + 1]));
-  return fmaxf(max3(m[0], m[1], m[2]), m[3]);
+  return max2(max3(m[0], m[1], m[2]), m[3]);
 }
 
 // 2^x for a pair on the FMA pipe, for -126 <= x < 128 (below: 2^-126): with n
 // the nearest integer, 2^x = 2^n p(x - n), p a polynomial fitted to the least
 // relative error on [-1/2, 1/2] (degree 3: 2^-13.7, for bf16 results; degree
-// 4: 2^-18.5, for fp16), n added to the exponent bits.
+// 4: 2^-18.5, for fp16), n added to the exponent bits.  NaN gives 2^-126: a
+// row with one has a reference that is NaN, and its other exponentials are NaN.
 template <bool BF16>
 __device__ __forceinline__ uint64_t exp2_poly_x2(uint64_t x2) {
   const float2 x = f32x2_parts(x2);

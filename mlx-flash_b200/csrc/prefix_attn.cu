@@ -431,7 +431,7 @@ __global__ void __launch_bounds__(PX_THREADS, 1) prefix_attn_kernel(const Prefix
       auto join = [&](float v) {
         if (h) sm.exchange[i][r] = __float2bfloat16_rn(v);
         bar_all(bar, 256);
-        if (!h) sm.exchange[i][r] = __float2bfloat16_rn(fmaxf(v, __bfloat162float(sm.exchange[i][r])));
+        if (!h) sm.exchange[i][r] = __float2bfloat16_rn(max2(v, __bfloat162float(sm.exchange[i][r])));
         bar_all(bar, 256);
         return __bfloat162float(sm.exchange[i][r]);
       };
@@ -475,16 +475,17 @@ __global__ void __launch_bounds__(PX_THREADS, 1) prefix_attn_kernel(const Prefix
         for (int c = 0; c < 64; c += 32) {
           uint32_t s[32];
           scores(c, s);
-          mx = fmaxf(mx, row_max(s));
+          mx = max2(mx, row_max(s));
         }
         mx *= zs;
-        if (bar_or(bar, 256, !ok || j == 0 || mx > m + 8.f)) {
+        if (bar_or(bar, 256, !ok || j == 0 || !(mx <= m + 8.f))) {
           if (bar_or(bar, 256, !ok)) {
             quit = true;
             break;
           }
-          const float both = join(mx);
-          const bool move = j == 0 || both > m + 8.f;
+          float both = join(mx);
+          if (both == INFINITY) both = __int_as_float(0x7fffffff);  // inf - inf
+          const bool move = j == 0 || !(both <= m + 8.f);
           if (j > 0) {
             // O holds blocks up to j - 1 once their product is done
             ok = wait_all(&sm.pv_done[i], uint32_t((j - 1) & 1));

@@ -330,9 +330,11 @@ __global__ void __launch_bounds__(PA_THREADS, 1) prompt_attn_kernel(const Prompt
           if (!ok) break;
           uint8_t* v = sm.ring[(it + 2 * j + 1) % NST];
           const int valid = min(PA_BN, kend - j * PA_BN);
+          // keys up to the item's first token are seen by all its rows
+          const int from = p.causal ? max(0, min(PA_BN, x.tok0 + 1 - j * PA_BN)) : valid, n = PA_BN - from;
           // a line = 64 columns of one key; the two warps take four lines each in turn
-          for (int line = (warp - 18) * 4 + (lane >> 3); line < 128 * (DP / 64); line += 8) {
-            const int key = line & 127, h = line >> 7, c = lane & 7;
+          for (int line = (warp - 18) * 4 + (lane >> 3); line < n * (DP / 64); line += 8) {
+            const int h = line >= n, key = from + line - h * n, c = lane & 7;
             uint4* at = reinterpret_cast<uint4*>(v + h * HALF + key * 128 + ((c ^ (key & 7)) << 4));
             if (key >= valid) {
               *at = make_uint4(0u, 0u, 0u, 0u);
@@ -537,7 +539,8 @@ __global__ void __launch_bounds__(PA_THREADS, 1) prompt_attn_kernel(const Prompt
       const int nb = i ? x.n1 : x.n0;
       const int t = x.tok0 + i * p.tpt + rt;
       const bool live = row_of_tile && t < x.len;
-      const int last = !live ? -1 : p.causal ? t : x.len - 1;  // last key the row sees
+      // last key the row sees (what rows past the sequence hold is not stored)
+      const int last = !row_of_tile ? -1 : p.causal ? t : x.len - 1;
       float m = -INFINITY, l = 0.f;  // m: reference of the exponents (scaled scores)
       bool quit = false;
       for (int j = 0; j < nb; ++j, ++done) {
@@ -550,9 +553,9 @@ __global__ void __launch_bounds__(PA_THREADS, 1) prompt_attn_kernel(const Prompt
           __syncwarp();
           if (lane == 0) mbar_arrive(&sm.s_read[i]);
         }
-        const bool masked = j >= x.mask;
+        const int rel = last - j * PA_BN - 64 * h;
+        const bool masked = j >= x.mask && !__all_sync(0xffffffffu, rel >= 63);
         if (masked) {
-          const int rel = last - j * PA_BN - 64 * h;
 #pragma unroll
           for (int c = 0; c < 64; ++c)
             if (c > rel) s[c] = 0xFF800000u;
@@ -563,7 +566,7 @@ __global__ void __launch_bounds__(PA_THREADS, 1) prompt_attn_kernel(const Prompt
         // of its maximum's bits
         exchange.top[h][lane] = uint16_t(__float_as_uint(top) >> 16);
         if (!ok) sm.quit[pair][j & 1] = 1;
-        if (bar_or(bar, 64, !ok || j == 0 || top > m + 8.f)) {
+        if (bar_or(bar, 64, !ok || j == 0 || !(top <= m + 8.f))) {
           if (*const_cast<volatile int*>(&sm.quit[pair][j & 1])) {
             quit = true;
             break;
@@ -572,8 +575,9 @@ __global__ void __launch_bounds__(PA_THREADS, 1) prompt_attn_kernel(const Prompt
           bar_all(bar, 64);
           exchange.top[h][lane] = uint16_t(__float_as_uint(top));  // then the lower half
           bar_all(bar, 64);
-          const float both = fmaxf(top, __uint_as_float(upper << 16 | exchange.top[1 - h][lane]));
-          const bool move = j == 0 || both > m + 8.f;
+          float both = max2(top, __uint_as_float(upper << 16 | exchange.top[1 - h][lane]));
+          if (both == INFINITY) both = __int_as_float(0x7fffffff);  // inf - inf
+          const bool move = j == 0 || !(both <= m + 8.f);
           if (j > 0) {
             // O holds blocks up to j - 1 once their product is done
             ok = wait_all(&sm.pv_done[i], uint32_t((done - 1) & 1));

@@ -349,6 +349,30 @@ def test_prompt_attention_many_sequences(dev, seed):
     check_prompt(out, lse, q, k, v, lens, True)
 
 
+@pytest.mark.parametrize("dt", ["bf16", "f16"])
+def test_prompt_attention_one_bad_key(dev, dt):
+    """NaN in any one key, wherever it lies in a block, makes the rows that see it NaN; an infinite score is softmax's."""
+    from b200flash.paged_prompt import prompt_attention
+
+    n = 256
+    q, k, v, cu = packed(dev, [n] * 128, 2, 1, 64, dt, seed=2)
+    at = torch.arange(128, device=dev) * (n + 1)  # key i of sequence i
+    bad = k.clone()
+    bad[at] = math.nan
+    assert bool(prompt_attention(q, bad, v, cu, causal=False).isnan().all())
+    k[at] = 0
+    k[at, 0, 0] = math.inf
+    out = prompt_attention(q, k, v, cu, causal=False).view(128, n, 2, 64)
+    up = (q[:, :, 0] > 0).view(128, n, 2)
+    assert bool(out[up].isnan().all())
+    for b in (0, 7, 70, 127):
+        s = slice(b * n, (b + 1) * n)
+        keep = [i for i in range(n) if i != b]
+        want, want_abs, _ = attend_reference(q[s], k[s][keep], v[s][keep], False, 0.125)
+        down = ~up[b] & (q[s][:, :, 0] < 0)
+        within(out[b][down], want[down], HALF_ULP[DT[dt]] * (want.abs() + want_abs)[down] + 1e-6)
+
+
 # ---- shared prefixes -----------------------------------------------------------------
 
 
@@ -462,6 +486,23 @@ def test_shared_prefix_attention_many_groups(dev):
 def test_shared_prefix_attention_rows(dev, n, Hq, Hkv, pre):
     """Groups of many tiles of rows, and of up to 16 heads to a KV head."""
     run_prefix(dev, [0, n], pre, [i % 3 for i in range(n)], Hq, Hkv, 128, 8, 16, seed=4)
+
+
+def test_shared_prefix_one_bad_key(dev):
+    """NaN in one key of the prefix, wherever it lies in a block."""
+    from b200flash.paged_prompt import shared_prefix_attention
+
+    g = torch.Generator(device=dev).manual_seed(7)
+    kc, ks, table, _ = paged_rows(dev, [256], 1, 64, 8, 128, g)
+    vc, vs, _, _ = paged_rows(dev, [256], 1, 64, 8, 128, g)
+    q = torch.randn(2, 4, 64, device=dev, generator=g).to(torch.bfloat16)
+    i32 = dict(dtype=torch.int32, device=dev)
+    for i in range(128):
+        bad = ks.clone()
+        bad[table[0, 1], 0, i] = math.nan
+        out = shared_prefix_attention(q, kc, bad, vc, vs, table, torch.tensor([256], **i32), torch.tensor([0, 2], **i32),
+                                      torch.zeros(2, 1, **i32), torch.zeros(2, **i32), 8, 128, 1)
+        assert bool(out.isnan().all()), i
 
 
 @pytest.mark.parametrize("scale", [-0.07, 0.0])
