@@ -61,7 +61,7 @@ struct PrefixSmem {
   uint8_t raw[PX_RAW][RAW];     // the same blocks as codes
   __nv_bfloat16 exchange[2][128];  // between the two threads of a row
   float largest[2][4];             // scales of the first block (K, V), per decoding warp
-  uint64_t raw_full[PX_RAW], raw_empty[PX_RAW], full[PX_RING], empty[PX_RING], q_full, s_full[2], p_full[4], pv_done[2],
+  uint64_t raw_full[PX_RAW], raw_empty[PX_RAW], full[PX_RING], empty[PX_RING], q_full, s_full[2], p_full[2], pv_done[2],
       drain;
   int item[6];  // group, first request, requests from there, prefix length, KV head, split
   int splits;
@@ -115,6 +115,7 @@ __device__ __forceinline__ int group_pairs(const int32_t* off, int g, int B, int
 }
 
 __device__ __forceinline__ bool px_wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag) {
+  if (mbar_try_wait(bar, parity)) return true;
   if (*abort_flag) return false;
   if (mbar_wait_bounded(bar, parity)) return true;
   *abort_flag = 1;
@@ -198,8 +199,7 @@ __global__ void __launch_bounds__(PX_THREADS, 1) prefix_attn_kernel(const Prefix
     mbar_init(&sm.q_full, 16);
     for (int i = 0; i < 2; ++i) {
       mbar_init(&sm.s_full[i], 1);
-      mbar_init(&sm.p_full[2 * i], 4);
-      mbar_init(&sm.p_full[2 * i + 1], 4);
+      mbar_init(&sm.p_full[i], 8);
       mbar_init(&sm.pv_done[i], 1);
     }
     mbar_init(&sm.drain, 1);
@@ -262,24 +262,21 @@ __global__ void __launch_bounds__(PX_THREADS, 1) prefix_attn_kernel(const Prefix
         ring.next();
         const Ring rv = ring;  // V_j
         ok = full_of(rv);
-        if (j + 1 < n) ring.next();  // K_{j+1}
+        if (ok && j + 1 < n) {  // K_{j+1}
+          ring.next();
+          ok = full_of(ring);
+        }
         for (int t = 0; ok && t < n_tiles; ++t) {
           const uint64_t v = v_desc + uint64_t(rv.s * (TILE >> 4));
-          for (int h = 0; ok && h < 2; ++h) {  // O_t += P_t V_j
-            ok = wait_all(&sm.p_full[2 * t + h], uint32_t(j & 1));
-            if (!ok) break;
-            tc_fence_after();
-#pragma unroll
-            for (int ks = 0; ks < 4; ++ks)
-              tc_mma_ts(one, tmem + 256 + DP * t, tmem + 128 * t + 64 * h + 8 * ks, v + (4 * h + ks) * (2048 >> 4), id_o,
-                        j > 0 || h > 0 || ks > 0);
-          }
+          ok = wait_all(&sm.p_full[t], uint32_t(j & 1));
           if (!ok) break;
+          tc_fence_after();
+#pragma unroll
+          for (int ks = 0; ks < 8; ++ks)  // O_t += P_t V_j
+            tc_mma_ts(one, tmem + 256 + DP * t, tmem + 128 * t + 64 * (ks >> 2) + 8 * (ks & 3), v + ks * (2048 >> 4),
+                      id_o, j > 0 || ks > 0);
           tc_commit_by(one, &sm.pv_done[t]);
-          if (j + 1 < n) {
-            if (t == 0) ok = full_of(ring);
-            if (ok) score(t, ring.s);
-          }
+          if (j + 1 < n) score(t, ring.s);
         }
         if (!ok) break;
         tc_commit_by(one, &sm.empty[rv.s]);
@@ -347,7 +344,7 @@ __global__ void __launch_bounds__(PX_THREADS, 1) prefix_attn_kernel(const Prefix
             if (sc[t * DG + e] < INFINITY) top = fmaxf(top, sc[t * DG + e]);
         top = warp_max<32>(top);
         if (lane == 0) sm.largest[v][warp & 3] = top;
-        bar_all(3 + v, 128);
+        bar_all(9 + v, 128);
         norm = pow2_inverse(fmaxf(fmaxf(sm.largest[v][0], sm.largest[v][1]), fmaxf(sm.largest[v][2], sm.largest[v][3])), -7);
       }
       if (!ok) break;
@@ -397,11 +394,11 @@ __global__ void __launch_bounds__(PX_THREADS, 1) prefix_attn_kernel(const Prefix
     __syncwarp();
   } else {
     // ============================ queries, softmax, partials ====================
-    // Two threads a row, 64 keys (and half the columns of O) each; threads of
-    // a tile leave its loops together: what a wait that gave up says goes
-    // through the tile's barrier first.
+    // Two threads a row, 64 keys (and half the columns of O) each.  The two
+    // warps of 32 rows share a barrier and leave the loops together: what a
+    // wait that gave up says goes through the barrier first.
     const int i = warp >> 3, h = (warp >> 2) & 1, r = tid & 127;  // tile, half of the keys, MMA row
-    const int bar = 1 + i;
+    const int bar = 1 + 4 * i + (warp & 3);
     // MMA row r of tile i: request row0 + i * tpt + r / G, query head hk * G + r % G
     const int req = i * p.tpt + r / p.G;
     const bool live = g >= 0 && r < p.tpt * p.G && req < rows;
@@ -430,9 +427,9 @@ __global__ void __launch_bounds__(PX_THREADS, 1) prefix_attn_kernel(const Prefix
       // a reference need not be exact
       auto join = [&](float v) {
         if (h) sm.exchange[i][r] = __float2bfloat16_rn(v);
-        bar_all(bar, 256);
+        bar_all(bar, 64);
         if (!h) sm.exchange[i][r] = __float2bfloat16_rn(max2(v, __bfloat162float(sm.exchange[i][r])));
-        bar_all(bar, 256);
+        bar_all(bar, 64);
         return __bfloat162float(sm.exchange[i][r]);
       };
       const float qn = pow2_inverse(join(top), 0);
@@ -478,8 +475,8 @@ __global__ void __launch_bounds__(PX_THREADS, 1) prefix_attn_kernel(const Prefix
           mx = max2(mx, row_max(s));
         }
         mx *= zs;
-        if (bar_or(bar, 256, !ok || j == 0 || !(mx <= m + 8.f))) {
-          if (bar_or(bar, 256, !ok)) {
+        if (bar_or(bar, 64, !ok || j == 0 || !(mx <= m + 8.f))) {
+          if (bar_or(bar, 64, !ok)) {
             quit = true;
             break;
           }
@@ -520,7 +517,7 @@ __global__ void __launch_bounds__(PX_THREADS, 1) prefix_attn_kernel(const Prefix
         tmem_wait_st();
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(&sm.p_full[2 * i + h]);
+        if (lane == 0) mbar_arrive(&sm.p_full[i]);
       }
       // ---- the partial: rows of O through shared memory, then one copy each ----
       // (the operands have been used up once both tiles' products are done)
@@ -543,7 +540,7 @@ __global__ void __launch_bounds__(PX_THREADS, 1) prefix_attn_kernel(const Prefix
         }
         fence_proxy_async_smem();
       }
-      bar_all(bar, 256);
+      bar_all(bar, 64);
       if (ok && live && h == 0) {
         bulk_s2g(p.o_part + part * DP, out, DP * 4);
         *reinterpret_cast<float2*>(p.ml_part + part * 2) = make_float2(m, l + *reinterpret_cast<const float*>(out + DP * 4));
