@@ -4,6 +4,8 @@
 // appended to the planned slots in the same pass.
 #include "common.cuh"
 
+#include <type_traits>
+
 namespace b2f {
 
 // ---- page plan --------------------------------------------------------------
@@ -17,7 +19,8 @@ namespace b2f {
 // itself is the cost: every CTA scans the lengths for itself (shared memory,
 // up to kScanRows requests) instead of waiting for a scan kernel.  More
 // requests take the scan in a launch of its own, which leaves both sums in
-// global memory for the fill.
+// global memory for the fill.  Measured: 4.2 us for 3 requests, 6.2 for 509
+// with 200003 tokens (3.3 MB), 11.4 for 2048; by two launches 14.5 for 2049.
 constexpr int kPlanThreads = 256;
 constexpr int kScanRows = 2048;
 
@@ -219,14 +222,12 @@ __device__ __forceinline__ uint2 pack4(const float (&v)[4]) {
 // quantizer; 8 neighbouring lanes hold a group of 64.
 template <typename Tag, int D>
 __device__ __forceinline__ void append_piece(uint4 w, int sub, int64_t row, int bits, uint8_t* codes, float* scales) {
+  using T2 = std::conditional_t<Tag::kBits == 8, __nv_bfloat162, __half2>;
   const float mi = bits == 8 ? 127.f : bits == 4 ? 7.f : 1.f;
   const typename Tag::T* e = reinterpret_cast<const typename Tag::T*>(&w);
-  float v[8], m = 0.f;
-#pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    v[i] = Tag::to_f(e[i]);
-    m = fmaxf(m, fabsf(v[i]));
-  }
+  const T2* e2 = reinterpret_cast<const T2*>(&w);
+  const T2 top = __hmax2(__hmax2(__habs2(e2[0]), __habs2(e2[1])), __hmax2(__habs2(e2[2]), __habs2(e2[3])));
+  float m = fmaxf(fmaxf(Tag::to_f(top.x), Tag::to_f(top.y)), 0.f);
 #pragma unroll
   for (int k = 1; k < 8; k <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, k));
   if (row < 0) return;
@@ -235,28 +236,48 @@ __device__ __forceinline__ void append_piece(uint4 w, int sub, int64_t row, int 
   // round(v / scale) to the rows' type: the product with the reciprocal is
   // within 2 ulp of the quotient, so both round alike unless the product lies
   // within 8 ulp of a midpoint of the type; there, divide.  Then to the nearest
-  // integer (ties to even) by adding 1.5 * 2^23.
+  // integer (ties to even) by adding 1.5 * 2^23, whose low byte is the code
+  // (signed); two values, then four, at a time.
   const float rs = __frcp_rn(scale);
   constexpr uint32_t kLow = (1u << (24 - Tag::kBits)) - 1;  // float bits below the type's last
-  uint32_t c[8];
+  float x[8];
+  uint32_t near = 0xFFFFFFFFu;
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
-    float x = __fmul_rn(v[i], rs);
-    if ((__float_as_uint(x) & kLow) - (kLow / 2 - 7u) <= 0x10u || !isfinite(rs)) x = __fdiv_rn(v[i], scale);
-    x = fminf(fmaxf(Tag::round(x), -mi), mi);
-    c[i] = __float_as_uint(__fadd_rn(x, 12582912.f)) - 0x4B400000u + uint32_t(int(mi));
+    x[i] = __fmul_rn(Tag::to_f(e[i]), rs);
+    near = min(near, (__float_as_uint(x[i]) & kLow) - (kLow / 2 - 7u));
   }
+  if (near <= 0x10u || !isfinite(rs)) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = __fdiv_rn(Tag::to_f(e[i]), scale);
+  }
+  T2 lo, hi;
+  lo.x = lo.y = Tag::from_f(-mi);
+  hi.x = hi.y = Tag::from_f(mi);
+  uint32_t c[8];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    T2 y;
+    y.x = Tag::from_f(x[2 * i]);
+    y.y = Tag::from_f(x[2 * i + 1]);
+    y = __hmin2(__hmax2(y, lo), hi);
+    c[2 * i] = __float_as_uint(__fadd_rn(Tag::to_f(y.x), 12582912.f));
+    c[2 * i + 1] = __float_as_uint(__fadd_rn(Tag::to_f(y.y), 12582912.f));
+  }
+  uint32_t b[2];  // a code a byte
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+    b[i] = (prmt(prmt(c[4 * i], c[4 * i + 1], 0x0040u), prmt(c[4 * i + 2], c[4 * i + 3], 0x0040u), 0x5410u) ^ 0x80808080u) -
+           (128u - uint32_t(mi)) * 0x01010101u;
   if (sub % 8 == 0) scales[row * (D / 64) + sub / 8] = scale;
   uint8_t* dst = codes + row * (D * bits / 8) + sub * bits;
   if (bits == 8) {
-    *reinterpret_cast<uint2*>(dst) = make_uint2(c[0] | c[1] << 8 | c[2] << 16 | c[3] << 24,
-                                                c[4] | c[5] << 8 | c[6] << 16 | c[7] << 24);
+    *reinterpret_cast<uint2*>(dst) = make_uint2(b[0], b[1]);
   } else if (bits == 4) {
-    *reinterpret_cast<uint32_t*>(dst) = (c[0] << 4 | c[1]) | (c[2] << 4 | c[3]) << 8 | (c[4] << 4 | c[5]) << 16 |
-                                        (c[6] << 4 | c[7]) << 24;
+    *reinterpret_cast<uint32_t*>(dst) = prmt(b[0] << 4 | b[0] >> 8, b[1] << 4 | b[1] >> 8, 0x6420u);
   } else {
-    *reinterpret_cast<uint16_t*>(dst) = uint16_t((c[0] << 6 | c[1] << 4 | c[2] << 2 | c[3]) |
-                                                 (c[4] << 6 | c[5] << 4 | c[6] << 2 | c[7]) << 8);
+    *reinterpret_cast<uint16_t*>(dst) =
+        uint16_t(prmt(b[0] << 6 | b[0] >> 4 | b[0] >> 14 | b[0] >> 24, b[1] << 6 | b[1] >> 4 | b[1] >> 14 | b[1] >> 24, 0x0040u));
   }
 }
 
@@ -502,8 +523,10 @@ __global__ void __launch_bounds__(32 * NR_WARPS, NR_CTAS) qk_norm_rope_stream_ke
 
 template <typename Tag, int D, bool APPEND>
 static int launch_norm_rope(const NormRopeParams& p, cudaStream_t st) {
-  // a CTA each up to 4 per SM: measured for 36 heads of 128 at 592 tokens, few F1, stream F2
-  if (p.T <= 4 * 148)
+  // A CTA a token up to 4 per SM, 2 where rows are appended.  Measured for 36
+  // heads of 128, a CTA a token against streamed: 3.4 / 4.9 us at 7 tokens,
+  // 5.6 / 6.5 at 592, 9.4 / 9.1 at 1184; appended, 5.4 / 6.3 us at 296, 9.0 / 7.4 at 592.
+  if (p.T <= (APPEND ? 2 : 4) * 148)
     return launch_kernel(qk_norm_rope_few_kernel<Tag, D, APPEND>, dim3{unsigned(p.T)}, dim3{256}, 0, st, p);
   constexpr auto kern = qk_norm_rope_stream_kernel<Tag, D, APPEND>;
   constexpr int smem = NR_WARPS * NR_STAGES * NR_CHUNK;
