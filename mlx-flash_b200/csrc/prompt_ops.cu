@@ -415,13 +415,20 @@ __global__ void __launch_bounds__(256) qk_norm_rope_few_kernel(const NormRopePar
 // while the warp computes (loads to registers: 4.4 TB/s at 32768 tokens of 40
 // heads).  Each warp has the same number of consecutive runs, and forms the
 // angles once for those of one token.
-constexpr int NR_WARPS = 4, NR_STAGES = 3, NR_CHUNK = 4096;
-constexpr int NR_CTAS = 4;  // per SM: 48 KB of ring each
+// Rows that are appended take more instructions a byte (the quantizer), so
+// more warps with less in flight each: 4 CTAs an SM with 3 runs a warp against
+// 5 with 2 took 29.4 / 27.5 us for 5003 tokens of 36 heads of 128, 93.1 / 89.5
+// for 20000; not appended, 4 x 3 against 6 x 2 took 67.9 / 72.7 us for 20000.
+// 32768 tokens of 40 heads (671 MB) take 115 us, 5.8 TB/s.
+constexpr int NR_WARPS = 4, NR_CHUNK = 4096;
+constexpr int nr_stages(bool append) { return append ? 2 : 3; }
+constexpr int nr_ctas(bool append) { return append ? 5 : 4; }
 
 template <typename Tag, int D, bool APPEND>
-__global__ void __launch_bounds__(32 * NR_WARPS, NR_CTAS) qk_norm_rope_stream_kernel(const NormRopeParams p) {
+__global__ void __launch_bounds__(32 * NR_WARPS, nr_ctas(APPEND)) qk_norm_rope_stream_kernel(const NormRopeParams p) {
   pdl_enter();
   using E = typename Tag::T;
+  constexpr int NR_STAGES = nr_stages(APPEND);
   constexpr int CH = NR_CHUNK / (2 * D), PER = 32 / (D / 8);  // heads of a run, of a warp's turn
   extern __shared__ __align__(128) uint8_t nr_smem[];
   __shared__ uint64_t full[NR_WARPS][NR_STAGES];
@@ -529,10 +536,10 @@ static int launch_norm_rope(const NormRopeParams& p, cudaStream_t st) {
   if (p.T <= (APPEND ? 2 : 4) * 148)
     return launch_kernel(qk_norm_rope_few_kernel<Tag, D, APPEND>, dim3{unsigned(p.T)}, dim3{256}, 0, st, p);
   constexpr auto kern = qk_norm_rope_stream_kernel<Tag, D, APPEND>;
-  constexpr int smem = NR_WARPS * NR_STAGES * NR_CHUNK;
+  constexpr int smem = NR_WARPS * nr_stages(APPEND) * NR_CHUNK;
   const int set = allow_smem<kern>(smem);
   if (set != B2F_OK) return set;
-  const int want = p.T, most = NR_CTAS * 148;
+  const int want = p.T, most = nr_ctas(APPEND) * 148;
   return launch_kernel(kern, dim3{unsigned(want < most ? want : most)}, dim3{32 * NR_WARPS}, smem, st, p);
 }
 
