@@ -8,9 +8,22 @@
 //   1. own tokens: the paged decode kernels of qkv_attn.cu, writing partials.
 //   2. prefix: CTA = (2 tiles of 128 rows, KV head, split of the prefix).
 //      S = Q K^T and O = P V on tcgen05 as in prompt_attn.cu; bulk copies bring
-//      the codes of a block of 128 keys, four warps turn them into fp16 tiles
+//      the codes of a block of 128 keys, eight warps turn them into fp16 tiles
 //      in shared memory.
 //   3. combine: out = sum 2^(m_s - m) O_s / sum 2^(m_s - m) l_s over splits.
+//
+// What bounds it: the prefix kernel's start (plan, page table, first copies and
+// their decoding: 10000 cycles before the first scores), then instructions (16
+// softmax and 8 decoding warps, 2500 cycles a block of two tiles).  It is let
+// onto the SMs as the own tokens' CTAs leave them.  A split costs a start, and
+// its partials are written and read: 8192 keys and 64 rows over 4 KV heads by
+// one CTA an SM against half as many 24 / 32 us, 20001 keys and 128 rows over
+// 8 KV heads 58 / 99 us.
+// Measured (own tokens, prefix, combine; 32 heads of 128): 64 rows behind 8192
+// tokens, up to 512 of their own, 4 KV heads 13.7 / 28.6 / 5.8 us, 44 us in
+// all (29 MB, 8.9 GFLOP); 128 rows in two groups behind 20001 and 16906, up to
+// 2000 of their own, 8 KV heads 74 / 79 / 6 us, 137 us in all (354 MB, 40.5
+// GFLOP); 4 rows behind 500 tokens 5.5 / 10.1 / 3.6 us.
 //
 // fp16 operands: a code is exact in 11 bits, and scale * code costs one
 // rounding of 2^-11, where bf16 would cost 2^-8 on K, V and P each -- more than
@@ -690,7 +703,9 @@ static int prefix_splits(int64_t B, int64_t Hkv, int64_t Ng, int64_t max_prefix)
 }
 
 // Splits of the requests' own tokens: about two CTAs per SM, 256 tokens or
-// more each (measured for the paged decode kernels at batch 1 to 64).
+// more each.  Measured with up to 2000 tokens and 4 KV heads, split against
+// whole: 7.3 / 23.8 us for one row, 11.5 / 23.6 for 16; 128 rows with 8 KV
+// heads, which have CTAs enough, 74 us whole, 81 in splits of 1024, 159 of 256.
 static int own_splits(int64_t B, int64_t Hkv, int64_t max_own) {
   if (max_own <= 0) return 0;
   const int64_t want = 296 / (B * Hkv) > 1 ? 296 / (B * Hkv) : 1, cap = max_own / 256 > 1 ? max_own / 256 : 1;

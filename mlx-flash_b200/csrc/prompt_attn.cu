@@ -8,28 +8,45 @@
 // tokens, not 128 of them, see a diagonal block.  Per block of 128 keys:
 //   S = Q K^T        tcgen05.mma, Q and K in shared memory (TMA, 128B swizzle)
 //   P = 2^(S c - m)  two threads per row, 64 keys each: the scores come out of
-//                    TMEM into registers, P goes back over S as 16 bits
+//                    TMEM into registers, P goes back to TMEM as 16 bits
 //   O += P V         tcgen05.mma with P read from TMEM, V as it lies (MN-major)
 // Softmax in base 2, m and l and O in float32; P is rounded to the inputs'
 // type because the tensor core takes both operands alike (its relative error
 // is that of the output's own rounding).  m moves, and O is rescaled, only
 // where a row's new maximum passes it by more than 8 (P stays below 2^8),
 // which after the first blocks is rare.  So a row's two threads have to agree
-// on one bit per block (a reduction in the barrier that keeps P off the scores
-// still being read; each leaves half of its maximum for the other before it),
-// and the rescale needs no warps of its own.  Where m moves it is the exact
-// maximum: the largest P of a row of up to 128 keys is 1, which 16 bits hold
-// (m rounded to 8 bits costs such rows 1.5 to 2.3 times the error of the
-// output's rounding, against 1.1 to 1.2, and a row of one key is not its V).
+// on one bit per block (a reduction in a barrier of the two warps that share
+// 32 rows; each leaves half of its maximum for the other before it), and the
+// rescale needs no warps of its own.  Where m moves it is the exact maximum:
+// the largest P of a row of up to 128 keys is 1, which 16 bits hold (m rounded
+// to 8 bits costs such rows 1.5 to 2.3 times the error of the output's
+// rounding, against 1.1 to 1.2, and a row of one key is not its V).
 //
 // Warps: 0-7 softmax of tile 0, 8-15 of tile 1 (also the epilogue), 16 issues
 // the MMAs, 17 plans the items and issues the TMA loads, 18-19 mend value
 // tiles (below) and store the output of whole tiles, which the epilogue leaves
 // in a ring stage (rows of a tile written by their threads cost a shared-memory
-// port cycle per 128-byte line: 4500 cycles a tile).  The two tiles alternate on the tensor core: while it works
-// on one, the other's softmax runs.  One thread per row left a warp of each
-// tile on a scheduler, 2400 cycles a block of softmax and 1250 of MMA in a
-// chain (1.17 PFLOP/s at 16384 tokens); two threads shorten the former.
+// port cycle per 128-byte line: 4500 cycles a tile).  The two tiles alternate:
+// while the tensor core works on one, the other's softmax runs.  One thread
+// per row left a warp of each tile on a scheduler, 2400 cycles a block of
+// softmax and 1250 of MMA in a chain (1.17 PFLOP/s at 16384 tokens); two
+// threads shorten the former.
+//
+// What bounds it: a block's chain of softmax (2100 cycles: 1536 of them
+// exponentials when both tiles compute, the rest loads, the barrier, the
+// stores) and MMA (1500), of which the two tiles overlap half; and power when
+// it runs for long.  Heads of up to 64 leave TMEM columns for P beside S: the
+// next scores are then computed under the softmax, and the tensor core is no
+// longer in the chain; there tile 1 begins behind tile 0's first reading of
+// its scores, so that their exponentials take turns (53 -> 49 us).  At 128
+// columns of O per tile P lies over S.  The longest sequences go first where a
+// warp holds them all (up to 31): 4 sequences of up to 1500 tokens, 28 blocks
+// on the busiest SM against 22.
+// Measured (kernel): 32 heads of 128, 4 KV heads, causal: 16384 tokens 1.71 ms,
+// 1.29 PFLOP/s (2.0 ms back to back, where power holds the clock at 1.4 GHz);
+// 16 sequences of 1 to 2047 tokens 185 us, 0.89 PFLOP/s (an item has 6 blocks
+// on average and costs 1.3 more at its ends); 3 of up to 60 tokens 11 us.
+// 16 heads of 64 in full, 4 sequences of 616 to 1500: 48 us, 0.44 PFLOP/s.
 //
 // A CTA (one per SM) takes item after item from the grid by cancelling CTAs
 // that have not been launched; the items' roles overlap: loads and the first

@@ -549,6 +549,34 @@ def test_shared_prefix_matches_decode_attention(dev):
     within(got, want, 2.0 ** -7 * want.double().abs() + 2.0 ** -7)
 
 
+def test_pages_past_32_bits(dev):
+    """Pages whose bytes lie past 4 GiB of the pool: the rows appended there, and the attention over them."""
+    from b200flash.paged_prompt import qk_norm_rope, shared_prefix_attention
+
+    Hq, Hkv, D, page, small, big = 16, 8, 128, 64, 6, 70_000
+    g = torch.Generator(device=dev).manual_seed(8)
+    T = 4 * page - 5
+    qkv = torch.randn(T, (Hq + 2 * Hkv) * D, device=dev, generator=g).to(torch.bfloat16)
+    w = torch.ones(D, dtype=torch.bfloat16, device=dev)
+    pos = torch.arange(T, dtype=torch.int32, device=dev)
+    i32 = dict(dtype=torch.int32, device=dev)
+    got = []
+    for pages in (small, big):
+        codes = [torch.empty(pages, Hkv, page, D, dtype=torch.uint8, device=dev) for _ in range(2)]
+        scales = [torch.empty(pages, Hkv, page, D // 64, dtype=torch.float32, device=dev) for _ in range(2)]
+        ids = pages - 1 - torch.arange(4, **i32)
+        slots = ids.long().repeat_interleave(page)[:T] * page + pos % page
+        q, _, _ = qk_norm_rope(qkv, Hq, Hkv, pos, w, w, cache=(codes[0], scales[0], codes[1], scales[1]), slots=slots)
+        out = shared_prefix_attention(q[-3:], codes[0], scales[0], codes[1], scales[1], ids[None, :3].contiguous(),
+                                      torch.tensor([2 * page + 9], **i32), torch.tensor([0, 2], **i32),
+                                      ids[3:].expand(3, 1).contiguous(), torch.tensor([40, 0, 7], **i32), 8, page, Hkv)
+        rows = [x[ids.long()].transpose(1, 2).flatten(0, 1)[:T].clone() for x in codes + scales]
+        got.append([out] + rows)
+        del codes, scales
+    for a, b in zip(*got):
+        assert torch.equal(a, b)
+
+
 # ---- refusals ------------------------------------------------------------------------
 
 
