@@ -154,6 +154,8 @@ __global__ void __launch_bounds__(PX_THREADS, 1) prefix_attn_kernel(const Prefix
     return;
   }
 
+  // test control: stalled producers issue nothing (read early: it is a chain of latencies from here to the first copy)
+  const bool stall = warp >= PX_COPY && producers_stalled();
   if (warp == 0) {
     const int span = 2 * p.tpt;
     int lo = 0, hi = 0, n = 0;  // this lane's group
@@ -299,24 +301,28 @@ __global__ void __launch_bounds__(PX_THREADS, 1) prefix_attn_kernel(const Prefix
       tc_commit_by(one, &sm.drain);
       mbar_wait_bounded(&sm.drain, 0u, 100000000ull);
       __syncwarp();
-    } else if (warp >= PX_COPY && n > 0 && !producers_stalled()) {  // test control: stalled producers issue nothing
+    } else if (warp >= PX_COPY && n > 0 && !stall) {
       // ============================ copies of codes and scales ==================
       // 16 keys a lane (pages hold a multiple of 16)
       const int v = warp - PX_COPY, part = lane;  // K or V
       const int32_t* pages = p.table + int64_t(g) * p.width;
       const uint8_t* codes = v ? p.vc : p.kc;
       const float* scales = v ? p.vs : p.ks;
-      auto page_of = [&](int j) {
+      // a page is loaded a block ahead, and looked at only where it is used
+      auto entry_of = [&](int j) {
         const int key = (j0 + j) * PX_BN + 16 * part;
-        return part < 8 && j < n && key < len ? max(pages[key / p.P], 0) : -1;
+        return part < 8 && j < n && key < len ? key / p.P : -1;
       };
-      int page = page_of(0), j = 0;
+      int entry = entry_of(0), page = 0, j = 0;
+      if (entry >= 0) page = pages[entry];
       for (; j < n; ++j) {
         const int key = (j0 + j) * PX_BN + 16 * part, it = 2 * j + v, s = it % PX_RAW;
         const int keys = min(PX_BN, (len - (j0 + j) * PX_BN + 15) & ~15);  // of the block, in whole sixteens
-        const int64_t row = (int64_t(page) * p.Hkv + hk) * p.P + key % p.P;
-        const bool have = page >= 0;
-        page = page_of(j + 1);
+        const int next_entry = entry_of(j + 1);
+        int next = 0;
+        if (next_entry >= 0) next = pages[next_entry];
+        const int64_t row = (int64_t(max(page, 0)) * p.Hkv + hk) * p.P + key % p.P;
+        const bool have = entry >= 0;
         if (it >= PX_RAW &&
             !__all_sync(0xffffffffu, px_wait(&sm.raw_empty[s], uint32_t((it / PX_RAW - 1) & 1), abort_flag)))
           break;
@@ -326,6 +332,8 @@ __global__ void __launch_bounds__(PX_THREADS, 1) prefix_attn_kernel(const Prefix
           bulk_g2s(sm.raw[s] + 16 * part * RB, codes + row * RB, 16 * RB, &sm.raw_full[s]);
           bulk_g2s(sm.raw[s] + SM::CODES + 16 * part * DG * 4, scales + row * DG, 16 * DG * 4, &sm.raw_full[s]);
         }
+        entry = next_entry;
+        page = next;
       }
       // the last copy issued lands before the CTA goes away (those before it were waited for)
       if (j > 0) {

@@ -148,6 +148,7 @@ __global__ void __launch_bounds__(PA_THREADS, 1) prompt_attn_kernel(const Prompt
     return;
   }
 
+  const bool stall = warp == 17 && producers_stalled();  // test control: stalled producers issue nothing
   if (tid == 0) {
     for (int s = 0; s < NST; ++s) {
       mbar_init(&sm.full[s], 1);
@@ -268,7 +269,7 @@ __global__ void __launch_bounds__(PA_THREADS, 1) prompt_attn_kernel(const Prompt
       if (x.len != 0) publish(x);  // 0: a spare CTA of the grid
       if (ok && x.len > 0) {
         const int all = x.blocks(), stages = x.stages();
-        if (lane == 0 && !producers_stalled()) {  // test control: stalled producers issue nothing
+        if (lane == 0 && !stall) {
           auto load = [&](int i) {  // K (even i) or V of block i / 2; then the stages of whole tiles
             const int n = it + i, s = n % NST;
             if (n >= NST && !wait_or_abort(&sm.empty[s], uint32_t((n / NST - 1) & 1), abort_flag)) return false;
