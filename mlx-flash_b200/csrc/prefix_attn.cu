@@ -58,9 +58,10 @@ struct PrefixParams {
   const int32_t *table, *lens, *off;
   int64_t width;
   float *o_part, *ml_part;  // [CTA][256 rows][DP], [CTA][256 rows] of (m, l)
+  int* quota;               // how the prefixes are split, for the combine
   float scale2;   // |softmax_scale| * log2(e)
   int negate;     // softmax_scale < 0: the MMA negates Q
-  int B, Ng, Hq, Hkv, G, P, tpt, max_splits, max_prefix;
+  int B, Ng, Hq, Hkv, G, P, tpt, max_prefix;
   int beside;     // launched to run beside the previous kernel (see launch_prefix)
 };
 
@@ -77,7 +78,7 @@ struct PrefixSmem {
   uint64_t raw_full[PX_RAW], raw_empty[PX_RAW], full[PX_RING], empty[PX_RING], q_full, s_full[2], p_full[2], pv_done[2],
       drain;
   int item[6];  // group, first request, requests from there, prefix length, KV head, split
-  int splits;
+  int per;  // blocks a CTA of the group
   uint32_t tmem;
   int abort_flag;
 };
@@ -116,15 +117,64 @@ __device__ __forceinline__ void spread_codes(const uint4& q, uint32_t (&w)[32 / 
   }
 }
 
-// Splits of each prefix: enough for one CTA per SM (a CTA takes the whole SM's
-// shared memory), by how many pairs of tiles the groups make -- which only the
-// device knows.
-__device__ __forceinline__ int splits_for(int pairs, int Hkv, int max_splits) {
-  return max(1, min(max_splits, PX_SMS / max(1, pairs * Hkv)));
-}
-__device__ __forceinline__ int group_pairs(const int32_t* off, int g, int B, int span) {
-  const int lo = min(max(off[g], 0), B), hi = min(max(off[g + 1], lo), B);
-  return (hi - lo + span - 1) / span;
+// The groups as the device finds them: which rows, how many pairs of tiles,
+// how many blocks of keys.
+struct PrefixGroup {
+  int lo, hi, len, pairs, blocks;
+  __device__ __forceinline__ void look(const int32_t* off, const int32_t* lens, int g, int Ng, int B, int span,
+                                       int max_prefix) {
+    lo = hi = len = 0;
+    if (g < Ng) {
+      lo = min(max(off[g], 0), B);
+      hi = min(max(off[g + 1], lo), B);
+      len = min(max(lens[g], 0), max_prefix);
+    }
+    pairs = (hi - lo + span - 1) / span;
+    blocks = pairs ? (len + PX_BN - 1) / PX_BN : 0;
+  }
+  // how a prefix is split: by `quota` blocks a CTA, or (negative) into -quota
+  __device__ __forceinline__ int splits(int quota) const {
+    return quota > 0 ? (blocks + quota - 1) / quota : min(blocks, -quota);
+  }
+};
+
+// How the prefixes are split, by the whole warp: the fewest blocks a CTA (to a
+// 32nd) with which all fit one CTA per SM (a CTA takes the whole SM's shared
+// memory), so that long and short prefixes end together; or all alike, where
+// that gives the longest no more.  Measured, alike against by quota: groups of
+// 8 rows behind 16000, 1000, 500 and 2000 tokens 37 / 19 us, of 64 behind
+// 20001 and 2000 55 / 41, of 60 and 68 behind 20001 and 16906 72 / 76.
+__device__ __forceinline__ int prefix_quota(const int32_t* off, const int32_t* lens, int Ng, int B, int span, int Hkv,
+                                            int max_prefix) {
+  const int lane = threadIdx.x & 31;
+  PrefixGroup own;
+  own.look(off, lens, lane, Ng, B, span, max_prefix);
+  auto over_groups = [&](auto f) {
+    f(own);
+    for (int g = 32 + lane; g < Ng; g += 32) {
+      PrefixGroup x;
+      x.look(off, lens, g, Ng, B, span, max_prefix);
+      f(x);
+    }
+  };
+  float work = 0.f;
+  int most = 1, pairs = 0;
+  over_groups([&](const PrefixGroup& x) {
+    work += float(x.pairs) * float(x.blocks);
+    most = max(most, x.blocks);
+    if (x.blocks) pairs += x.pairs;
+  });
+  most = __reduce_max_sync(0xffffffffu, most);
+  const float even = warp_sum<32>(work) * float(Hkv) / float(PX_SMS);  // blocks a CTA if it came out even
+  int quota = even < float(most) ? max(1, int(ceilf(even))) : most;
+  const int alike = max(1, min(most, PX_SMS / max(1, __reduce_add_sync(0xffffffffu, pairs) * Hkv)));
+  while (quota < (most + alike - 1) / alike) {
+    int ctas = 0;
+    over_groups([&](const PrefixGroup& x) { ctas += x.pairs * x.splits(quota); });
+    if (__reduce_add_sync(0xffffffffu, ctas) * Hkv <= PX_SMS) return quota;
+    quota += max(1, quota / 32);
+  }
+  return -alike;
 }
 
 __device__ __forceinline__ bool px_wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag) {
@@ -158,23 +208,14 @@ __global__ void __launch_bounds__(PX_THREADS, 1) prefix_attn_kernel(const Prefix
   const bool stall = warp >= PX_COPY && producers_stalled();
   if (warp == 0) {
     const int span = 2 * p.tpt;
-    int lo = 0, hi = 0, n = 0;  // this lane's group
-    auto look = [&](int g) {
-      lo = hi = n = 0;
-      if (g >= p.Ng) return;
-      lo = min(max(p.off[g], 0), p.B);
-      hi = min(max(p.off[g + 1], lo), p.B);
-      n = min(max(p.lens[g], 0), p.max_prefix);
-    };
-    look(lane);
-    int pairs = (hi - lo + span - 1) / span;
-    for (int x = 32 + lane; x < p.Ng; x += 32) pairs += group_pairs(p.off, x, p.B, span);
-    const int splits = splits_for(__reduce_add_sync(0xffffffffu, pairs), p.Hkv, p.max_splits);
-    const int split = blockIdx.x % splits, hk = blockIdx.x / splits % p.Hkv;
-    int left = blockIdx.x / splits / p.Hkv, g = -1, row0 = 0, rows = 0, len = 0;
+    const int quota = prefix_quota(p.off, p.lens, p.Ng, p.B, span, p.Hkv, p.max_prefix);
+    if (blockIdx.x == 0 && lane == 0) *p.quota = quota;
+    int left = blockIdx.x, g = -1, row0 = 0, rows = 0, len = 0, hk = 0, split = 0, per = 1;
     for (int g0 = 0; g0 < p.Ng && g < 0; g0 += 32) {
-      if (g0) look(g0 + lane);
-      int s = (hi - lo + span - 1) / span;
+      PrefixGroup x;
+      x.look(p.off, p.lens, g0 + lane, p.Ng, p.B, span, p.max_prefix);
+      const int mine = x.splits(quota), ctas = x.pairs * mine * p.Hkv;
+      int s = ctas;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
         const int a = __shfl_up_sync(0xffffffffu, s, o);
@@ -183,12 +224,14 @@ __global__ void __launch_bounds__(PX_THREADS, 1) prefix_attn_kernel(const Prefix
       const unsigned hit = __ballot_sync(0xffffffffu, s > left);
       if (hit) {
         const int w = __ffs(hit) - 1;
-        const int before = w ? __shfl_sync(0xffffffffu, s, max(w - 1, 0)) : 0;
-        const int a = __shfl_sync(0xffffffffu, lo, w), b = __shfl_sync(0xffffffffu, hi, w);
-        len = __shfl_sync(0xffffffffu, n, w);
+        const int at = left - __shfl_sync(0xffffffffu, s - ctas, w), splits = __shfl_sync(0xffffffffu, mine, w);
+        len = __shfl_sync(0xffffffffu, x.len, w);
         g = g0 + w;
-        row0 = a + (left - before) * span;
-        rows = b - row0;
+        split = at % splits;
+        per = quota > 0 ? quota : ((len + PX_BN - 1) / PX_BN + splits - 1) / splits;
+        hk = at / splits % p.Hkv;
+        row0 = __shfl_sync(0xffffffffu, x.lo, w) + at / splits / p.Hkv * span;
+        rows = __shfl_sync(0xffffffffu, x.hi, w) - row0;
       } else {
         left -= __shfl_sync(0xffffffffu, s, 31);
       }
@@ -200,7 +243,7 @@ __global__ void __launch_bounds__(PX_THREADS, 1) prefix_attn_kernel(const Prefix
       sm.item[3] = len;
       sm.item[4] = hk;
       sm.item[5] = split;
-      sm.splits = splits;
+      sm.per = per;
     }
   } else if (tid == 32) {
     for (int s = 0; s < PX_RAW; ++s) {
@@ -232,10 +275,10 @@ __global__ void __launch_bounds__(PX_THREADS, 1) prefix_attn_kernel(const Prefix
   const int g = __shfl_sync(0xffffffffu, sm.item[0], 0), row0 = __shfl_sync(0xffffffffu, sm.item[1], 0);
   const int rows = __shfl_sync(0xffffffffu, sm.item[2], 0), len = __shfl_sync(0xffffffffu, sm.item[3], 0);
   const int hk = __shfl_sync(0xffffffffu, sm.item[4], 0), split = __shfl_sync(0xffffffffu, sm.item[5], 0);
-  const int splits = __shfl_sync(0xffffffffu, sm.splits, 0);
-  const int blocks = (len + PX_BN - 1) / PX_BN, per = (blocks + splits - 1) / splits;
+  const int per = __shfl_sync(0xffffffffu, sm.per, 0);
+  const int blocks = (len + PX_BN - 1) / PX_BN;
   const int j0 = split * per;
-  const int n = g < 0 ? 0 : min(blocks, j0 + per) - j0;  // this split's blocks (g < 0: a spare CTA of the grid)
+  const int n = g < 0 ? 0 : max(0, min(blocks, j0 + per) - j0);  // this split's blocks (g < 0: a spare CTA of the grid)
   const int n_tiles = rows > p.tpt ? 2 : 1;
 
   if (warp >= PX_MMA) {
@@ -428,7 +471,7 @@ __global__ void __launch_bounds__(PX_THREADS, 1) prefix_attn_kernel(const Prefix
     auto wait_all = [&](uint64_t* b, uint32_t parity) {
       return bool(__all_sync(0xffffffffu, px_wait(b, parity, abort_flag)));
     };
-    if (n <= 0) {  // fewer blocks than splits
+    if (n <= 0) {  // rounding left this split nothing
       if (live && h == 0) *reinterpret_cast<float2*>(p.ml_part + part * 2) = make_float2(-INFINITY, 0.f);
     } else if (i < n_tiles) {
       // ---- this row's query, scaled by a power of two into fp16; a half of its columns each ----
@@ -587,9 +630,10 @@ __global__ void __launch_bounds__(PX_THREADS, 1) prefix_attn_kernel(const Prefix
 struct CombineParams {
   const float *o_prefix, *ml_prefix;  // [CTA][256][D] and (m, l), as prefix_attn_kernel leaves them
   const float *o_own, *ml_own;        // [B * Hq][n_own][D] and (m, l)
-  const int32_t* off;
+  const int* quota;
+  const int32_t *off, *lens;
   __nv_bfloat16* out;
-  int Ng, B, Hq, Hkv, tpt, max_splits, n_own;
+  int Ng, B, Hq, Hkv, tpt, max_prefix, n_own, ctas;
 };
 
 template <int D>
@@ -600,30 +644,34 @@ __global__ void __launch_bounds__(256) prefix_combine_kernel(const CombineParams
   const int lane = threadIdx.x & 31;
   if (bh >= int64_t(p.B) * p.Hq) return;
   const int b = int(bh / p.Hq), h = int(bh - int64_t(b) * p.Hq), G = p.Hq / p.Hkv, span = 2 * p.tpt;
-  // the request's pair of tiles (over all groups) and its place in the group
-  int pairs = 0, pair = -1, rel = 0;
+  // the group's splits, its first CTA, the request's place in it
+  int ctas = 0, sp = 0, rel = 0;
+  const int quota = p.Ng ? *p.quota : 1;
   for (int g0 = 0; g0 < p.Ng; g0 += 32) {
-    const int g = g0 + lane;
-    const int lo = g < p.Ng ? min(max(p.off[g], 0), p.B) : 0, hi = g < p.Ng ? min(max(p.off[g + 1], lo), p.B) : 0;
-    const int n = (hi - lo + span - 1) / span;
-    int s = n;
+    PrefixGroup x;
+    x.look(p.off, p.lens, g0 + lane, p.Ng, p.B, span, p.max_prefix);
+    const int mine = x.splits(quota);
+    int s = x.pairs * mine * p.Hkv;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
       const int a = __shfl_up_sync(0xffffffffu, s, o);
       if (lane >= o) s += a;
     }
-    const unsigned hit = __ballot_sync(0xffffffffu, b >= lo && b < hi);
-    if (hit && pair < 0) {
+    const unsigned hit = __ballot_sync(0xffffffffu, b >= x.lo && b < x.hi);
+    if (hit) {
       const int w = __ffs(hit) - 1;
-      rel = b - __shfl_sync(0xffffffffu, lo, w);
-      pair = pairs + __shfl_sync(0xffffffffu, s - n, w) + rel / span;
+      rel = b - __shfl_sync(0xffffffffu, x.lo, w);
+      sp = __shfl_sync(0xffffffffu, mine, w);
+      ctas += __shfl_sync(0xffffffffu, s - x.pairs * mine * p.Hkv, w);
+      break;
     }
-    pairs += __shfl_sync(0xffffffffu, s, 31);
+    ctas += __shfl_sync(0xffffffffu, s, 31);
   }
-  const int splits = splits_for(pairs, p.Hkv, p.max_splits), sp = pair < 0 ? 0 : splits;
+  const int first = ctas + (rel / span * p.Hkv + h / G) * sp;
+  if (first < 0 || first + sp > p.ctas) sp = 0;  // (group offsets that fall)
   const int count = sp + p.n_own;
   // partial s of the row: the prefix's splits, then the own tokens'
-  const int64_t at = ((int64_t(pair) * p.Hkv + h / G) * splits) * 256 + rel % span / p.tpt * 128 + rel % p.tpt * G + h % G;
+  const int64_t at = int64_t(first) * 256 + rel % span / p.tpt * 128 + rel % p.tpt * G + h % G;
   auto ml_of = [&](int s) {
     return s < sp ? reinterpret_cast<const float2*>(p.ml_prefix)[at + s * 256]
                   : reinterpret_cast<const float2*>(p.ml_own)[bh * p.n_own + s - sp];
@@ -702,14 +750,6 @@ static int launch_prefix_bits(const PrefixParams& p, int bits, unsigned grid, cu
   return launch_prefix<DP, 2>(p, grid, st);
 }
 
-// Most splits that a prefix can get (one pair of tiles in all; a split has a
-// block of keys at least).
-static int prefix_splits(int64_t B, int64_t Hkv, int64_t Ng, int64_t max_prefix) {
-  if (Ng <= 0 || max_prefix <= 0 || B <= 0) return 0;
-  const int64_t blocks = (max_prefix + PX_BN - 1) / PX_BN, want = PX_SMS / Hkv > 1 ? PX_SMS / Hkv : 1;
-  return int(want < blocks ? want : blocks);
-}
-
 // Splits of the requests' own tokens: about two CTAs per SM, 256 tokens or
 // more each.  Measured with up to 2000 tokens and 4 KV heads, split against
 // whole: 7.3 / 23.8 us for one row, 11.5 / 23.6 for 16; 128 rows with 8 KV
@@ -725,15 +765,16 @@ static int own_splits(int64_t B, int64_t Hkv, int64_t max_own) {
 // a partial pair of tiles per group at most, and more splits than one only
 // while they fit the SMs.
 static int64_t prefix_ctas(int64_t B, int64_t G, int64_t Hkv, int64_t Ng, int64_t max_prefix) {
-  if (prefix_splits(B, Hkv, Ng, max_prefix) == 0) return 0;
+  if (Ng <= 0 || max_prefix <= 0 || B <= 0) return 0;
   const int64_t n = (B / (2 * (128 / G)) + Ng) * Hkv;
   return n > PX_SMS ? n : PX_SMS;
 }
 
-// Floats of the partials: prefix, own tokens.
-static int64_t partial_floats(int64_t B, int64_t Hq, int64_t Hkv, int64_t D, int64_t Ng, int64_t max_prefix,
-                              int64_t max_own) {
-  return (prefix_ctas(B, Hq / Hkv, Hkv, Ng, max_prefix) * 256 + B * Hq * own_splits(B, Hkv, max_own)) * (D + 2);
+// Floats of the workspace: the partials of prefix and own tokens, the quota.
+static int64_t workspace_floats(int64_t B, int64_t Hq, int64_t Hkv, int64_t D, int64_t Ng, int64_t max_prefix,
+                                int64_t max_own) {
+  const int64_t rows = prefix_ctas(B, Hq / Hkv, Hkv, Ng, max_prefix) * 256 + B * Hq * own_splits(B, Hkv, max_own);
+  return rows ? rows * (D + 2) + 4 : 0;
 }
 
 B2F_DEFINE_WAIT_CONTROLS(prefix_attn)
@@ -747,7 +788,7 @@ extern "C" {
 int64_t b2f_shared_prefix_attn_workspace_bytes(int64_t B, int64_t Hq, int64_t Hkv, int64_t D, int64_t n_groups,
                                                int64_t max_prefix, int64_t max_own) {
   if (B <= 0 || Hq <= 0 || Hkv <= 0 || D <= 0 || Hq / Hkv > 16) return 0;
-  return partial_floats(B, Hq, Hkv, D, n_groups, max_prefix, max_own) * int64_t(sizeof(float));
+  return workspace_floats(B, Hq, Hkv, D, n_groups, max_prefix, max_own) * int64_t(sizeof(float));
 }
 
 int b2f_shared_prefix_attn(const void* q, const uint8_t* k_pages, const float* k_scales, const uint8_t* v_pages,
@@ -775,11 +816,11 @@ int b2f_shared_prefix_attn(const void* q, const uint8_t* k_pages, const float* k
   const int64_t G = Hq / Hkv, tpt = 128 / G;
   if (max_prefix > prefix_pages * page_size) max_prefix = prefix_pages * page_size;
   if (max_own > max_pages * page_size) max_own = max_pages * page_size;
-  const int np = prefix_splits(B, Hkv, n_groups, max_prefix), no = own_splits(B, Hkv, max_own);
+  const int no = own_splits(B, Hkv, max_own);
   const int64_t ctas = prefix_ctas(B, G, Hkv, n_groups, max_prefix);
   if (ctas > 0x7fffffff) return B2F_ERR_UNSUPPORTED;
-  if (np + no > 0) {
-    if (!workspace || workspace_bytes < partial_floats(B, Hq, Hkv, D, n_groups, max_prefix, max_own) * 4)
+  if (ctas + no > 0) {
+    if (!workspace || workspace_bytes < workspace_floats(B, Hq, Hkv, D, n_groups, max_prefix, max_own) * 4)
       return B2F_ERR_WORKSPACE;
     if (!aligned(workspace, 16)) return B2F_ERR_ALIGN;
   }
@@ -787,6 +828,7 @@ int b2f_shared_prefix_attn(const void* q, const uint8_t* k_pages, const float* k
   float* o_own = o_prefix + ctas * 256 * D;
   float* ml_prefix = o_own + B * Hq * no * D;
   float* ml_own = ml_prefix + ctas * 256 * 2;
+  int* quota = reinterpret_cast<int*>(ml_own + B * Hq * no * 2);
   const __nv_bfloat16* qb = static_cast<const __nv_bfloat16*>(q);
   cudaStream_t st = as_stream(stream);
   int rc;
@@ -795,17 +837,18 @@ int b2f_shared_prefix_attn(const void* q, const uint8_t* k_pages, const float* k
                              int(Hkv), int(D), int(page_size), bits, softmax_scale, no, int(max_own), o_own, ml_own, st);
     if (rc != B2F_OK) return rc;
   }
-  if (np > 0) {
+  if (ctas > 0) {
     const float s2 = fabsf(softmax_scale) * kLog2e;
     PrefixParams p{qb, k_pages, v_pages, k_scales, v_scales, prefix_table, prefix_lens, group_offsets, prefix_pages,
-                   o_prefix, ml_prefix, s2 <= 1e-30f ? 1e-30f : s2, softmax_scale < 0.f, int(B), int(n_groups), int(Hq),
-                   int(Hkv), int(G), int(page_size), int(tpt), np, int(max_prefix), no > 0};
+                   o_prefix, ml_prefix, quota, s2 <= 1e-30f ? 1e-30f : s2, softmax_scale < 0.f, int(B), int(n_groups), int(Hq),
+                   int(Hkv), int(G), int(page_size), int(tpt), int(max_prefix), no > 0};
     rc = D == 64 ? launch_prefix_bits<64>(p, bits, unsigned(ctas), st)
                  : launch_prefix_bits<128>(p, bits, unsigned(ctas), st);
     if (rc != B2F_OK) return rc;
   }
-  const CombineParams c{o_prefix, ml_prefix, o_own, ml_own, group_offsets, static_cast<__nv_bfloat16*>(out),
-                        np > 0 ? int(n_groups) : 0, int(B), int(Hq), int(Hkv), int(tpt), np, no};
+  const CombineParams c{o_prefix, ml_prefix, o_own, ml_own, quota, group_offsets, prefix_lens,
+                        static_cast<__nv_bfloat16*>(out), ctas > 0 ? int(n_groups) : 0, int(B), int(Hq), int(Hkv),
+                        int(tpt), int(max_prefix), no, int(ctas)};
   return launch_kernel(D == 64 ? prefix_combine_kernel<64> : prefix_combine_kernel<128>,
                        dim3{unsigned((B * Hq + 7) / 8)}, dim3{256}, 0, st, c);
 }

@@ -459,6 +459,7 @@ def run_prefix(dev, off, pre, own, Hq, Hkv, D, bits, page, seed=0, qscale=1.5, k
     ([0, 40], [1500], list(range(40)), 16, 2, 128, 8, 64),
     ([0, 70], [300], [i % 7 for i in range(70)], 8, 1, 128, 8, 128),
     ([0, 2], [0], [0, 50], 8, 2, 128, 8, 64),
+    ([0, 3, 40, 41], [5, 3000, 129], [i % 9 for i in range(45)], 16, 4, 128, 8, 64),
     ([], [], [0, 50, 7], 8, 2, 128, 8, 64),
 ])
 @pytest.mark.parametrize("tight", [False, True])
