@@ -105,8 +105,14 @@ struct PromptSmem {
   static constexpr int P_AT = APART ? 256 : 0, P_TILE = APART ? 64 : 128, O_AT = APART ? 384 : 256;
   uint8_t q[2][TILE];
   uint8_t ring[STAGES][TILE];  // K_0 V_0 K_1 V_1 ...
-  union {                      // between the two warps of 32 rows
-    uint16_t top[2][32];
+  // Between the two warps of 32 rows.  A thread reads the other's maximum after
+  // a block's last barrier.  With P over the scores the next ones need both
+  // threads' P, so the word is free by then; with P apart they do not, and the
+  // next block's maxima go into words of their own, which that block's barrier
+  // orders before the ones after.
+  static constexpr int TOPS = APART ? 2 : 1;
+  union {
+    uint16_t top[TOPS][2][32];
     float sum[32];
   } exchange[8];
   int quit[8][2];              // per pair of warps and parity of the block: a wait gave up
@@ -582,18 +588,19 @@ __global__ void __launch_bounds__(PA_THREADS, 1) prompt_attn_kernel(const Prompt
         // every score of the 32 rows has been read past this barrier, and what
         // a thread leaves before it can be read by the other: the upper half
         // of its maximum's bits
-        exchange.top[h][lane] = uint16_t(__float_as_uint(top) >> 16);
+        auto& tops = exchange.top[j % SM::TOPS];
+        tops[h][lane] = uint16_t(__float_as_uint(top) >> 16);
         if (!ok) sm.quit[pair][j & 1] = 1;
         if (bar_or(bar, 64, !ok || j == 0 || !(top <= m + 8.f))) {
           if (*const_cast<volatile int*>(&sm.quit[pair][j & 1])) {
             quit = true;
             break;
           }
-          const uint32_t upper = exchange.top[1 - h][lane];
+          const uint32_t upper = tops[1 - h][lane];
           bar_all(bar, 64);
-          exchange.top[h][lane] = uint16_t(__float_as_uint(top));  // then the lower half
+          tops[h][lane] = uint16_t(__float_as_uint(top));  // then the lower half
           bar_all(bar, 64);
-          float both = max2(top, __uint_as_float(upper << 16 | exchange.top[1 - h][lane]));
+          float both = max2(top, __uint_as_float(upper << 16 | tops[1 - h][lane]));
           if (both == INFINITY) both = __int_as_float(0x7fffffff);  // inf - inf
           const bool move = j == 0 || !(both <= m + 8.f);
           if (j > 0) {
