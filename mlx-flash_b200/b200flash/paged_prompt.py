@@ -219,6 +219,8 @@ def shared_prefix_attention(q: torch.Tensor, k_pages: torch.Tensor, k_scales: to
     each over its own ``seq_lens[b]`` tokens of ``block_table[b]``; requests
     outside every group have their own tokens only.  ``max_prefix_len`` and
     ``max_seq_len`` bound the lengths (by default what the tables can hold).
+    A table entry below 0 (a page that ``plan_pages`` could not give) reads
+    page 0: what such a row gives means nothing, and stays within the pool.
     """
     dev = require_cuda(q, k_pages, k_scales, v_pages, v_scales, prefix_table, prefix_lens, group_offsets, block_table,
                        seq_lens)

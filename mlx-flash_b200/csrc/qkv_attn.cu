@@ -41,13 +41,20 @@ struct AttnParams {
   int max_len;     // PART kernels: the longest sequence read
 };
 
+// Page of entry `e` of sequence b's table row.  An entry below 0 is one that
+// got no page (b2f_page_plan with too few): page 0 is read in its place, so
+// that a call whose batch did not fit stays within the pool.
+__device__ __forceinline__ int page_of(const AttnParams& p, int b, int e) {
+  return max(p.block_table[int64_t(b) * p.max_pages + e], 0);
+}
+
 // The kernels' PART form writes partials for a combine with other splits of
 // the same rows (prefix_attn.cu), whatever n_splits is, and takes q and V of
 // any magnitude: query rows are scaled into fp16 by a power of two from their
 // absmax, V scales by one from the split's first token; both are undone in
 // float32.
 __device__ __forceinline__ float v_reference(const AttnParams& p, int b, int hkv, int token, int DG, int shift) {
-  const int page = p.block_table[int64_t(b) * p.max_pages + token / p.PS];
+  const int page = page_of(p, b, token / p.PS);
   const int64_t row = int64_t(page) * p.Hkv * p.PS + hkv * p.head_stride + (token % p.PS) * p.slot_stride;
   float top = 0.f;
   for (int g = 0; g < DG; ++g) top = fmaxf(top, p.vs[row * DG + g]);
@@ -210,7 +217,7 @@ __global__ void __launch_bounds__(RING ? 160 : 128) qkv_decode_attn_kernel(const
   };
   auto load_tile = [&](int sub, Tile& T) {
     const int t0 = sub * 16;
-    const int page = p.block_table[int64_t(b) * p.max_pages + t0 / p.PS];
+    const int page = page_of(p, b, t0 / p.PS);
     // row of token t0; token t0+i is at rowbase + i*slot_stride
     const int64_t rowbase = int64_t(page) * p.Hkv * p.PS + hkv * p.head_stride + (t0 % p.PS) * p.slot_stride;
     const int64_t ss = p.slot_stride;
@@ -435,7 +442,7 @@ __global__ void __launch_bounds__(RING ? 160 : 128) qkv_decode_attn_kernel(const
             break;
           }
           if (*abort_flag) break;
-          const int page = p.block_table[int64_t(b) * p.max_pages + pg0 + jj];
+          const int page = page_of(p, b, pg0 + jj);
           const int64_t rowbase = (int64_t(page) * p.Hkv + hkv) * p.PS;
           uint8_t* sb = attn_smem + slot * p.slot_bytes;
           mbar_arrive_expect_tx(&full[slot], uint32_t(2 * code_bytes + 2 * sc_bytes));
@@ -690,7 +697,7 @@ __global__ void __launch_bounds__(160, 2) qkv_decode_attn_t8_kernel(const AttnPa
           break;
         }
         if (*abort_flag) break;
-        const int page = p.block_table[int64_t(b) * p.max_pages + pg0 + it];
+        const int page = page_of(p, b, pg0 + it);
         const int64_t rowbase = (int64_t(page) * p.Hkv + hkv) * p.PS;
         uint8_t* sb = attn_smem + slot * p.slot_bytes;
         mbar_arrive_expect_tx(&full[slot], uint32_t(2 * code_bytes + 2 * sc_bytes));
