@@ -73,7 +73,7 @@ struct PrefixSmem {
   uint8_t q[2][TILE];           // at the end, with the ring, the output rows
   uint8_t ring[PX_RING][TILE];  // K_0 V_0 K_1 V_1 ..., fp16
   uint8_t raw[PX_RAW][RAW];     // the same blocks as codes
-  __nv_bfloat16 exchange[2][128];  // between the two threads of a row
+  uint16_t exchange[2][128];    // between the two threads of a row
   float largest[2][4];             // scales of the first block (K, V), per decoding warp
   uint64_t raw_full[PX_RAW], raw_empty[PX_RAW], full[PX_RING], empty[PX_RING], q_full, s_full[2], p_full[2], pv_done[2],
       drain;
@@ -487,14 +487,27 @@ __global__ void __launch_bounds__(PX_THREADS, 1) prefix_attn_kernel(const Prefix
 #pragma unroll
         for (int k = 0; k < 4; ++k) top = fmaxf(top, fmaxf(fabsf(__low2float(e[k])), fabsf(__high2float(e[k]))));
       }
-      // max with the row's other thread, to 8 bits: both take the same value, and
-      // a reference need not be exact
+      // max with the row's other thread.  The reference is the exact maximum: P
+      // goes to fp16, which an error of a few in the exponent overflows or
+      // empties, and rounded to 8 bits it is off by 32 at 10000.  Shared
+      // memory has room for half a float per row, so each hands over two halves.
       auto join = [&](float v) {
-        if (h) sm.exchange[i][r] = __float2bfloat16_rn(v);
-        bar_all(bar, 64);
-        if (!h) sm.exchange[i][r] = __float2bfloat16_rn(max2(v, __bfloat162float(sm.exchange[i][r])));
-        bar_all(bar, 64);
-        return __bfloat162float(sm.exchange[i][r]);
+        uint32_t other = 0;
+#pragma unroll
+        for (int part = 0; part < 2; ++part) {
+          const uint16_t mine = uint16_t(__float_as_uint(v) >> (part ? 0 : 16));
+          uint16_t theirs = 0;
+          if (h) sm.exchange[i][r] = mine;
+          bar_all(bar, 64);
+          if (!h) {
+            theirs = sm.exchange[i][r];
+            sm.exchange[i][r] = mine;
+          }
+          bar_all(bar, 64);
+          if (h) theirs = sm.exchange[i][r];
+          other = other << 16 | theirs;
+        }
+        return max2(v, __uint_as_float(other));
       };
       const float qn = pow2_inverse(join(top), 0);
 #pragma unroll

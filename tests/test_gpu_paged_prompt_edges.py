@@ -42,3 +42,63 @@ def test_entries_without_a_page_read_page_0(dev, Hq, Hkv, D, bits, page):
     args = (q, kc, ks, vc, vs)
     assert torch.equal(decode_attention(*args, table, plan.seq_lens, bits, page, Hkv),
                        decode_attention(*args, table.clamp(min=0), plan.seq_lens, bits, page, Hkv))
+
+
+# ---- shared prefixes: large scores ---------------------------------------------------
+
+
+def exact_rows(dev, rows, D, page, g):
+    """One KV head's pages whose key ``t`` holds the whole numbers ``rows[t]`` (codes, scale 1); random values."""
+    n = len(rows)
+    pages = -(-n // page)
+    kc = torch.full((pages, 1, page, D), 127, dtype=torch.uint8, device=dev)
+    kc.view(-1, D)[:n] += torch.tensor(rows, device=dev).to(torch.uint8)  # mod 256: signed values
+    ks = torch.ones(pages, 1, page, D // 64, device=dev)
+    vc, vs, _, _ = paged_rows(dev, [pages * page], 1, D, 8, page, g)
+    vc, vs = vc[:pages].contiguous(), vs[:pages].contiguous()
+    v = (vc.double() - 127).view(pages, 1, page, -1, 64) * vs.double()[..., None]
+    return kc, ks, vc, vs, v.view(pages * page, 1, D)[:n]
+
+
+@pytest.mark.parametrize("n_own", [0, 60])
+@pytest.mark.parametrize("first", [80, 128, 160, 1600, -80, -128, -160, -1600])
+@pytest.mark.parametrize("D", [64, 128])
+def test_shared_prefix_large_scores(dev, D, first, n_own):
+    """Scores of up to 102400 in base 2, of either sign, at several places within a step of a 16-bit float.
+
+    Every product and sum of q and K is a whole number of eighths of at most 24 bits, so a score of M differs from the
+    exact one by the rounding of its scaling in base 2 only, 3 * 2^-24 |M|; the own tokens' kernel sums codes with 1024
+    added in float32, whose roundings come to 10 * 2^-24 * 1151 sum |q|.  A probability moves by twice ln 2 of that.
+    """
+    from b200flash.paged_prompt import shared_prefix_attention
+
+    page, n = 64, 300
+    g = torch.Generator(device=dev).manual_seed(D + first)
+    step = torch.randint(-40, 41, (n + n_own,), device=dev, generator=g).tolist()
+    offs = [0, 13, 31, 45, 100]
+    rows = [[64, 1, s] + [0] * (D - 3) for s in step]
+    kc, ks, vc, vs, v = exact_rows(dev, rows, D, page, g)
+    q = torch.zeros(len(offs), 2, D, device=dev)
+    q[:, :, 0] = first
+    q[:, :, 1] = torch.tensor(offs, device=dev)[:, None]
+    q[:, 0, 2], q[:, 1, 2] = 0.125, -0.125
+    q = q.to(torch.bfloat16)
+    i32 = dict(dtype=torch.int32, device=dev)
+    B = len(offs)
+    pages = torch.arange(kc.shape[0], **i32)
+    if n_own:  # the prefix's last page and the own tokens' first are different pages
+        cut = 256
+        own = pages[cut // page:].expand(B, -1).contiguous()
+    else:
+        cut, own = n, torch.zeros(B, 1, **i32)
+    out = shared_prefix_attention(q, kc, ks, vc, vs, pages[None, : -(-cut // page)].contiguous(),
+                                  torch.tensor([cut], **i32), torch.tensor([0, B], **i32), own,
+                                  torch.full((B,), n + n_own - cut, **i32), 8, page, 1, softmax_scale=math.log(2))
+    k = torch.tensor(rows, dtype=torch.float64, device=dev)[:, None]
+    for b in range(B):
+        o, o_abs, _ = attend_reference(q[b][None], k, v, False, math.log(2))
+        most = abs(first) * 64 + 105
+        score = 3 * 2.0 ** -24 * most
+        if n_own:
+            score += 10 * 2.0 ** -24 * 1151 * float(q[b].double().abs().sum(-1).max())
+        within(out[b], o[0], 2.0 ** -8 * (o[0].abs() + o_abs[0]) + 2 * math.log(2) * score * o_abs[0] + 1e-6, f"row {b}")
