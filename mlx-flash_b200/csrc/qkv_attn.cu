@@ -50,16 +50,35 @@ __device__ __forceinline__ int page_of(const AttnParams& p, int b, int e) {
 
 // The kernels' PART form writes partials for a combine with other splits of
 // the same rows (prefix_attn.cu), whatever n_splits is, and takes q and V of
-// any magnitude: query rows are scaled into fp16 by a power of two from their
-// absmax, V scales by one from the split's first token; both are undone in
-// float32.
-__device__ __forceinline__ float v_reference(const AttnParams& p, int b, int hkv, int token, int DG, int shift) {
-  const int page = page_of(p, b, token / p.PS);
-  const int64_t row = int64_t(page) * p.Hkv * p.PS + hkv * p.head_stride + (token % p.PS) * p.slot_stride;
-  float top = 0.f;
-  for (int g = 0; g < DG; ++g) top = fmaxf(top, p.vs[row * DG + g]);
-  return pow2_inverse(top, shift);
-}
+// any magnitude.
+//   Query rows are scaled into fp16 by a power of two from their absmax, which
+// is undone in float32.
+//   Codes enter the products as code - max_int, exactly: with an offset that is
+// subtracted behind them, a group of zeros (scale 1 in the cache, whatever
+// lies beside it) would leave 2^-14 of its scale behind.  The subtractions cost
+// what the products that carry the offset do (128 rows over 8 KV heads, up to
+// 2000 tokens each: 74.4 / 74.6 us; 64 rows over 4, up to 512: 12.8 / 13.7).
+//   P' = P * scale is what fp16 holds of P and of V's scales: the exponent of P
+// is shifted so that the largest scale a warp has met gives P' below 2^15.  P'
+// has 11 bits down to 2^-14, so scales 2^28 below the largest keep them.  l and
+// the partial's m are those of the shifted P.
+struct VShift {
+  int top = 81;       // largest biased exponent of a scale; from 2^-46 up
+  float shift = 60.f;  // P is shifted by 14 - (top - 127)
+  // Takes in a tile's scales (the largest of each group of this lane; infinite
+  // ones, whose group's outputs are not finite anyway, do not count).  Every
+  // lane calls it; returns by how much the shift rose (it falls).
+  template <int DG>
+  __device__ __forceinline__ float cover(const float (&mx)[DG]) {
+    float v = 0.f;
+#pragma unroll
+    for (int g = 0; g < DG; ++g) v = fmaxf(v, mx[g] < INFINITY ? mx[g] : 0.f);
+    top = max(top, int(__reduce_max_sync(0xffffffffu, __float_as_uint(v)) >> 23));
+    const float before = shift;
+    shift = float(141 - top);
+    return shift - before;
+  }
+};
 // largest magnitude of 16 consecutive values (32-byte aligned)
 __device__ __forceinline__ float absmax16(const __nv_bfloat16* x) {
   float top = 0.f;
@@ -71,10 +90,6 @@ __device__ __forceinline__ float absmax16(const __nv_bfloat16* x) {
     for (int k = 0; k < 4; ++k) top = fmaxf(top, fmaxf(fabsf(__low2float(e[k])), fabsf(__high2float(e[k]))));
   }
   return top;
-}
-__device__ __forceinline__ float scaled_up_to(float s, float f, float top) {
-  const float x = s * f;
-  return x > top ? top : x;  // NaN stays
 }
 
 // Named barrier `id` over the first `n` threads of the CTA.
@@ -131,7 +146,9 @@ __global__ void __launch_bounds__(RING ? 160 : 128) qkv_decode_attn_kernel(const
   uint32_t qa[KSTEPS][4];
   float qg[2][DG];
   float hs[2];  // PART: scores = S * hs
-  const float vn = PART && sub_begin < sub_end ? v_reference(p, b, hkv, sub_begin * 16, DG, -7) : 1.f;
+  VShift vshift;  // PART
+  const uint32_t off2 = pack_f16x2(KOFF, KOFF);
+  auto k_codes = [&](uint32_t w) { return PART ? hsub2_u(w, off2) : w; };
 #pragma unroll
   for (int h2 = 0; h2 < 2; ++h2) {
     const int head = r + 8 * h2;
@@ -289,15 +306,15 @@ __global__ void __launch_bounds__(RING ? 160 : 128) qkv_decode_attn_kernel(const
 #pragma unroll
           for (int st = 0; st < 4; ++st) {
             const uint32_t w = kw[nt][g][st];
-            const uint32_t bf[2] = {prmt(w, 0x64646464u, 0x4140u), prmt(w, 0x64646464u, 0x4342u)};
+            const uint32_t bf[2] = {k_codes(prmt(w, 0x64646464u, 0x4140u)), k_codes(prmt(w, 0x64646464u, 0x4342u))};
             mma_f16_16816(sacc[g], qa[g * 4 + st], bf);
           }
         } else if constexpr (BITS == 2) {
           const uint32_t w = kw[nt][g][0];
 #pragma unroll
           for (int st = 0; st < 4; ++st) {
-            const uint32_t bf[2] = {and_or(w >> (4 * st), 0x00030003u, 0x64006400u),
-                                    and_or(w >> (4 * st + 2), 0x00030003u, 0x64006400u)};
+            const uint32_t bf[2] = {k_codes(and_or(w >> (4 * st), 0x00030003u, 0x64006400u)),
+                                    k_codes(and_or(w >> (4 * st + 2), 0x00030003u, 0x64006400u))};
             mma_f16_16816(sacc[g], qa[g * 4 + st], bf);
           }
         } else {
@@ -308,8 +325,8 @@ __global__ void __launch_bounds__(RING ? 160 : 128) qkv_decode_attn_kernel(const
             const uint32_t e04 = and_or(w >> 4, 0x000F000Fu, 0x64006400u);
             const uint32_t e37 = and_or(w >> 8, 0x000F000Fu, 0x64006400u);
             const uint32_t e26 = and_or(w >> 12, 0x000F000Fu, 0x64006400u);
-            const uint32_t bA[2] = {e04, e15};
-            const uint32_t bB[2] = {e26, e37};
+            const uint32_t bA[2] = {k_codes(e04), k_codes(e15)};
+            const uint32_t bB[2] = {k_codes(e26), k_codes(e37)};
             mma_f16_16816(sacc[g], qa[g * 4 + 2 * wi], bA);
             mma_f16_16816(sacc[g], qa[g * 4 + 2 * wi + 1], bB);
           }
@@ -320,7 +337,7 @@ __global__ void __launch_bounds__(RING ? 160 : 128) qkv_decode_attn_kernel(const
         const int row = i >> 1, e = i & 1;
         float v = 0.f;
 #pragma unroll
-        for (int g = 0; g < DG; ++g) v += ksc[nt][e][g] * (sacc[g][i] - KOFF * qg[row][g]);
+        for (int g = 0; g < DG; ++g) v += ksc[nt][e][g] * (PART ? sacc[g][i] : sacc[g][i] - KOFF * qg[row][g]);
         const int tok = nt * 8 + 2 * c + e;
         if constexpr (PART) v *= hs[row];
         s[nt][i] = (t0 + tok < len) ? v : -INFINITY;
@@ -328,13 +345,20 @@ __global__ void __launch_bounds__(RING ? 160 : 128) qkv_decode_attn_kernel(const
     }
 
     // ---- online softmax (rows r and r+8) --------------------------------
+    float rose = 0.f;
+    if constexpr (PART) {
+      float mx[DG];
+#pragma unroll
+      for (int g = 0; g < DG; ++g) mx[g] = fmaxf(fmaxf(vsc[0][g], vsc[1][g]), fmaxf(vsc[2][g], vsc[3][g]));
+      rose = vshift.cover(mx);
+    }
     float pr[2][4];
 #pragma unroll
     for (int row = 0; row < 2; ++row) {
       float mt = fmaxf(fmaxf(s[0][2 * row], s[0][2 * row + 1]), fmaxf(s[1][2 * row], s[1][2 * row + 1]));
       mt = fmaxf(mt, __shfl_xor_sync(0xffffffffu, mt, 1));
       mt = fmaxf(mt, __shfl_xor_sync(0xffffffffu, mt, 2));
-      const float mnew = fmaxf(m_run[row], mt);
+      const float mnew = PART ? fmaxf(m_run[row] - rose, mt - vshift.shift) : fmaxf(m_run[row], mt);
       const bool none = (mnew == -INFINITY);
       const float alpha = none ? 1.f : exp2f(m_run[row] - mnew);
       float lsum = 0.f;
@@ -356,20 +380,26 @@ __global__ void __launch_bounds__(RING ? 160 : 128) qkv_decode_attn_kernel(const
     }
 
     // ---- O += P.V --------------------------------------------------------
-    const uint32_t pa[4] = {pack_f16x2(pr[0][0], pr[0][1]), pack_f16x2(pr[0][2], pr[0][3]),
-                            pack_f16x2(pr[1][0], pr[1][1]), pack_f16x2(pr[1][2], pr[1][3])};
+    uint32_t pa[PART ? DG : 1][4];
     uint32_t vs01[DG], vs23[DG];
 #pragma unroll
     for (int g = 0; g < DG; ++g) {
-      if constexpr (PART) {  // 255 * 256 is the last fp16 value
-        vs01[g] = pack_f16x2(scaled_up_to(vsc[0][g], vn, 256.f), scaled_up_to(vsc[1][g], vn, 256.f));
-        vs23[g] = pack_f16x2(scaled_up_to(vsc[2][g], vn, 256.f), scaled_up_to(vsc[3][g], vn, 256.f));
+      if constexpr (PART) {  // the scales go into P
+        pa[g][0] = pack_f16x2(pr[0][0] * vsc[0][g], pr[0][1] * vsc[1][g]);
+        pa[g][1] = pack_f16x2(pr[0][2] * vsc[0][g], pr[0][3] * vsc[1][g]);
+        pa[g][2] = pack_f16x2(pr[1][0] * vsc[2][g], pr[1][1] * vsc[3][g]);
+        pa[g][3] = pack_f16x2(pr[1][2] * vsc[2][g], pr[1][3] * vsc[3][g]);
       } else {
         vs01[g] = pack_f16x2(vsc[0][g], vsc[1][g]);
         vs23[g] = pack_f16x2(vsc[2][g], vsc[3][g]);
       }
     }
-    const uint32_t off2 = pack_f16x2(KOFF, KOFF);
+    if constexpr (!PART) {
+      pa[0][0] = pack_f16x2(pr[0][0], pr[0][1]);
+      pa[0][1] = pack_f16x2(pr[0][2], pr[0][3]);
+      pa[0][2] = pack_f16x2(pr[1][0], pr[1][1]);
+      pa[0][3] = pack_f16x2(pr[1][2], pr[1][3]);
+    }
 #pragma unroll
     for (int j = 0; j < NTD; ++j) {
       const int gj = j >> 3, jj = j & 7;
@@ -397,8 +427,12 @@ __global__ void __launch_bounds__(RING ? 160 : 128) qkv_decode_attn_kernel(const
         x01 = and_or(y01, 0x000F000Fu, 0x64006400u);
         x23 = and_or(y23, 0x000F000Fu, 0x64006400u);
       }
-      const uint32_t bfr[2] = {hmul2_u(hsub2_u(x01, off2), vs01[gj]), hmul2_u(hsub2_u(x23, off2), vs23[gj])};
-      mma_f16_16816(oacc[j], pa, bfr);
+      uint32_t bfr[2] = {hsub2_u(x01, off2), hsub2_u(x23, off2)};
+      if constexpr (!PART) {
+        bfr[0] = hmul2_u(bfr[0], vs01[gj]);
+        bfr[1] = hmul2_u(bfr[1], vs23[gj]);
+      }
+      mma_f16_16816(oacc[j], pa[PART ? gj : 0], bfr);
     }
   };
 
@@ -574,7 +608,7 @@ __global__ void __launch_bounds__(RING ? 160 : 128) qkv_decode_attn_kernel(const
     const int64_t bh = int64_t(b) * p.Hq + hq0 + head;
     if constexpr (PART) {
       const int64_t part = bh * p.n_splits + split;
-      p.o_part[part * D + d] = o / vn;
+      p.o_part[part * D + d] = o;
       if (d == 0) {
         p.ml_part[part * 2 + 0] = mstar;
         p.ml_part[part * 2 + 1] = l;
@@ -715,13 +749,19 @@ __global__ void __launch_bounds__(160, 2) qkv_decode_attn_t8_kernel(const AttnPa
   }
 
   // ---- consumer warps 0..3 ---------------------------------------------------
+  auto exact_codes = [](uint32_t (&a)[4]) {  // 1024 + code -> code - 127
+    if constexpr (PART) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) a[i] = hsub2_u(a[i], 0x647F647Fu);
+    }
+  };
   const uint32_t ONE2 = 0x3C003C00u;
   const uint32_t ones[4] = {ONE2, ONE2, ONE2, ONE2};
   {
     uint32_t qb[DG * 4][2];
     float kq[2][DG];  // heads 2c, 2c+1
     float hs[2];      // PART: scores = S * hs
-    const float vn = PART && sub_begin < sub_end ? v_reference(p, b, hkv, sub_begin * 16, DG, 0) : 1.f;
+    VShift vshift;    // PART
     // ---- q^T fragments (head g, dims 64grp+16c+[0,16)) and (1024+127)*sum(q)
     {
       const bool hv = g < G;
@@ -826,13 +866,8 @@ __global__ void __launch_bounds__(160, 2) qkv_decode_attn_t8_kernel(const AttnPa
                 const float2 vv = *reinterpret_cast<const float2*>(vsb + row * DG);
                 ksc[t][h][0] = kk.x;
                 ksc[t][h][1] = kk.y;
-                if constexpr (PART) {  // P <= 1, so P' stays below fp16's last value
-                  vsc[t][h][0] = valid[t][h] ? scaled_up_to(vv.x, vn, 32768.f) : 0.f;
-                  vsc[t][h][1] = valid[t][h] ? scaled_up_to(vv.y, vn, 32768.f) : 0.f;
-                } else {
-                  vsc[t][h][0] = valid[t][h] ? vv.x : 0.f;
-                  vsc[t][h][1] = valid[t][h] ? vv.y : 0.f;
-                }
+                vsc[t][h][0] = valid[t][h] ? vv.x : 0.f;
+                vsc[t][h][1] = valid[t][h] ? vv.y : 0.f;
               }
             }
 
@@ -849,8 +884,9 @@ __global__ void __launch_bounds__(160, 2) qkv_decode_attn_t8_kernel(const AttnPa
                 const uint32_t k1[4] = {kw[t][1][grp].x, kw[t][1][grp].y, kw[t][1][grp].z, kw[t][1][grp].w};
     #pragma unroll
                 for (int st = 0; st < 4; ++st) {
-                  const uint32_t a[4] = {prmt(k0[st], 0x64646464u, 0x4140u), prmt(k1[st], 0x64646464u, 0x4140u),
-                                         prmt(k0[st], 0x64646464u, 0x4342u), prmt(k1[st], 0x64646464u, 0x4342u)};
+                  uint32_t a[4] = {prmt(k0[st], 0x64646464u, 0x4140u), prmt(k1[st], 0x64646464u, 0x4140u),
+                                   prmt(k0[st], 0x64646464u, 0x4342u), prmt(k1[st], 0x64646464u, 0x4342u)};
+                  exact_codes(a);
                   mma_f16_16816(sacc[grp], a, qb[grp * 4 + st]);
                 }
               }
@@ -859,13 +895,24 @@ __global__ void __launch_bounds__(160, 2) qkv_decode_attn_t8_kernel(const AttnPa
                 const int h = i >> 1, e = i & 1;
                 float v = 0.f;
     #pragma unroll
-                for (int grp = 0; grp < DG; ++grp) v += ksc[t][h][grp] * (sacc[grp][i] - kq[e][grp]);
+                for (int grp = 0; grp < DG; ++grp) v += ksc[t][h][grp] * (PART ? sacc[grp][i] : sacc[grp][i] - kq[e][grp]);
                 if constexpr (PART) v *= hs[e];
                 s[t][i] = valid[t][h] ? v : -INFINITY;
               }
             }
 
             // ---- online softmax (heads 2c, 2c+1 over the 8 lanes of a column) --
+            float rose = 0.f;
+            if constexpr (PART) {
+              float mx[DG];
+    #pragma unroll
+              for (int grp = 0; grp < DG; ++grp) {
+                mx[grp] = fmaxf(vsc[0][0][grp], vsc[0][1][grp]);
+    #pragma unroll
+                for (int t = 1; t < NT; ++t) mx[grp] = fmaxf(mx[grp], fmaxf(vsc[t][0][grp], vsc[t][1][grp]));
+              }
+              rose = vshift.cover(mx);
+            }
             float pr[NT][4];
     #pragma unroll
             for (int e = 0; e < 2; ++e) {
@@ -875,7 +922,7 @@ __global__ void __launch_bounds__(160, 2) qkv_decode_attn_t8_kernel(const AttnPa
               mt = fmaxf(mt, __shfl_xor_sync(0xffffffffu, mt, 4));
               mt = fmaxf(mt, __shfl_xor_sync(0xffffffffu, mt, 8));
               mt = fmaxf(mt, __shfl_xor_sync(0xffffffffu, mt, 16));
-              const float mnew = fmaxf(m_run[e], mt);
+              const float mnew = PART ? fmaxf(m_run[e] - rose, mt - vshift.shift) : fmaxf(m_run[e], mt);
               const bool none = (mnew == -INFINITY);
               const float alpha = none ? 1.f : fast_exp2(m_run[e] - mnew);
               float lsum = 0.f;
@@ -907,7 +954,7 @@ __global__ void __launch_bounds__(160, 2) qkv_decode_attn_t8_kernel(const AttnPa
                 const uint32_t xlo = pack_f16x2(pr[t][0] * vsc[t][0][grp], pr[t][1] * vsc[t][0][grp]);
                 const uint32_t xhi = pack_f16x2(pr[t][2] * vsc[t][1][grp], pr[t][3] * vsc[t][1][grp]);
                 const uint32_t bp[2] = {movmatrix_trans(xlo), movmatrix_trans(xhi)};
-                mma_f16_16816(oone[grp], ones, bp);
+                if constexpr (!PART) mma_f16_16816(oone[grp], ones, bp);
     #pragma unroll
                 for (int jl = 0; jl < 4; ++jl) {
                   const int bs = 2 * (jl & 1);
@@ -917,10 +964,11 @@ __global__ void __launch_bounds__(160, 2) qkv_decode_attn_t8_kernel(const AttnPa
                   const uint32_t w1 = (jl >> 1) ? vw[t][1][grp].y : vw[t][1][grp].x;
                   const uint32_t w2 = (jl >> 1) ? vw[t][2][grp].y : vw[t][2][grp].x;
                   const uint32_t w3 = (jl >> 1) ? vw[t][3][grp].y : vw[t][3][grp].x;
-                  const uint32_t a[4] = {and_or(prmt(w0, w1, sel_lo), 0x00FF00FFu, 0x64006400u),
-                                         and_or(prmt(w0, w1, sel_hi), 0x00FF00FFu, 0x64006400u),
-                                         and_or(prmt(w2, w3, sel_lo), 0x00FF00FFu, 0x64006400u),
-                                         and_or(prmt(w2, w3, sel_hi), 0x00FF00FFu, 0x64006400u)};
+                  uint32_t a[4] = {and_or(prmt(w0, w1, sel_lo), 0x00FF00FFu, 0x64006400u),
+                                   and_or(prmt(w0, w1, sel_hi), 0x00FF00FFu, 0x64006400u),
+                                   and_or(prmt(w2, w3, sel_lo), 0x00FF00FFu, 0x64006400u),
+                                   and_or(prmt(w2, w3, sel_hi), 0x00FF00FFu, 0x64006400u)};
+                  exact_codes(a);
                   mma_f16_16816(oacc[grp * 4 + jl], a, bp);
                 }
               }
@@ -949,7 +997,8 @@ __global__ void __launch_bounds__(160, 2) qkv_decode_attn_t8_kernel(const AttnPa
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
             const int d = 64 * grp + vdim + 2 * jl + h;
-            sm_o[(warp * G + head) * D + d] = oacc[j][2 * h + e] - KOFF * oone[grp][2 * h + e];
+            sm_o[(warp * G + head) * D + d] =
+                PART ? oacc[j][2 * h + e] : oacc[j][2 * h + e] - KOFF * oone[grp][2 * h + e];
           }
         }
       }
@@ -974,7 +1023,7 @@ __global__ void __launch_bounds__(160, 2) qkv_decode_attn_t8_kernel(const AttnPa
       const int64_t bh = int64_t(b) * p.Hq + hq0 + head;
       if constexpr (PART) {
         const int64_t part = bh * p.n_splits + int(blockIdx.x);
-        p.o_part[part * D + d] = o / vn;
+        p.o_part[part * D + d] = o;
         if (d == 0) {
           p.ml_part[part * 2 + 0] = mstar;
           p.ml_part[part * 2 + 1] = l;

@@ -67,8 +67,8 @@ def test_shared_prefix_large_scores(dev, D, first, n_own):
     """Scores of up to 102400 in base 2, of either sign, at several places within a step of a 16-bit float.
 
     Every product and sum of q and K is a whole number of eighths of at most 24 bits, so a score of M differs from the
-    exact one by the rounding of its scaling in base 2 only, 3 * 2^-24 |M|; the own tokens' kernel sums codes with 1024
-    added in float32, whose roundings come to 10 * 2^-24 * 1151 sum |q|.  A probability moves by twice ln 2 of that.
+    exact one by the rounding of its scaling in base 2 only, 3 * 2^-24 |M|; own tokens are given the roundings of sums of
+    codes with 1024 added in float32, 10 * 2^-24 * 1151 sum |q|.  A probability moves by twice ln 2 of that.
     """
     from b200flash.paged_prompt import shared_prefix_attention
 
@@ -102,3 +102,110 @@ def test_shared_prefix_large_scores(dev, D, first, n_own):
         if n_own:
             score += 10 * 2.0 ** -24 * 1151 * float(q[b].double().abs().sum(-1).max())
         within(out[b], o[0], 2.0 ** -8 * (o[0].abs() + o_abs[0]) + 2 * math.log(2) * score * o_abs[0] + 1e-6, f"row {b}")
+
+
+# ---- shared prefixes: rows of very different magnitudes ------------------------------
+
+
+def cache_of(x, bits, page):
+    """Pages (in order) of the rows ``x`` [n, Hkv, D], and the values that they stand for in 64 bits."""
+    from b200flash.quantized_kv_cache import quantize_tensor
+
+    n, Hkv, D = x.shape
+    pages = max(1, -(-n // page))
+    full = torch.zeros(pages * page, Hkv, D, dtype=x.dtype, device=x.device)
+    full[:n] = x
+    codes, scales, _ = quantize_tensor(full.view(pages, page, Hkv, D).transpose(1, 2).contiguous(), bits, 64)
+    c = codes
+    if bits < 8:
+        c = torch.stack([(codes >> s) & (2 ** bits - 1) for s in range(8 - bits, -1, -bits)], -1).flatten(-2)
+    v = (c.double() - (2 ** (bits - 1) - 1)).view(pages, Hkv, page, -1, 64) * scales.double()[..., None]
+    return codes, scales, v.reshape(pages, Hkv, page, D).transpose(1, 2).reshape(-1, Hkv, D)[:n]
+
+
+def run_rows(k, v, own, bits, page, q, softmax_scale, splits=1):
+    """Attention of ``q`` over the rows ``k``, ``v`` [n, Hkv, D], as one request's own tokens or as its prefix."""
+    from b200flash.paged_prompt import shared_prefix_attention
+
+    dev, n, Hkv = q.device, k.shape[0], k.shape[1]
+    kc, ks, kv = cache_of(k, bits, page)
+    vc, vs, vv = cache_of(v, bits, page)
+    i32 = dict(dtype=torch.int32, device=dev)
+    B = q.shape[0]
+    table = torch.arange(kc.shape[0], **i32)
+    lens = torch.full((B,), n, **i32)
+    empty, none = torch.zeros(B, 1, **i32), torch.zeros(B, **i32)
+    if own:
+        out = shared_prefix_attention(q, kc, ks, vc, vs, empty[:0], none[:0], none[:1], table.expand(B, -1).contiguous(),
+                                      lens, bits, page, Hkv, softmax_scale=softmax_scale)
+    else:
+        out = shared_prefix_attention(q, kc, ks, vc, vs, table[None], lens[:1], torch.tensor([0, B], **i32), empty, none,
+                                      bits, page, Hkv, softmax_scale=softmax_scale)
+    return out, kv, vv
+
+
+def check_rows(out, q, kv, vv, softmax_scale, floor):
+    """The bound of run_prefix: roundings of P, V and the output, 2^-11 of each product in a score."""
+    G = q.shape[1] // kv.shape[1]
+    for b in range(q.shape[0]):
+        o, o_abs, _ = attend_reference(q[b][None], kv, vv, False, softmax_scale)
+        move = 2.0 ** -11 * torch.einsum("hd,mhd->hm", q[b].double().abs(), kv.abs().repeat_interleave(G, 1)).amax(-1)
+        within(out[b], o[0], 2.0 ** -8 * (o[0].abs() + o_abs[0]) + 2 * softmax_scale * move[:, None] * o_abs[0] + floor,
+               f"row {b}")
+
+
+FORMS = [  # Hq, Hkv, D, bits, page: every form of the own-token kernel, every width of the prefix kernel
+    (8, 2, 128, 8, 64), (8, 2, 128, 8, 16), (16, 1, 128, 8, 16), (8, 2, 64, 8, 64), (8, 2, 128, 4, 16),
+    (4, 2, 64, 4, 32), (8, 2, 128, 2, 16), (8, 2, 64, 2, 32), (4, 1, 128, 8, 512),
+]
+
+
+def zeros_among_small_values(dev, form, size, own):
+    Hq, Hkv, D, bits, page = form
+    g = torch.Generator(device=dev).manual_seed(int(-math.log10(size)) + D)
+    n = 300
+    k, v = (torch.randn(n, Hkv, D, device=dev, generator=g) for _ in range(2))
+    v *= size
+    for at in (0, 37, 38, 250, 299):
+        k[at] = v[at] = 0  # a group of zeros has scale 1
+    k[20, 0, :64] = v[60, :, :64] = v[129, 0, :64] = 0
+    k, v = k.to(torch.bfloat16), v.to(torch.bfloat16)
+    q = torch.randn(3, Hq, D, device=dev, generator=g).to(torch.bfloat16)
+    out, kv, vv = run_rows(k, v, own, bits, page, q, D ** -0.5)
+    check_rows(out, q, kv, vv, D ** -0.5, 1e-6 * size)
+    # small keys: the scores are made up for by the queries
+    k2 = (k.float() * size).to(torch.bfloat16)
+    q2 = (q.float() / size).to(torch.bfloat16)
+    out, kv, vv = run_rows(k2, v, own, bits, page, q2, D ** -0.5)
+    check_rows(out, q2, kv, vv, D ** -0.5, 1e-6 * size)
+
+
+def values_that_jump(dev, form, ratio, own, dtype=torch.bfloat16):
+    """Values ``ratio`` times larger or smaller from some token on, to rows that see either side, or both."""
+    Hq, Hkv, D, bits, page = form
+    g = torch.Generator(device=dev).manual_seed(D + bits)
+    n = 300
+    for first in (1, 3, 40, 128, 130, 290):
+        for scale in (ratio, 1 / ratio):
+            k, v = (torch.randn(n, Hkv, D, device=dev, generator=g) for _ in range(2))
+            v[first:] *= scale
+            k[:, :, 0] = 0
+            k[first:, :, 0] = 7.0
+            q = torch.randn(3, Hq, D, device=dev, generator=g)
+            # scores of the second part: 60 higher, 60 lower, alike
+            q[:, :, 0] = torch.tensor([60.0, -60.0, 0.0], device=dev)[:, None] * D ** 0.5 / 7.0
+            k, v, q = k.to(dtype), v.to(dtype), q.to(torch.bfloat16)
+            out, kv, vv = run_rows(k, v, own, bits, page, q, D ** -0.5)
+            check_rows(out, q, kv, vv, D ** -0.5, 1e-6 * min(1.0, scale))
+
+
+@pytest.mark.parametrize("size", [0.1, 1e-2, 1e-4, 1e-6])
+@pytest.mark.parametrize("form", FORMS)
+def test_own_tokens_of_zeros_among_small_values(dev, form, size):
+    zeros_among_small_values(dev, form, size, own=True)
+
+
+@pytest.mark.parametrize("ratio", [2.0 ** 8, 1e5, 2.0 ** 20])
+@pytest.mark.parametrize("form", FORMS)
+def test_own_tokens_whose_values_jump(dev, form, ratio):
+    values_that_jump(dev, form, ratio, own=True)
