@@ -29,8 +29,13 @@
 // rounding of 2^-11, where bf16 would cost 2^-8 on K, V and P each -- more than
 // the output's own rounding.  fp16's range is made up for by powers of two,
 // which are exact: each query row is scaled by its own absmax, K and V by the
-// largest scale of the CTA's first block (2^14 up to saturation, 2^14 down to
-// the first lost bit); the scores and the output are scaled back in float32.
+// largest scale of each block (groups of zeros, whose scale is 1 whatever lies
+// beside them, do not count), which lands at 2^(15-BITS): nothing is cut, and
+// below it a scale of 8 significant bits (rows quantized as bf16) is exact for
+// 2^(32-BITS), one of 11 for 2^(29-BITS).  K's power comes back into the scores.
+// V's goes into them as an exponent: with v = 2^a v' the row's weights are
+// 2^(s + a - m), whose products with v' add up to 2^-m sum 2^s v, and which
+// times 2^-a add up to l = 2^-m sum 2^s.
 #include "attn_tc.cuh"
 
 namespace b2f {
@@ -42,7 +47,7 @@ int launch_own_partials(const __nv_bfloat16* q, const uint8_t* kc, const float* 
                         int bits, float scale, int n_splits, int max_len, float* o_part, float* ml_part,
                         cudaStream_t st);
 
-// warps 0-15 softmax, 16-19 decode K, 20-23 V, 24 issues the MMAs, 25 copies K, 26 V
+// warps 0-15 softmax, 16-19 decode K, 20-23 V, 24 issues the MMAs, 25 copies K and finds its power, 26 V
 constexpr int PX_THREADS = 864;
 constexpr int PX_MMA = 24, PX_COPY = 25;
 constexpr int PX_BN = 128;  // keys per block
@@ -74,9 +79,15 @@ struct PrefixSmem {
   uint8_t ring[PX_RING][TILE];  // K_0 V_0 K_1 V_1 ..., fp16
   uint8_t raw[PX_RAW][RAW];     // the same blocks as codes
   uint16_t exchange[2][128];    // between the two threads of a row
-  float largest[2][4];             // scales of the first block (K, V), per decoding warp
+  // Of block j (mod 8: the copies are at most 4 blocks ahead of the softmax).
+  float norm[2][8];             // the power of K, of V; negative: some keys do not count
+  float k_back[8];              // 1 / the power of K
+  float2 v_power[8];            // a, 2^-a
   uint64_t raw_full[PX_RAW], raw_empty[PX_RAW], full[PX_RING], empty[PX_RING], q_full, s_full[2], p_full[2], pv_done[2],
       drain;
+  // Block j (mod 4) has its power.  The MMA warp waits for V's before the scores
+  // of j; four blocks on there is another only after P V of j.
+  uint64_t norm_full[2][4];
   int item[6];  // group, first request, requests from there, prefix length, KV head, split
   int per;  // blocks a CTA of the group
   uint32_t tmem;
@@ -255,6 +266,7 @@ __global__ void __launch_bounds__(PX_THREADS, 1) prefix_attn_kernel(const Prefix
       mbar_init(&sm.empty[s], 1);
     }
     mbar_init(&sm.q_full, 16);
+    for (int i = 0; i < 8; ++i) mbar_init(&sm.norm_full[i >> 2][i & 3], 1);
     for (int i = 0; i < 2; ++i) {
       mbar_init(&sm.s_full[i], 1);
       mbar_init(&sm.p_full[i], 8);
@@ -309,8 +321,11 @@ __global__ void __launch_bounds__(PX_THREADS, 1) prefix_attn_kernel(const Prefix
         }
         tc_commit_by(one, &sm.s_full[t]);
       };
+      // Scores are issued once V's power of their block is known: it goes into
+      // them, and the softmax warps wait for the scores only.
+      auto power_of = [&](int j) { return wait_all(&sm.norm_full[1][j & 3], uint32_t((j >> 2) & 1)); };
       Ring ring;
-      bool ok = wait_all(&sm.q_full, 0u) && full_of(ring);
+      bool ok = wait_all(&sm.q_full, 0u) && power_of(0) && full_of(ring);
       if (ok) {
         tc_fence_after();
         for (int t = 0; t < n_tiles; ++t) score(t, ring.s);
@@ -322,7 +337,7 @@ __global__ void __launch_bounds__(PX_THREADS, 1) prefix_attn_kernel(const Prefix
         ok = full_of(rv);
         if (ok && j + 1 < n) {  // K_{j+1}
           ring.next();
-          ok = full_of(ring);
+          ok = power_of(j + 1) && full_of(ring);
         }
         for (int t = 0; ok && t < n_tiles; ++t) {
           const uint64_t v = v_desc + uint64_t(rv.s * (TILE >> 4));
@@ -351,21 +366,27 @@ __global__ void __launch_bounds__(PX_THREADS, 1) prefix_attn_kernel(const Prefix
       const int32_t* pages = p.table + int64_t(g) * p.width;
       const uint8_t* codes = v ? p.vc : p.kc;
       const float* scales = v ? p.vs : p.ks;
-      // a page is loaded a block ahead, and looked at only where it is used
+      // A page is loaded a block ahead, and looked at only where it is used; all
+      // that a copy needs is worked out before its stage is free.
       auto entry_of = [&](int j) {
         const int key = (j0 + j) * PX_BN + 16 * part;
         return part < 8 && j < n && key < len ? key / p.P : -1;
       };
-      int entry = entry_of(0), page = 0, j = 0;
-      if (entry >= 0) page = pages[entry];
+      auto page_of = [&](int entry) { return entry >= 0 ? pages[entry] : 0; };
+      int entry = entry_of(0), page = page_of(entry), j = 0;
+      int64_t row = 0;
+      bool have = false;
+      auto look = [&](int j) {  // where the lane's keys of block j are; the next block's page
+        row = (int64_t(max(page, 0)) * p.Hkv + hk) * p.P + ((j0 + j) * PX_BN + 16 * part) % p.P;
+        have = entry >= 0;
+        entry = entry_of(j + 1);
+        page = page_of(entry);
+      };
+      look(0);
       for (; j < n; ++j) {
-        const int key = (j0 + j) * PX_BN + 16 * part, it = 2 * j + v, s = it % PX_RAW;
-        const int keys = min(PX_BN, (len - (j0 + j) * PX_BN + 15) & ~15);  // of the block, in whole sixteens
-        const int next_entry = entry_of(j + 1);
-        int next = 0;
-        if (next_entry >= 0) next = pages[next_entry];
-        const int64_t row = (int64_t(max(page, 0)) * p.Hkv + hk) * p.P + key % p.P;
-        const bool have = entry >= 0;
+        const int it = 2 * j + v, s = it % PX_RAW;
+        const int valid = len - (j0 + j) * PX_BN;         // keys of the block (128 or more: all)
+        const int keys = min(PX_BN, (valid + 15) & ~15);  // in whole sixteens
         if (it >= PX_RAW &&
             !__all_sync(0xffffffffu, px_wait(&sm.raw_empty[s], uint32_t((it / PX_RAW - 1) & 1), abort_flag)))
           break;
@@ -375,8 +396,49 @@ __global__ void __launch_bounds__(PX_THREADS, 1) prefix_attn_kernel(const Prefix
           bulk_g2s(sm.raw[s] + 16 * part * RB, codes + row * RB, 16 * RB, &sm.raw_full[s]);
           bulk_g2s(sm.raw[s] + SM::CODES + 16 * part * DG * 4, scales + row * DG, 16 * DG * 4, &sm.raw_full[s]);
         }
-        entry = next_entry;
-        page = next;
+        look(j + 1);
+        // the block's power, from the largest scale (4 keys a lane), while the
+        // decoding warps take the codes into registers
+        if (!__all_sync(0xffffffffu, px_wait(&sm.raw_full[s], uint32_t((it / PX_RAW) & 1), abort_flag))) {
+          ++j;
+          break;
+        }
+        const float* sc = reinterpret_cast<const float*>(sm.raw[s] + SM::CODES);
+        float top = 0.f;
+        bool careful = valid < PX_BN;
+        if (!careful) {
+#pragma unroll
+          for (int e = 0; e < DG; ++e) {
+            const float4 x = reinterpret_cast<const float4*>(sc)[lane * DG + e];
+            top = fmaxf(top, fmaxf(fmaxf(x.x, x.y), fmaxf(x.z, x.w)));
+          }
+          top = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(top)));
+          careful = top == 1.f || top == INFINITY;
+        }
+        if (careful) {  // keys past the prefix, groups of zeros and infinite scales do not count
+          top = 0.f;
+          for (int e = 4 * DG * lane; e < min(valid * DG, 4 * DG * (lane + 1)); ++e) {
+            const float x = sc[e];
+            uint32_t some = x < INFINITY;
+            if (x == 1.f) {
+              constexpr uint32_t ZEROS = BITS == 8 ? 0x7F7F7F7Fu : BITS == 4 ? 0x77777777u : 0x55555555u;
+              const uint4* at = reinterpret_cast<const uint4*>(sm.raw[s] + e * (8 * BITS));
+              some = 0;
+              for (int i = 0; i < BITS / 2; ++i)
+                some |= (at[i].x ^ ZEROS) | (at[i].y ^ ZEROS) | (at[i].z ^ ZEROS) | (at[i].w ^ ZEROS);
+            }
+            if (some) top = fmaxf(top, x);
+          }
+          top = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(top)));
+        }
+        if (lane == 0) {
+          const float norm = top > 0.f ? fminf(pow2_inverse(top, 15 - BITS), 0x1p60f) : 0x1p60f;
+          sm.norm[v][j & 7] = careful ? -norm : norm;
+          if (v) sm.v_power[j & 7] = make_float2(float(127 - int(__float_as_uint(norm) >> 23)), norm);
+          else sm.k_back[j & 7] = 1.f / norm;
+          mbar_arrive(&sm.norm_full[v][j & 3]);
+        }
+        __syncwarp();
       }
       // the last copy issued lands before the CTA goes away (those before it were waited for)
       if (j > 0) {
@@ -393,24 +455,10 @@ __global__ void __launch_bounds__(PX_THREADS, 1) prefix_attn_kernel(const Prefix
     const int v = (warp - 16) >> 2;  // K or V
     const int t = tid - 512 - 128 * v, sub = t % LPR;
     constexpr uint32_t OFF = 0x64006400u + uint32_t(TOP) * 0x00010001u;  // 1024 + TOP, twice
-    float norm = 1.f;
     bool ok = true;
     for (int j = 0; j < n; ++j) {
       const int it = 2 * j + v, s = it % PX_RAW, st = it % NST;
       ok = __all_sync(0xffffffffu, ok && px_wait(&sm.raw_full[s], uint32_t((it / PX_RAW) & 1), abort_flag));
-      if (j == 0) {
-        // the reference: the first block's largest scale, which puts its
-        // largest value in [2^(BITS-8), 2^(BITS-6))
-        float top = 0.f;
-        const float* sc = reinterpret_cast<const float*>(sm.raw[s] + SM::CODES);
-        if (ok && t < len - j0 * PX_BN)
-          for (int e = 0; e < DG; ++e)
-            if (sc[t * DG + e] < INFINITY) top = fmaxf(top, sc[t * DG + e]);
-        top = warp_max<32>(top);
-        if (lane == 0) sm.largest[v][warp & 3] = top;
-        bar_all(9 + v, 128);
-        norm = pow2_inverse(fmaxf(fmaxf(sm.largest[v][0], sm.largest[v][1]), fmaxf(sm.largest[v][2], sm.largest[v][3])), -7);
-      }
       if (!ok) break;
       // the lane's codes and scales into registers: the stage is free for the next copy
       const int valid = len - (j0 + j) * PX_BN;  // keys of the block (128 or more: all)
@@ -424,20 +472,35 @@ __global__ void __launch_bounds__(PX_THREADS, 1) prefix_attn_kernel(const Prefix
         for (int c = 0; c < CPT; ++c) {
           const int chunk = sub + LPR * c;
           w[k][c] = *reinterpret_cast<const uint4*>(sm.raw[s] + row * RB + chunk * 16);
-          sc[k][c] = row < valid ? scales[row * DG + chunk * (128 / BITS) / 64] : 0.f;
+          sc[k][c] = scales[row * DG + chunk * (128 / BITS) / 64];
         }
       }
       __syncwarp();
       if (lane == 0) mbar_arrive(&sm.raw_empty[s]);
-      ok = it < NST || __all_sync(0xffffffffu, px_wait(&sm.empty[st], uint32_t((it / NST - 1) & 1), abort_flag));
+      ok = __all_sync(0xffffffffu, px_wait(&sm.norm_full[v][j & 3], uint32_t((j >> 2) & 1), abort_flag)) &&
+           (it < NST || __all_sync(0xffffffffu, px_wait(&sm.empty[st], uint32_t((it / NST - 1) & 1), abort_flag)));
       if (!ok) break;
+      const float norm = sm.norm[v][j & 7];
+#pragma unroll
+      for (int k = 0; k < LPR; ++k)
+#pragma unroll
+        for (int c = 0; c < CPT; ++c) sc[k][c] *= fabsf(norm);
+      if (norm < 0.f) {
+#pragma unroll
+        for (int k = 0; k < LPR; ++k)
+#pragma unroll
+          for (int c = 0; c < CPT; ++c) {
+            // past the prefix; a group of zeros beside smaller scales
+            const bool passes = sc[k][c] > float(1 << (16 - BITS)) && sc[k][c] < INFINITY;
+            if (t / LPR + (128 / LPR) * k >= valid || passes) sc[k][c] = 0.f;
+          }
+      }
 #pragma unroll
       for (int k = 0; k < LPR; ++k) {
         const int row = t / LPR + (128 / LPR) * k;
 #pragma unroll
         for (int c = 0; c < CPT; ++c) {
-          const float x0 = sc[k][c] * norm;
-          const __half2 h2 = __float2half2_rn(x0 > 256.f ? 256.f : x0);  // 255 * 256 is the last fp16 value; NaN stays
+          const __half2 h2 = __float2half2_rn(sc[k][c]);
           const uint32_t s2 = *reinterpret_cast<const uint32_t*>(&h2);
           uint32_t b[32 / BITS];
           spread_codes<BITS>(w[k][c], b);
@@ -525,14 +588,14 @@ __global__ void __launch_bounds__(PX_THREADS, 1) prefix_attn_kernel(const Prefix
       if (lane == 0) mbar_arrive(&sm.q_full);
       const uint32_t lane_at = uint32_t(32 * (warp & 3)) << 16;
       const uint32_t s_at = tmem + lane_at + 128 * i + 64 * h, o_at = tmem + lane_at + 256 + DP * i + DP / 2 * h;
-      float zs = p.scale2 / qn;  // scores in base 2 = S * zs, once K's reference is known
+      const float zq = p.scale2 / qn;  // scores in base 2 = S * zq * K's power back
       float m = -INFINITY, l = 0.f;  // m: reference of the exponents
       bool ok = true, quit = false;
       for (int j = 0; j < n; ++j) {
         ok = ok && wait_all(&sm.s_full[i], uint32_t(j & 1));
         tc_fence_after();
-        if (j == 0)
-          zs /= pow2_inverse(fmaxf(fmaxf(sm.largest[0][0], sm.largest[0][1]), fmaxf(sm.largest[0][2], sm.largest[0][3])), -7);
+        const float2 power = sm.v_power[j & 7];
+        const float zs = fmaxf(zq * sm.k_back[j & 7], 1e-37f);  // above 0: a masked score stays -inf
         const int valid = len - (j0 + j) * PX_BN - 64 * h;  // keys of this half (64 or more: all)
         const bool masked = valid < 64;
         // the scores are read twice, 32 at a time: 64 at once and P do not fit 72 registers
@@ -551,15 +614,17 @@ __global__ void __launch_bounds__(PX_THREADS, 1) prefix_attn_kernel(const Prefix
           scores(c, s);
           mx = max2(mx, row_max(s));
         }
-        mx *= zs;
-        if (bar_or(bar, 64, !ok || j == 0 || !(mx <= m + 8.f))) {
+        mx = fmaf(mx, zs, power.x);
+        // P up to 2^7 when m moves and 2^15 before it does: 11 bits for weights 2^-21 of the largest
+        if (bar_or(bar, 64, !ok || j == 0 || !(mx <= m + 15.f))) {
           if (bar_or(bar, 64, !ok)) {
             quit = true;
             break;
           }
           float both = join(mx);
           if (both == INFINITY) both = __int_as_float(0x7fffffff);  // inf - inf
-          const bool move = j == 0 || !(both <= m + 8.f);
+          const bool move = j == 0 || !(both <= m + 15.f);
+          both -= 7.f;
           if (j > 0) {
             // O holds blocks up to j - 1 once their product is done
             ok = wait_all(&sm.pv_done[i], uint32_t((j - 1) & 1));
@@ -580,17 +645,18 @@ __global__ void __launch_bounds__(PX_THREADS, 1) prefix_attn_kernel(const Prefix
           if (move) m = both;
         }
         const float ref = m == -INFINITY ? 0.f : m;
+        const float from = ref - power.x;
         uint64_t sum[2] = {0ull, 0ull};
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
           uint32_t s[32], pk[16];
           scores(32 * c, s);
-          if (masked) exp_row<false, false>(s, zs, ref, sum, pk);  // exact zeros
-          else exp_row<false, true>(s, zs, ref, sum, pk);
+          if (masked) exp_row<false, false>(s, zs, from, sum, pk);  // exact zeros
+          else exp_row<false, true>(s, zs, from, sum, pk);
           tmem_st16(s_at + 16 * c, pk);  // P goes over this thread's own scores, behind their reading
         }
         const float2 l2 = f32x2_parts(add_x2(sum[0], sum[1]));
-        l += l2.x + l2.y;
+        l = fmaf(l2.x + l2.y, power.y, l);
         tmem_wait_st();
         tc_fence_before();
         __syncwarp();
@@ -602,8 +668,6 @@ __global__ void __launch_bounds__(PX_THREADS, 1) prefix_attn_kernel(const Prefix
       tc_fence_after();
       uint8_t* out = sm.q[0] + (i * 128 + r) * SM::PITCH;
       if (ok) {
-        const float back = 1.f / pow2_inverse(fmaxf(fmaxf(sm.largest[1][0], sm.largest[1][1]),
-                                                    fmaxf(sm.largest[1][2], sm.largest[1][3])), -7);
         if (h) *reinterpret_cast<float*>(out + DP * 4) = l;  // behind the row: this thread's sum
 #pragma unroll
         for (int c = 0; c < DP / 2; c += 16) {
@@ -612,8 +676,8 @@ __global__ void __launch_bounds__(PX_THREADS, 1) prefix_attn_kernel(const Prefix
 #pragma unroll
           for (int e = 0; e < 16; e += 4)
             *reinterpret_cast<float4*>(out + (DP / 2 * h + c + e) * 4) =
-                make_float4(__uint_as_float(o[e]) * back, __uint_as_float(o[e + 1]) * back,
-                            __uint_as_float(o[e + 2]) * back, __uint_as_float(o[e + 3]) * back);
+                make_float4(__uint_as_float(o[e]), __uint_as_float(o[e + 1]), __uint_as_float(o[e + 2]),
+                            __uint_as_float(o[e + 3]));
         }
         fence_proxy_async_smem();
       }

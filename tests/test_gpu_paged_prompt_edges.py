@@ -209,3 +209,22 @@ def test_own_tokens_of_zeros_among_small_values(dev, form, size):
 @pytest.mark.parametrize("form", FORMS)
 def test_own_tokens_whose_values_jump(dev, form, ratio):
     values_that_jump(dev, form, ratio, own=True)
+
+
+@pytest.mark.parametrize("size", [0.1, 1e-2, 1e-4, 1e-6])
+@pytest.mark.parametrize("form", FORMS)
+def test_prefixes_of_zeros_among_small_values(dev, form, size):
+    zeros_among_small_values(dev, form, size, own=False)
+
+
+@pytest.mark.parametrize("ratio", [2.0 ** 8, 1e5, 2.0 ** 20])
+@pytest.mark.parametrize("form", FORMS)
+def test_prefixes_whose_values_jump(dev, form, ratio):
+    values_that_jump(dev, form, ratio, own=False)
+
+
+@pytest.mark.parametrize("form", [f for f in FORMS if f[3] == 8])
+@pytest.mark.parametrize("own", [False, True])
+def test_half_precision_rows_whose_values_jump(dev, form, own):
+    """Scales of 11 significant bits, as rows appended in fp16 have them."""
+    values_that_jump(dev, form, 2.0 ** 10, own, dtype=torch.float16)
