@@ -230,16 +230,21 @@ __device__ __forceinline__ float row_max(const uint32_t (&s)[N]) {
   return max2(max3(m[0], m[1], m[2]), m[3]);
 }
 
-// 2^x for a pair on the FMA pipe, for -126 <= x < 128 (below: 2^-126): with n
-// the nearest integer, 2^x = 2^n p(x - n), p a polynomial fitted to the least
-// relative error on [-1/2, 1/2] (degree 3: 2^-13.7, for bf16 results; degree
-// 4: 2^-18.5, for fp16), n added to the exponent bits.  NaN gives 2^-126: a
-// row with one has a reference that is NaN, and its other exponentials are NaN.
+// 2^x for a pair on the FMA pipe, for -126 <= x < 128: with n the nearest
+// integer, 2^x = 2^n p(x - n), p a polynomial fitted to the least relative
+// error on [-1/2, 1/2] (degree 3: 2^-13.7, for bf16 results; degree 4: 2^-18.5,
+// for fp16), n added to the exponent bits.  Below -126 the sum falls among the
+// subnormals: less than 2^-126, and from just above -127 down below 2^-138,
+// which either type rounds to 0 (a value of 2^127 behind it counts for nothing).
+// There x is held just above -127, where p is just above 1: at 1 or below, the
+// sum would borrow from the sign.  NaN gives the same: a row with one has a
+// reference that is NaN, and its other exponentials are NaN.
 template <bool BF16>
 __device__ __forceinline__ uint64_t exp2_poly_x2(uint64_t x2) {
   const float2 x = f32x2_parts(x2);
   constexpr float kRound = 12582912.f;  // 1.5 * 2^23: the sum's low bits are the nearest integer
-  const uint64_t v = f32x2(fmaxf(x.x, -126.f), fmaxf(x.y, -126.f));
+  constexpr float kLeast = -126.9998f;  // p is 1.00006 (degree 3), 1.00014 (degree 4) there
+  const uint64_t v = f32x2(fmaxf(x.x, kLeast), fmaxf(x.y, kLeast));
   const uint64_t t = add_x2(v, f32x2(kRound, kRound));
   const uint64_t n = add_x2(t, f32x2(-kRound, -kRound));
   const uint64_t r = fma_x2(n, f32x2(-1.f, -1.f), v);

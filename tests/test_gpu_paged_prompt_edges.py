@@ -228,3 +228,25 @@ def test_prefixes_whose_values_jump(dev, form, ratio):
 def test_half_precision_rows_whose_values_jump(dev, form, own):
     """Scales of 11 significant bits, as rows appended in fp16 have them."""
     values_that_jump(dev, form, 2.0 ** 10, own, dtype=torch.float16)
+
+
+# ---- infinite scores, huge values ----------------------------------------------------
+
+
+def test_prompt_huge_value_behind_a_negligible_score(dev):
+    """exp(-300) times the largest bf16 value is 0, wherever the key lies in its block."""
+    from b200flash.paged_prompt import prompt_attention
+
+    n = 256
+    q, k, v, cu = packed(dev, [n] * 128, 2, 1, 64, "bf16", seed=12)
+    at = torch.arange(128, device=dev) * (n + 1)  # key i of sequence i
+    q[:, :, 0], k[:, :, 0] = 16.0, 0.0
+    k[at, 0, 0] = -150.0  # a score of -300
+    v[at] = 3e38
+    out = prompt_attention(q, k, v, cu, causal=False, softmax_scale=0.125)
+    for b in (0, 5, 6, 7, 62, 70, 126, 127):
+        s = slice(b * n, (b + 1) * n)
+        keep = [i for i in range(n) if i != b]
+        k2, v2 = k[s][keep], v[s][keep]
+        o, o_abs, _ = attend_reference(q[s], k2, v2, False, 0.125)
+        within(out[s], o, HALF_ULP[torch.bfloat16] * (o.abs() + o_abs) + 1e-6, f"key {b}")
