@@ -826,7 +826,8 @@ int b2f_qk_norm_rope_rows(const void* qkv, int64_t ld, int dtype, int64_t T, int
  * [cu_seqlens[b], cu_seqlens[b+1]) (int32 [B+1], from 0, at most T).  With
  * causal, a row sees its sequence up to itself.  out [T, Hq, D] of `dtype`;
  * rows past the last sequence are 0.  lse (float32 [T, Hq] or NULL): natural
- * log of each row's sum of exp(score), -inf where a row sees nothing.
+ * log of each row's sum of exp(score), -inf where a row sees nothing.  A row
+ * whose scores are all -inf is NaN (0 / 0), its lse -inf.
  * D a multiple of 8 up to 128; Hq/Hkv up to 128. */
 int b2f_prompt_attn(const void* q, int64_t q_row, int64_t q_head, const void* k, int64_t k_row,
                     int64_t k_head, const void* v, int64_t v_row, int64_t v_head, int dtype,

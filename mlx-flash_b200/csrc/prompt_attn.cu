@@ -646,7 +646,8 @@ __global__ void __launch_bounds__(PA_THREADS, 1) prompt_attn_kernel(const Prompt
         tc_fence_after();
         l = joined(l);  // (the last product needed every thread's P: all maxima have been read)
         const int64_t row = int64_t(x.row0 + t) * p.Hq + x.hk * p.G + rh;
-        const float inv = l > 0.f ? 1.f / l : l;  // l is NaN where a score is
+        // NaN where a score is (l is), and where all scores are -inf (a row sees its own key at least)
+        const float inv = m == -INFINITY ? __int_as_float(0x7fffffff) : 1.f / l;
         const bool any_bad = *const_cast<volatile int*>(&sm.any_bad[slot]) != 0;
         const int seen = t - x.mask * PA_BN;  // keys up to here, from the first masked block
         // a whole tile leaves through the ring stage that the planner grants it
@@ -695,7 +696,7 @@ __global__ void __launch_bounds__(PA_THREADS, 1) prompt_attn_kernel(const Prompt
           }
           if (staged) fence_proxy_async_smem();
           if (live && p.lse && h == 0)
-            p.lse[row] = l > 0.f ? (m + log2f(l)) * 0.6931471805599453f : l == 0.f ? -INFINITY : l;
+            p.lse[row] = m == -INFINITY ? m : (m + log2f(l)) * 0.6931471805599453f;
         }
         tc_fence_before();
         __syncwarp();

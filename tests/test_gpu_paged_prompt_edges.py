@@ -233,6 +233,27 @@ def test_half_precision_rows_whose_values_jump(dev, form, own):
 # ---- infinite scores, huge values ----------------------------------------------------
 
 
+@pytest.mark.parametrize("dt", ["bf16", "f16"])
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("D", [64, 128])
+def test_prompt_rows_whose_scores_are_all_minus_infinity(dev, D, causal, dt):
+    """The formula gives NaN there, whether or not a block has masked keys; their lse is -inf; other rows are as ever."""
+    from b200flash.paged_prompt import prompt_attention
+
+    lens = [256, 300, 128]
+    q, k, v, cu = packed(dev, lens, 4, 2, D, dt, seed=D)
+    q[:, 0, 0], q[:, 2, 0] = 2.0, 2.0
+    q[:, 1, 0], q[:, 3, 0] = 0.0, 0.0
+    clean = k.clone()
+    k[256:556, :, 0] = -math.inf
+    out, lse = prompt_attention(q, k, v, cu, causal=causal, return_lse=True)
+    want = prompt_attention(q, clean, v, cu, causal=causal)
+    for s in (slice(0, 256), slice(556, 684)):
+        assert torch.equal(out[s], want[s])
+    assert bool(out[256:556].isnan().all())  # heads 1 and 3: 0 * inf
+    assert bool((lse[256:556, 0::2] == -math.inf).all())
+
+
 def test_prompt_huge_value_behind_a_negligible_score(dev):
     """exp(-300) times the largest bf16 value is 0, wherever the key lies in its block."""
     from b200flash.paged_prompt import prompt_attention
