@@ -708,7 +708,7 @@ struct CombineParams {
   const float *o_prefix, *ml_prefix;  // [CTA][256][D] and (m, l), as prefix_attn_kernel leaves them
   const float *o_own, *ml_own;        // [B * Hq][n_own][D] and (m, l)
   const int* quota;
-  const int32_t *off, *lens;
+  const int32_t *off, *lens, *own_lens;
   __nv_bfloat16* out;
   int Ng, B, Hq, Hkv, tpt, max_prefix, n_own, ctas;
 };
@@ -791,7 +791,9 @@ __global__ void __launch_bounds__(256) prefix_combine_kernel(const CombineParams
       }
     }
   }
-  const float inv = l != 0.f ? 1.f / l : 0.f;
+  float inv = l != 0.f ? 1.f / l : 0.f;
+  // all scores are -inf: 0 / 0 (NaN maxima, which the comparisons pass over, come with sums that are NaN)
+  if (top == -INFINITY && (sp > 0 || (p.n_own > 0 && p.own_lens[b] > 0))) inv = __int_as_float(0x7fffffff);
   uint32_t y[V / 2];
 #pragma unroll
   for (int e = 0; e < V / 2; ++e) y[e] = pack_bf16x2(acc[2 * e] * inv, acc[2 * e + 1] * inv);
@@ -923,7 +925,7 @@ int b2f_shared_prefix_attn(const void* q, const uint8_t* k_pages, const float* k
                  : launch_prefix_bits<128>(p, bits, unsigned(ctas), st);
     if (rc != B2F_OK) return rc;
   }
-  const CombineParams c{o_prefix, ml_prefix, o_own, ml_own, quota, group_offsets, prefix_lens,
+  const CombineParams c{o_prefix, ml_prefix, o_own, ml_own, quota, group_offsets, prefix_lens, seq_lens,
                         static_cast<__nv_bfloat16*>(out), ctas > 0 ? int(n_groups) : 0, int(B), int(Hq), int(Hkv),
                         int(tpt), int(max_prefix), no, int(ctas)};
   return launch_kernel(D == 64 ? prefix_combine_kernel<64> : prefix_combine_kernel<128>,

@@ -271,3 +271,33 @@ def test_prompt_huge_value_behind_a_negligible_score(dev):
         k2, v2 = k[s][keep], v[s][keep]
         o, o_abs, _ = attend_reference(q[s], k2, v2, False, 0.125)
         within(out[s], o, HALF_ULP[torch.bfloat16] * (o.abs() + o_abs) + 1e-6, f"key {b}")
+
+
+@pytest.mark.parametrize("n_pre,n_own", [(256, 0), (300, 0), (256, 40), (0, 40), (0, 128), (100, 3)])
+@pytest.mark.parametrize("D,bits,Hq", [(128, 8, 4), (64, 8, 4), (128, 4, 16)])
+def test_shared_prefix_rows_whose_scores_are_all_minus_infinity(dev, D, bits, Hq, n_pre, n_own):
+    """NaN, as the formula gives; with one finite score the rest weighs nothing."""
+    from b200flash.paged_prompt import shared_prefix_attention
+
+    page = 64
+    g = torch.Generator(device=dev).manual_seed(n_pre + n_own)
+    npp, npo = -(-n_pre // page), -(-n_own // page)
+    kc, ks, _, _ = paged_rows(dev, [(npp + npo + 1) * page], 1, D, bits, page, g)
+    vc, vs, _, _ = paged_rows(dev, [(npp + npo + 1) * page], 1, D, bits, page, g)
+    kc.fill_({8: 100, 4: 0x33}[bits])  # below the code of 0
+    ks.fill_(math.inf)
+    q = torch.rand(2, Hq, D, device=dev, generator=g).add(0.5).to(torch.bfloat16)
+    i32 = dict(dtype=torch.int32, device=dev)
+    pre = torch.arange(npp, **i32)[None] if npp else torch.zeros(1, 1, **i32)
+    own = (npp + torch.arange(npo, **i32)).expand(2, npo).contiguous() if npo else torch.zeros(2, 1, **i32)
+
+    def run():
+        return shared_prefix_attention(q, kc, ks, vc, vs, pre, torch.tensor([n_pre], **i32), torch.tensor([0, 2], **i32),
+                                       own, torch.full((2,), n_own, **i32), bits, page, 1)
+
+    assert bool(run().isnan().all())
+    p, s = (npp + (n_own - 1) // page, (n_own - 1) % page) if n_own else ((n_pre - 1) // page, (n_pre - 1) % page)
+    ks[p, 0, s] = 0.01
+    c = vc[p, 0, s] if bits == 8 else torch.stack([vc[p, 0, s] >> 4, vc[p, 0, s] & 15], -1).flatten()
+    want = ((c.double() - (2 ** (bits - 1) - 1)).view(-1, 64) * vs[p, 0, s].double()[:, None]).flatten()
+    within(run(), want.expand(2, Hq, D), 2.0 ** -8 * want.abs().expand(2, Hq, D) * 2 + 1e-6)
