@@ -10,11 +10,11 @@ lengths is one packed run of rows:
 * :func:`prompt_attention`         attention of each packed sequence over itself, causal or full
 * :func:`shared_prefix_attention`  decode rows that share long prefixes, each prefix read once for its group
 
-All are stream-ordered on the current stream, never wait for the host, and can
-be captured in a CUDA graph.
+All are stream-ordered on the current stream and can be captured in a CUDA
+graph.  None waits for the host, but for the first :func:`qk_norm_rope` with a
+rotary base, which copies its frequencies from there (not inside a capture).
 """
 
-import functools
 from typing import NamedTuple, Optional
 
 import torch
@@ -88,11 +88,25 @@ def plan_pages(new_lens: torch.Tensor, free_pages: torch.Tensor, page_size: int,
     return out
 
 
-@functools.lru_cache(maxsize=32)
+# Kernels in flight and captured graphs hold the addresses of these: none is ever dropped.
+_frequencies = {}
+
+
 def rope_frequencies(rotary_dim: int, theta: float, device) -> torch.Tensor:
-    """``theta ** (-2 i / rotary_dim)`` for ``i < rotary_dim / 2``, float64 on ``device`` (kept per argument)."""
-    return torch.tensor([theta ** (-2.0 * i / rotary_dim) for i in range(rotary_dim // 2)], dtype=torch.float64,
-                        device=device)
+    """``theta ** (-2 i / rotary_dim)`` for ``i < rotary_dim / 2``, float64 on ``device`` (kept per argument).
+
+    A first call inside a capture forms them on the device, in the graph, and
+    keeps none: their memory is the graph's.
+    """
+    key = (rotary_dim, theta, device)
+    got = _frequencies.get(key)
+    if got is None:
+        if torch.device(device).type == "cuda" and torch.cuda.is_current_stream_capturing():
+            i = torch.arange(rotary_dim // 2, dtype=torch.float64, device=device)
+            return torch.pow(theta, i * (-2.0 / rotary_dim))
+        got = _frequencies[key] = torch.tensor([theta ** (-2.0 * i / rotary_dim) for i in range(rotary_dim // 2)],
+                                               dtype=torch.float64, device=device)
+    return got
 
 
 def qk_norm_rope(qkv: torch.Tensor, n_heads: int, n_kv_heads: int, positions: torch.Tensor, q_norm: torch.Tensor,
