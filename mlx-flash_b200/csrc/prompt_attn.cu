@@ -188,6 +188,16 @@ __global__ void __launch_bounds__(PA_THREADS, 1) prompt_attn_kernel(const Prompt
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
   for (int i = tid; i < 2 * DP; i += PA_THREADS) sm.bad[i / DP][i % DP] = PA_NO_BAD;
+  // Where the heads of a group do not divide 128, no load touches the last rows
+  // of a Q tile: zeros, for whatever lay there before could send their warps
+  // through the rescale in every block.
+  if (const int rows = p.tpt * p.G; rows < 128) {
+    for (int i = tid; i < 2 * (DP / 64) * 8 * (128 - rows); i += PA_THREADS) {
+      const int part = i / (8 * (128 - rows)), at = i % (8 * (128 - rows));  // tile and 64 columns, 16 bytes
+      reinterpret_cast<uint4*>(sm.q[0] + part * HALF + rows * 128)[at] = make_uint4(0u, 0u, 0u, 0u);
+    }
+    fence_proxy_async_smem();
+  }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();

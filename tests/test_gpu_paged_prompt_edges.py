@@ -301,3 +301,20 @@ def test_shared_prefix_rows_whose_scores_are_all_minus_infinity(dev, D, bits, Hq
     c = vc[p, 0, s] if bits == 8 else torch.stack([vc[p, 0, s] >> 4, vc[p, 0, s] & 15], -1).flatten()
     want = ((c.double() - (2 ** (bits - 1) - 1)).view(-1, 64) * vs[p, 0, s].double()[:, None]).flatten()
     within(run(), want.expand(2, Hq, D), 2.0 ** -8 * want.abs().expand(2, Hq, D) * 2 + 1e-6)
+
+
+@pytest.mark.parametrize("Hq,Hkv,D", [(24, 8, 128), (12, 1, 128), (24, 1, 64), (14, 2, 80)])
+def test_prompt_groups_that_do_not_divide_a_tile(dev, Hq, Hkv, D):
+    """Whatever an earlier call left in shared memory (here NaN queries), the rows of a tile that no head fills stay out."""
+    from b200flash.paged_prompt import prompt_attention
+
+    lens = [700, 300, 1]
+    q, k, v, cu = packed(dev, lens, Hq, Hkv, D, "bf16", seed=Hq)
+    nan = torch.full((8192, 32, 128), math.nan, dtype=torch.bfloat16, device=dev)
+    kn = torch.zeros(8192, 4, 128, dtype=torch.bfloat16, device=dev)
+    first = prompt_attention(q, k, v, cu, causal=False)
+    prompt_attention(nan, kn, kn, torch.tensor([0, 8192], dtype=torch.int32, device=dev))
+    assert torch.equal(prompt_attention(q, k, v, cu, causal=False), first)
+    for s in (slice(0, 700), slice(700, 1000)):
+        o, o_abs, _ = attend_reference(q[s], k[s], v[s], False, D ** -0.5)
+        within(first[s], o, HALF_ULP[q.dtype] * (o.abs() + o_abs) + 1e-6)
