@@ -18,6 +18,7 @@ read once for all requests behind it, and their own tokens
 (``shared_prefix_attention``).
 """
 
+import contextlib
 from typing import Sequence
 
 import torch
@@ -42,6 +43,7 @@ class SharedPromptBatch:
         self.prefix_table = torch.zeros(0, 1, dtype=torch.int32, device=self.device)
         self.prefix_lens = torch.zeros(0, dtype=torch.int32, device=self.device)
         self.own_lens = []
+        self._own_pages = []  # of the started requests, a tensor per step that took some
 
     # -- pages ------------------------------------------------------------------
     def _pages(self, tokens: int) -> int:
@@ -52,6 +54,16 @@ class SharedPromptBatch:
             raise RuntimeError(f"{pages} pages wanted, {self._free.shape[0]} free")
         taken, self._free = self._free[:pages], self._free[pages:]
         return taken
+
+    @contextlib.contextmanager
+    def _given_back(self):
+        """Pages taken inside the block are free again if it raises."""
+        before = self._free
+        try:
+            yield
+        except BaseException:
+            self._free = before
+            raise
 
     # -- the layers ---------------------------------------------------------------
     def _forward(self, tokens, positions, slots, attend, out_rows):
@@ -97,11 +109,12 @@ class SharedPromptBatch:
         i32 = dict(dtype=torch.int32, device=self.device)
         table = torch.zeros(len(lens), max(self._pages(n) for n in lens), **i32)
         new_lens = torch.tensor(lens, **i32)
-        plan = plan_pages(new_lens, self._take(sum(self._pages(n) for n in lens)), self.page, T, table)
         tokens = torch.tensor([t for p in prompts for t in p], **i32)
-        logits = self._forward(tokens, plan.positions, plan.slots,
-                               lambda q, k, v, kv: prompt_attention(q, k, v, plan.cu_seqlens),
-                               plan.cu_seqlens[1:].long() - 1)
+        with self._given_back():
+            plan = plan_pages(new_lens, self._take(sum(self._pages(n) for n in lens)), self.page, T, table)
+            logits = self._forward(tokens, plan.positions, plan.slots,
+                                   lambda q, k, v, kv: prompt_attention(q, k, v, plan.cu_seqlens),
+                                   plan.cu_seqlens[1:].long() - 1)
         self.prompt_lens += lens
         both = torch.zeros(len(self.prompt_lens), max(table.shape[1], self.prefix_table.shape[1]), **i32)
         both[: self.prefix_table.shape[0], : self.prefix_table.shape[1]] = self.prefix_table
@@ -113,11 +126,14 @@ class SharedPromptBatch:
     # -- requests -----------------------------------------------------------------
     def start(self, prompt_of: Sequence[int], max_own: int = 1024):
         """Start one request per entry, behind the prompt of that index (in
-        rising order), each with room for ``max_own`` tokens of its own."""
+        rising order), each with room for ``max_own`` tokens of its own.
+        Requests that were started before end, and give their pages back."""
         n = len(self.prompt_lens)
         if any(p < 0 or p >= n for p in prompt_of) or list(prompt_of) != sorted(prompt_of):
             raise ValueError(f"requests name prompts 0..{n - 1} in rising order")
         i32 = dict(dtype=torch.int32, device=self.device)
+        self._free = torch.cat([self._free] + self._own_pages)
+        self._own_pages = []
         self.max_own = max_own
         self.own_lens = [0] * len(prompt_of)
         self._lens = torch.zeros(len(prompt_of), **i32)
@@ -133,16 +149,21 @@ class SharedPromptBatch:
             raise ValueError(f"step takes one token for each of the {B} requests")
         if max(self.own_lens) >= self.max_own:
             raise RuntimeError(f"a request has used its {self.max_own} tokens")
-        pages = sum(n % self.page == 0 for n in self.own_lens)
-        plan = plan_pages(self._one, self._take(pages), self.page, B, self._table, context_lens=self._lens)
-        self._lens = plan.seq_lens
-        self.own_lens = [n + 1 for n in self.own_lens]
+        own_lens = [n + 1 for n in self.own_lens]
         s = self.dec.s
 
         def attend(q, k, v, kv):
             return shared_prefix_attention(q, kv["kc"], kv["ks"], kv["vc"], kv["vs"], self.prefix_table,
-                                           self.prefix_lens, self._groups, self._table, self._lens, s.kv_bits, self.page,
-                                           s.n_kv_heads, max_prefix_len=max(self.prompt_lens),
-                                           max_seq_len=max(self.own_lens))
+                                           self.prefix_lens, self._groups, self._table, plan.seq_lens, s.kv_bits,
+                                           self.page, s.n_kv_heads, max_prefix_len=max(self.prompt_lens),
+                                           max_seq_len=max(own_lens))
 
-        return self._forward(tokens.to(torch.int32), plan.positions + self._base, plan.slots, attend, None)
+        with self._given_back():
+            pages = self._take(sum(n % self.page == 0 for n in self.own_lens))
+            plan = plan_pages(self._one, pages, self.page, B, self._table, context_lens=self._lens)
+            logits = self._forward(tokens.to(torch.int32), plan.positions + self._base, plan.slots, attend, None)
+        # a step that failed leaves nothing behind: its pages, table entries and rows are written again
+        if pages.shape[0]:
+            self._own_pages.append(pages)
+        self._lens, self.own_lens = plan.seq_lens, own_lens
+        return logits
