@@ -30,11 +30,19 @@ from .paged_prompt import plan_pages, prompt_attention, qk_norm_rope, shared_pre
 
 
 class SharedPromptBatch:
-    """Packed prompts and the requests that decode behind them (one GPU)."""
+    """Packed prompts and the requests that decode behind them (one GPU).
+
+    The decoder's whole page pool is the batch's from here on: the decoder's
+    own rows hold none (a decoder whose rows do is refused), and neither its
+    ``step`` nor another batch runs over it meanwhile.
+    """
 
     def __init__(self, decoder):
         if decoder.world != 1:
             raise ValueError("SharedPromptBatch serves a decoder that holds all of its experts")
+        if bool((torch.maximum(decoder.positions, decoder.seq_lens) > 0).any()):
+            raise ValueError("the decoder's rows hold tokens in the pages that SharedPromptBatch would write to; zero its "
+                             "positions and seq_lens to give them up")
         self.dec = decoder
         self.page = decoder.page
         self.device = decoder.dev

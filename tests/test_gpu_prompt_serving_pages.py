@@ -57,3 +57,16 @@ def test_requests_that_end_give_their_pages_back(dev):
             assert torch.equal(batch.step(tokens), out[1 + t])
         assert batch._free.shape[0] == left
     assert len(set(batch._free.tolist())) == left
+
+
+def test_a_decoder_in_use_is_refused(dev):
+    dec = Qwen3MoeDecoder(SHAPE, max_batch=2, max_context=64, page_size=16, device=dev, seed=5)
+    dec.step()
+    with pytest.raises(ValueError, match="hold tokens"):
+        SharedPromptBatch(dec)
+    dec.seq_lens.zero_()
+    dec.positions.zero_()
+    SharedPromptBatch(dec)
+    dec.fill_random_context(40)
+    with pytest.raises(ValueError, match="hold tokens"):
+        SharedPromptBatch(dec)
