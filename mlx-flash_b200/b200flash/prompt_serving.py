@@ -110,6 +110,8 @@ class SharedPromptBatch:
         the bf16 ``[len(prompts), vocab]`` logits after each one's last token."""
         if not prompts or any(len(p) == 0 for p in prompts):
             raise ValueError("prompts must be non-empty token lists")
+        if not all(0 <= t < self.dec.s.vocab for p in prompts for t in p):
+            raise ValueError(f"tokens must lie in 0..{self.dec.s.vocab - 1}: they index the embedding")
         if self.own_lens:
             raise ValueError("prompts are added before the requests start")
         lens = [len(p) for p in prompts]
@@ -151,7 +153,7 @@ class SharedPromptBatch:
         self._table = torch.zeros(len(prompt_of), self._pages(max_own), **i32)
 
     def step(self, tokens: torch.Tensor) -> torch.Tensor:
-        """One token of each request (int32 ``[B]``) -> bf16 logits ``[B, vocab]``."""
+        """One token of each request (int32 ``[B]``, each below ``vocab``) -> bf16 logits ``[B, vocab]``."""
         B = len(self.own_lens)
         if B == 0 or tuple(tokens.shape) != (B,):
             raise ValueError(f"step takes one token for each of the {B} requests")

@@ -70,3 +70,11 @@ def test_a_decoder_in_use_is_refused(dev):
     dec.fill_random_context(40)
     with pytest.raises(ValueError, match="hold tokens"):
         SharedPromptBatch(dec)
+
+
+@pytest.mark.parametrize("bad", [-1, SHAPE.vocab, 1 << 40])
+def test_tokens_outside_the_vocabulary_are_refused(dev, bad):
+    batch = batch_of(dev)
+    with pytest.raises(ValueError, match="tokens must lie"):
+        batch.add_prompts([[1, 2], [3, bad]])
+    assert batch._free.shape[0] == batch.dec.num_pages
