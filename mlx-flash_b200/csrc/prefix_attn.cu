@@ -841,11 +841,11 @@ static int own_splits(int64_t B, int64_t Hkv, int64_t max_own) {
 }
 
 // CTAs of the prefix kernel, each with room for the partials of its two tiles:
-// a partial pair of tiles per group at most, and more splits than one only
-// while they fit the SMs.
+// a partial pair of tiles at most per group with rows, of which there are no
+// more than rows, and more splits than one only while they fit the SMs.
 static int64_t prefix_ctas(int64_t B, int64_t G, int64_t Hkv, int64_t Ng, int64_t max_prefix) {
   if (Ng <= 0 || max_prefix <= 0 || B <= 0) return 0;
-  const int64_t n = (B / (2 * (128 / G)) + Ng) * Hkv;
+  const int64_t n = (B / (2 * (128 / G)) + (Ng < B ? Ng : B)) * Hkv;
   return n > PX_SMS ? n : PX_SMS;
 }
 

@@ -318,3 +318,28 @@ def test_prompt_groups_that_do_not_divide_a_tile(dev, Hq, Hkv, D):
     for s in (slice(0, 700), slice(700, 1000)):
         o, o_abs, _ = attend_reference(q[s], k[s], v[s], False, D ** -0.5)
         within(first[s], o, HALF_ULP[q.dtype] * (o.abs() + o_abs) + 1e-6)
+
+
+def test_shared_prefix_many_prefixes_few_requests(dev):
+    """Thousands of prefixes, requests behind a few of them: all but their groups are empty."""
+    from b200flash.paged_prompt import shared_prefix_attention
+
+    Hq, Hkv, D, page, n = 8, 2, 128, 16, 3000
+    g = torch.Generator(device=dev).manual_seed(13)
+    at = [5, 5, 700, 2999]  # the prefix of each request
+    pre = [(i * 37) % 48 + 1 for i in range(n)]
+    kc, ks, table, kv = paged_rows(dev, [48] * 8 + [20] * 4, Hkv, D, 8, page, g)
+    vc, vs, _, _ = paged_rows(dev, [48] * 8 + [20] * 4, Hkv, D, 8, page, g)
+    i32 = dict(dtype=torch.int32, device=dev)
+    q = torch.randn(4, Hq, D, device=dev, generator=g).to(torch.bfloat16)
+    prefix = table[torch.arange(n, device=dev) % 8].contiguous()
+    off = torch.tensor([sum(p < i for p in at) for i in range(n + 1)], **i32)
+    lens = torch.tensor([20, 0, 7, 16], **i32)
+    out = shared_prefix_attention(q, kc, ks, vc, vs, prefix, torch.tensor(pre, **i32), off, table[8:].contiguous(), lens, 8,
+                                  page, Hkv)
+    for b, p in enumerate(at):  # the same request alone
+        want = shared_prefix_attention(q[b: b + 1], kc, ks, vc, vs, prefix[p: p + 1], torch.tensor([pre[p]], **i32),
+                                       torch.tensor([0, 1], **i32), table[8 + b: 9 + b].contiguous(), lens[b: b + 1], 8, page,
+                                       Hkv)
+        # other splits: float32 sums in another order, so the two may round to neighbours
+        within(out[b], want[0].double(), 2.0 ** -7 * want[0].double().abs() + 1e-4)
