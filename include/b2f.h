@@ -848,7 +848,7 @@ int64_t b2f_shared_prefix_attn_workspace_bytes(int64_t B, int64_t Hq, int64_t Hk
  * no prefix.  A prefix is read and decoded once for its group.  out bf16
  * [B, Hq, D]; a row that sees nothing is 0, one whose scores are all -inf NaN.
  * max_prefix / max_own: upper bounds of the lengths (they size the splits;
- * longer lengths are cut).  A table entry below 0 (a page that b2f_page_plan
+ * longer lengths are cut; with 0 the table may be NULL).  A table entry below 0 (a page that b2f_page_plan
  * could not give) reads page 0.  D in {64, 128}; bits in {2, 4, 8}; group_size 64; Hq/Hkv <= 16; page_size
  * a multiple of 16. */
 int b2f_shared_prefix_attn(const void* q, const uint8_t* k_pages, const float* k_scales,

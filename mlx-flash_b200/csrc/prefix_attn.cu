@@ -886,8 +886,8 @@ int b2f_shared_prefix_attn(const void* q, const uint8_t* k_pages, const float* k
   if (page_size > (1 << 20) || prefix_pages * page_size > (int64_t(1) << 30) || max_pages * page_size > (int64_t(1) << 30))
     return B2F_ERR_UNSUPPORTED;
   if (B == 0) return B2F_OK;
-  if (!q || !k_pages || !k_scales || !v_pages || !v_scales || !block_table || !seq_lens || !out ||
-      (n_groups > 0 && (!prefix_table || !prefix_lens || !group_offsets)))
+  if (!q || !k_pages || !k_scales || !v_pages || !v_scales || !seq_lens || !out || (max_own > 0 && !block_table) ||
+      (n_groups > 0 && (!prefix_lens || !group_offsets || (max_prefix > 0 && !prefix_table))))
     return B2F_ERR_INVALID;
   if (!aligned(q, 16) || !aligned(k_pages, 16) || !aligned(v_pages, 16) || !aligned(k_scales, 16) ||
       !aligned(v_scales, 16) || !aligned(out, 16))

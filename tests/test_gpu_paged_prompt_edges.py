@@ -343,3 +343,24 @@ def test_shared_prefix_many_prefixes_few_requests(dev):
                                        Hkv)
         # other splits: float32 sums in another order, so the two may round to neighbours
         within(out[b], want[0].double(), 2.0 ** -7 * want[0].double().abs() + 1e-4)
+
+
+def test_shared_prefix_tables_without_columns(dev):
+    """No request has tokens of its own yet, or no prefix has any: tables of no pages."""
+    from b200flash.paged_prompt import shared_prefix_attention
+
+    g = torch.Generator(device=dev).manual_seed(14)
+    kc, ks, table, _ = paged_rows(dev, [90, 40, 7], 2, 128, 8, 16, g)
+    vc, vs, _, _ = paged_rows(dev, [90, 40, 7], 2, 128, 8, 16, g)
+    q = torch.randn(2, 8, 128, device=dev, generator=g).to(torch.bfloat16)
+    i32 = dict(dtype=torch.int32, device=dev)
+
+    def run(prefix, n_pre, own, n_own):
+        return shared_prefix_attention(q, kc, ks, vc, vs, prefix, torch.tensor([n_pre], **i32), torch.tensor([0, 2], **i32),
+                                       own, torch.tensor(n_own, **i32), 8, 16, 2)
+
+    none = torch.zeros(2, 0, **i32)
+    pre, own = table[:1].contiguous(), table[1:].contiguous()
+    assert torch.equal(run(pre, 90, none, [0, 0]), run(pre, 90, own, [0, 0]))
+    assert torch.equal(run(none[:1], 0, own, [40, 7]), run(pre, 0, own, [40, 7]))
+    assert bool((run(none[:1], 0, none, [0, 0]) == 0).all())
