@@ -364,3 +364,39 @@ def test_shared_prefix_tables_without_columns(dev):
     assert torch.equal(run(pre, 90, none, [0, 0]), run(pre, 90, own, [0, 0]))
     assert torch.equal(run(none[:1], 0, own, [40, 7]), run(pre, 0, own, [40, 7]))
     assert bool((run(none[:1], 0, none, [0, 0]) == 0).all())
+
+
+# ---- shared prefixes: scales of the softmax against the formula ----------------------
+
+
+@pytest.mark.parametrize("scale", [-0.07, 0.0, 0.5, 1e-12])
+@pytest.mark.parametrize("form", FORMS)
+def test_shared_prefix_scales_of_the_softmax(dev, form, scale):
+    """Prefix and own tokens under softmax scales of either sign and 0, at the bound of run_prefix."""
+    from b200flash.paged_prompt import shared_prefix_attention
+
+    Hq, Hkv, D, bits, page = form
+    g = torch.Generator(device=dev).manual_seed(D + bits)
+    n_pre, n_own = 200, [40, 0, 7]
+    rows = [(torch.randn(n, Hkv, D, device=dev, generator=g).to(torch.bfloat16),
+             torch.randn(n, Hkv, D, device=dev, generator=g).to(torch.bfloat16)) for n in [n_pre] + n_own]
+    kc, ks, vc, vs, tables, vals, at = [], [], [], [], [], [], 0
+    for k, v in rows:
+        c, s, kv = cache_of(k, bits, page)
+        d, t, vv = cache_of(v, bits, page)
+        kc.append(c), ks.append(s), vc.append(d), vs.append(t)
+        tables.append(list(range(at, at + c.shape[0])))
+        vals.append((kv, vv))
+        at += c.shape[0]
+    i32 = dict(dtype=torch.int32, device=dev)
+    width = max(len(t) for t in tables)
+    table = torch.tensor([t + [0] * (width - len(t)) for t in tables], **i32)
+    q = torch.randn(3, Hq, D, device=dev, generator=g).to(torch.bfloat16)
+    out = shared_prefix_attention(q, torch.cat(kc), torch.cat(ks), torch.cat(vc), torch.cat(vs), table[:1].contiguous(),
+                                  torch.tensor([n_pre], **i32), torch.tensor([0, 3], **i32), table[1:].contiguous(),
+                                  torch.tensor(n_own, **i32), bits, page, Hkv, softmax_scale=scale)
+    for b in range(3):
+        k, v = (torch.cat([vals[0][i], vals[1 + b][i]]) for i in (0, 1))
+        o, o_abs, _ = attend_reference(q[b][None], k, v, False, scale)
+        move = 2.0 ** -11 * torch.einsum("hd,mhd->hm", q[b].double().abs(), k.abs().repeat_interleave(Hq // Hkv, 1)).amax(-1)
+        within(out[b], o[0], 2.0 ** -8 * (o[0].abs() + o_abs[0]) + 2 * abs(scale) * move[:, None] * o_abs[0] + 1e-6, f"row {b}")
