@@ -190,8 +190,8 @@ def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqle
 
     ``q`` bf16 or fp16 ``[T, Hq, D]``, ``k`` / ``v`` ``[T, Hkv, D]`` (views of
     packed projections are taken as they are), ``D`` a multiple of 8 up to
-    128; sequence ``b`` is rows ``cu_seqlens[b]:cu_seqlens[b + 1]`` (int32).
-    Rows past the last sequence come out 0.  With ``return_lse`` also the
+    128; sequence ``b`` is rows ``cu_seqlens[b]:cu_seqlens[b + 1]`` (int32,
+    rising from 0).  Rows past the last sequence come out 0.  With ``return_lse`` also the
     float32 ``[T, Hq]`` log of each row's softmax sum.
     """
     dev = require_cuda(q, k, v, cu_seqlens)

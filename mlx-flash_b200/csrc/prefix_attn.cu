@@ -13,17 +13,18 @@
 //   3. combine: out = sum 2^(m_s - m) O_s / sum 2^(m_s - m) l_s over splits.
 //
 // What bounds it: the prefix kernel's start (plan, page table, first copies and
-// their decoding: 10000 cycles before the first scores), then instructions (16
-// softmax and 8 decoding warps, 2500 cycles a block of two tiles).  It is let
-// onto the SMs as the own tokens' CTAs leave them.  A split costs a start, and
+// their decoding: 10000 cycles before the first scores), then the chain of a
+// block (copy, decoding, scores, softmax, product): 5200 cycles a block of two
+// tiles in splits of 27, with half of the issue slots used.  It is let onto the
+// SMs as the own tokens' CTAs leave them.  A split costs a start, and
 // its partials are written and read: 8192 keys and 64 rows over 4 KV heads by
 // one CTA an SM against half as many 24 / 32 us, 20001 keys and 128 rows over
 // 8 KV heads 58 / 99 us.
 // Measured (own tokens, prefix, combine; 32 heads of 128): 64 rows behind 8192
-// tokens, up to 512 of their own, 4 KV heads 13.7 / 28.6 / 5.8 us, 44 us in
+// tokens, up to 512 of their own, 4 KV heads 12.8 / 28.2 / 5.8 us, 43 us in
 // all (29 MB, 8.9 GFLOP); 128 rows in two groups behind 20001 and 16906, up to
-// 2000 of their own, 8 KV heads 74 / 79 / 6 us, 137 us in all (354 MB, 40.5
-// GFLOP); 4 rows behind 500 tokens 5.5 / 10.1 / 3.6 us.
+// 2000 of their own, 8 KV heads 75 / 78 / 6 us, 141 us in all (354 MB, 40.5
+// GFLOP); 4 rows behind 500 tokens 5.0 / 10.2 / 3.8 us.
 //
 // fp16 operands: a code is exact in 11 bits, and scale * code costs one
 // rounding of 2^-11, where bf16 would cost 2^-8 on K, V and P each -- more than

@@ -38,15 +38,18 @@
 // it runs for long.  Heads of up to 64 leave TMEM columns for P beside S: the
 // next scores are then computed under the softmax, and the tensor core is no
 // longer in the chain; there tile 1 begins behind tile 0's first reading of
-// its scores, so that their exponentials take turns (53 -> 49 us).  At 128
-// columns of O per tile P lies over S.  The longest sequences go first where a
-// warp holds them all (up to 31): 4 sequences of up to 1500 tokens, 28 blocks
-// on the busiest SM against 22.
-// Measured (kernel): 32 heads of 128, 4 KV heads, causal: 16384 tokens 1.71 ms,
-// 1.29 PFLOP/s (2.0 ms back to back, where power holds the clock at 1.4 GHz);
-// 16 sequences of 1 to 2047 tokens 185 us, 0.89 PFLOP/s (an item has 6 blocks
-// on average and costs 1.3 more at its ends); 3 of up to 60 tokens 11 us.
-// 16 heads of 64 in full, 4 sequences of 616 to 1500: 48 us, 0.44 PFLOP/s.
+// its scores, so that their exponentials take turns (53 -> 49 us).  A block of
+// two tiles takes 4100 cycles there, of which the exponentials account for
+// 1536 (the unit is busy 39 % of the time, issue 51 %, the tensor core 26 %).
+// At 128 columns of O per tile P lies over S.  The longest sequences go first
+// where a warp holds them all (up to 31): 4 sequences of up to 1500 tokens, 28
+// blocks on the busiest SM against 22.
+// Measured (kernel): 32 heads of 128, 4 KV heads, causal: 16384 tokens 1.69 to
+// 1.75 ms, 1.3 PFLOP/s (2.0 ms back to back, where power holds the clock at
+// 1.4 GHz); 16 sequences of 1 to 2047 tokens 185 to 192 us, 0.87 PFLOP/s (an
+// item has 6 blocks on average and costs 1.3 more at its ends); 3 of up to 60
+// tokens 11 us.
+// 16 heads of 64 in full, 4 sequences of 616 to 1500: 50 us, 0.42 PFLOP/s.
 //
 // A CTA (one per SM) takes item after item from the grid by cancelling CTAs
 // that have not been launched; the items' roles overlap: loads and the first

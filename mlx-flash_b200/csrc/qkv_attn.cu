@@ -13,7 +13,7 @@
 //               become fp16 1024+code with one prmt/lop3 per two values;
 //               per 64-wide group: s += kscale*(acc - (1024+max_int)*sum(q))
 //   online softmax in base 2 (q is pre-scaled by softmax_scale*log2(e))
-//   O += P.V    P from the S accumulators (FA2 register reuse), V codes
+//   O += P.V    P from the S accumulators, in registers; V codes
 //               decoded to fp16 (code-max_int)*vscale in registers.
 // Splits write (m, l, O) partials; a combine kernel merges them.
 #include "common.cuh"
