@@ -436,7 +436,7 @@ __global__ void __launch_bounds__(PX_THREADS, 1) prefix_attn_kernel(const Prefix
           const float norm = top > 0.f ? fminf(pow2_inverse(top, 15 - BITS), 0x1p60f) : 0x1p60f;
           sm.norm[v][j & 7] = careful ? -norm : norm;
           if (v) sm.v_power[j & 7] = make_float2(float(127 - int(__float_as_uint(norm) >> 23)), norm);
-          else sm.k_back[j & 7] = 1.f / norm;
+          else sm.k_back[j & 7] = __uint_as_float((254u << 23) - __float_as_uint(norm));  // 1 / norm
           mbar_arrive(&sm.norm_full[v][j & 3]);
         }
         __syncwarp();
